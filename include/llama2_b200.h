@@ -47,8 +47,9 @@ enum l2b_status {
     L2B_ERR_NO_DEVICE = 8
 };
 
-/* GGML tensor types the reference can load (src/load_gguf.jl:26-42,135-154), and bf16 for layer-stack models. */
-enum l2b_ggml_type { L2B_TYPE_F32 = 0, L2B_TYPE_Q4_K = 12, L2B_TYPE_Q5_K = 13, L2B_TYPE_Q6_K = 14, L2B_TYPE_BF16 = 30 };
+/* GGML tensor types the reference can load (src/load_gguf.jl:26-42,135-154), bf16 for layer-stack models, and f16 for paged
+ * caches, their rows and logits. */
+enum l2b_ggml_type { L2B_TYPE_F32 = 0, L2B_TYPE_F16 = 1, L2B_TYPE_Q4_K = 12, L2B_TYPE_Q5_K = 13, L2B_TYPE_Q6_K = 14, L2B_TYPE_BF16 = 30 };
 
 /* Tensor roles = the fields of TransformerWeights / TransformerLayerWeights
  * (src/inference.jl:27-48). */
@@ -289,6 +290,107 @@ int32_t l2b_swiglu(float* host_hb, const float* host_hb2, int64_t n);
 int32_t l2b_argmax(const float* host_logits, int64_t n, int32_t* index);
 /* logits ./= T; softmax!; wsample (src/inference.jl:361-368) with a supplied uniform in [0,1). */
 int32_t l2b_sample_temperature(const float* host_logits, int64_t n, float temperature, double uniform, int32_t* index);
+
+/* ---- paged cache: append, attention (no counterpart in the reference, whose KVCache is one array per sequence, src/inference.jl:62-70) -----------
+ * For callers that keep their sequences' keys and values themselves, in pages, and may let all of them begin with the same positions (a system
+ * prompt, a document) that are stored once.  All buffers are device memory of the caller's and all of one device, which need not be the current one; the
+ * calls allocate nothing, are asynchronous on `stream` (cudaStream_t; NULL = default) and may be captured into a graph.  The descriptors are read
+ * during the call only; what their pointers point to is read when the kernels run, so a captured call serves other lengths and pages later.
+ *
+ * Pages: dev_k, dev_v [n_pages][n_kv_heads][page_size][head_size]. */
+typedef struct l2b_paged_cache {
+    void* dev_k;
+    void* dev_v;
+    int32_t type;       /* L2B_TYPE_F16 or L2B_TYPE_BF16 */
+    int32_t n_pages;
+    int32_t page_size;  /* a power of two, 8 .. 1024 */
+    int32_t n_kv_heads;
+    int32_t head_size;  /* a multiple of 8, at most 128 */
+    int32_t reserved;
+} l2b_paged_cache;
+/* A batch has n_query rows of each sequence, in all row buffers: sequence i has rows i * n_query .., of which the first dev_counts[i] (all, where
+ * dev_counts is NULL) are new tokens.  The others are padding: nothing is written for them.
+ *   dev_lengths [n_seq]        the sequence's own positions, the new tokens' included, which are the last ones; negative: the sequence sits this step out;
+ *   dev_pages [n_seq][pages_per_seq]   the pages of own positions 0 .. page_size - 1, page_size .. and so on;
+ *   dev_prefix_pages           the pages of the prefix_len positions that lie in front of every sequence's own ones (the last may be partly filled).
+ * An entry outside 0 .. n_pages - 1 (-1, say) is no page: its positions are not attended and rows that would go there are not written.  So are
+ * positions behind pages_per_seq pages.  prefix_len + pages_per_seq * page_size is at most 2^31 - 1. */
+typedef struct l2b_paged_batch {
+    int32_t n_seq;
+    int32_t n_query;
+    const int32_t* dev_lengths;
+    const int32_t* dev_counts;
+    const int32_t* dev_pages;
+    int32_t pages_per_seq;
+    int32_t prefix_len;
+    const int32_t* dev_prefix_pages;
+} l2b_paged_batch;
+/* The rows of a batch as the projections leave them; strides in values from row to row (q, k and v may be parts of one product's rows).
+ * Rows and gains lie on 16-byte boundaries. */
+typedef struct l2b_paged_rows {
+    int32_t type;            /* of q, k, v and q_out: L2B_TYPE_F32, or the cache's type */
+    int32_t n_heads;         /* of q */
+    const void* dev_q;       /* [rows][n_heads][head_size]; NULL (with dev_q_out): keys and values only */
+    const void* dev_k;       /* [rows][n_kv_heads][head_size] */
+    const void* dev_v;
+    int64_t q_stride, k_stride, v_stride;
+    void* dev_q_out;         /* may be dev_q, with the same stride */
+    int64_t q_out_stride;
+    const float* dev_q_gain; /* [head_size], rms norm of every query head; NULL: none */
+    const float* dev_k_gain;
+    float eps;
+    float rope_freq_base;    /* 0: no rotation */
+    int32_t rope_is_neox;
+    int32_t reserved;
+} l2b_paged_rows;
+/* For every new token: rmsnorm! of its query and key heads one by one (src/inference.jl:102-110; where there are gains), rope!
+ * (src/inference.jl:112-167) at position prefix_len + own position with angles worked out in 64 bits, the queries to dev_q_out, keys and values into the
+ * sequence's pages.  Two new tokens with the same page and slot: which one's values end there is not determined. */
+int32_t l2b_paged_append_device(const l2b_paged_cache* cache, const l2b_paged_batch* batch, const l2b_paged_rows* rows, void* stream);
+typedef struct l2b_paged_queries {
+    int32_t type;      /* of q and out: L2B_TYPE_F32, or the cache's type */
+    int32_t n_heads;   /* a multiple of n_kv_heads: head h reads key/value head h / (n_heads / n_kv_heads) */
+    const void* dev_q; /* [rows][n_heads][head_size], rows on 16-byte boundaries, strides in values */
+    int64_t q_stride;
+    void* dev_out;
+    int64_t out_stride;
+    float scale;       /* 0: 1 / sqrt(head_size) */
+    int32_t reserved;
+} l2b_paged_queries;
+/* attention_weights! + scale + softmax! + combine_values! (src/inference.jl:263-278) of every new token over the prefix and over its sequence's own
+ * positions up to its own (the last of dev_counts[i] tokens sees dev_lengths[i] of them).  A token that sees nothing gets zeros.
+ * The workspace (at least l2b_paged_attention_workspace bytes, on a 16-byte boundary; any contents) is written while the call runs: calls that may run
+ * at the same time take different ones, captured calls too. */
+int32_t l2b_paged_attention_workspace(const l2b_paged_cache* cache, const l2b_paged_batch* batch, const l2b_paged_queries* queries, int64_t* bytes);
+int32_t l2b_paged_attention_device(const l2b_paged_cache* cache, const l2b_paged_batch* batch, const l2b_paged_queries* queries, void* dev_workspace,
+                                   int64_t workspace_bytes, void* stream);
+
+/* ---- sampling a batch, on device pointers ----------------------------------------------------------------------------
+ * logits ./= T; softmax!; wsample (src/inference.jl:361-368) of every row, among the tokens that three cuts leave.  With w_i = exp((x_i - max) / T) and the
+ * tokens in order (larger logits first, of equal ones the lower index first):
+ *   top_k in 1 .. vocab keeps the first top_k; other values: no cut;
+ *   top_p < 1 keeps those of them before which less than top_p of their whole mass lies; 1 and more: no cut;
+ *   min_p > 0 keeps those with w_i >= min_p;
+ *   the first one is always kept.
+ * The token is the first, by index, at which the kept tokens' cumulated mass exceeds uniform times their whole (computed so that the result hangs on the
+ * row alone).  T <= 0: argmax, first of equals.  Logits that are -inf or no numbers are never chosen; a row without any other gets token -1 and
+ * probability 0.  Several +inf share the mass equally. */
+typedef struct l2b_sampling {
+    int32_t type;                 /* of the logits: L2B_TYPE_F32, L2B_TYPE_F16 or L2B_TYPE_BF16 */
+    int32_t n_rows;
+    int32_t vocab;                /* at most 393216 */
+    int32_t reserved;
+    const void* dev_logits;       /* [n_rows][vocab], `stride` values from row to row */
+    int64_t stride;
+    const float* dev_temperature; /* [n_rows] each; NULL: 1 */
+    const int32_t* dev_top_k;     /* NULL: no cut */
+    const float* dev_top_p;
+    const float* dev_min_p;
+    const double* dev_uniform;    /* [n_rows], in [0, 1) */
+    int32_t* dev_tokens;          /* [n_rows] */
+    float* dev_probs;             /* [n_rows] probability with which the token was drawn; may be NULL */
+} l2b_sampling;
+int32_t l2b_sample_device(const l2b_sampling* sampling, void* stream);
 
 /* ---- resident matrices (for measurement with inputs already in HBM) ----------------- */
 /* Upload `copies` identical copies of one matrix (copies > 1 lets a benchmark rotate through more than the L2). */

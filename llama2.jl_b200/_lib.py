@@ -11,7 +11,7 @@ _HERE = os.path.dirname(os.path.abspath(__file__))
 LIB_PATH = os.environ.get("L2B_LIBRARY") or os.path.join(_HERE, "libllama2_b200.so")
 
 OK, ERR_BAD_ARG, ERR_UNSUPPORTED_TYPE, ERR_CUDA, _ERR_UNUSED, ERR_TIMEOUT, ERR_OOM, ERR_STATE, ERR_NO_DEVICE = range(9)
-TYPE_F32, TYPE_Q4_K, TYPE_Q5_K, TYPE_Q6_K, TYPE_BF16 = 0, 12, 13, 14, 30
+TYPE_F32, TYPE_F16, TYPE_Q4_K, TYPE_Q5_K, TYPE_Q6_K, TYPE_BF16 = 0, 1, 12, 13, 14, 30
 BLOCK_BYTES = {TYPE_Q4_K: 144, TYPE_Q5_K: 176, TYPE_Q6_K: 210}
 (ROLE_TOKEN_EMBEDDING, ROLE_RMS_ATT, ROLE_WQ, ROLE_WK, ROLE_WV, ROLE_WO, ROLE_RMS_FFN, ROLE_W1, ROLE_W2, ROLE_W3,
  ROLE_RMS_FINAL, ROLE_OUTPUT) = range(12)
@@ -32,6 +32,39 @@ class Config(C.Structure):
         ("act_planes", C.c_int32), ("device", C.c_int32), ("tp_size", C.c_int32), ("tp_rank", C.c_int32),
         ("reserved", C.c_int32 * 7),
     ]
+
+
+class PagedCache(C.Structure):
+    """l2b_paged_cache: the pages that hold the keys and values of many sequences."""
+    _fields_ = [("dev_k", C.c_void_p), ("dev_v", C.c_void_p), ("type", C.c_int32), ("n_pages", C.c_int32), ("page_size", C.c_int32),
+                ("n_kv_heads", C.c_int32), ("head_size", C.c_int32), ("reserved", C.c_int32)]
+
+
+class PagedBatch(C.Structure):
+    """l2b_paged_batch: the sequences of one step, their page tables and the prefix that they share."""
+    _fields_ = [("n_seq", C.c_int32), ("n_query", C.c_int32), ("dev_lengths", C.c_void_p), ("dev_counts", C.c_void_p), ("dev_pages", C.c_void_p),
+                ("pages_per_seq", C.c_int32), ("prefix_len", C.c_int32), ("dev_prefix_pages", C.c_void_p)]
+
+
+class PagedRows(C.Structure):
+    """l2b_paged_rows: new queries, keys and values, and what happens to them on their way."""
+    _fields_ = [("type", C.c_int32), ("n_heads", C.c_int32), ("dev_q", C.c_void_p), ("dev_k", C.c_void_p), ("dev_v", C.c_void_p),
+                ("q_stride", C.c_int64), ("k_stride", C.c_int64), ("v_stride", C.c_int64), ("dev_q_out", C.c_void_p), ("q_out_stride", C.c_int64),
+                ("dev_q_gain", C.c_void_p), ("dev_k_gain", C.c_void_p), ("eps", C.c_float), ("rope_freq_base", C.c_float),
+                ("rope_is_neox", C.c_int32), ("reserved", C.c_int32)]
+
+
+class PagedQueries(C.Structure):
+    """l2b_paged_queries: queries of an attention call and where its results go."""
+    _fields_ = [("type", C.c_int32), ("n_heads", C.c_int32), ("dev_q", C.c_void_p), ("q_stride", C.c_int64), ("dev_out", C.c_void_p),
+                ("out_stride", C.c_int64), ("scale", C.c_float), ("reserved", C.c_int32)]
+
+
+class Sampling(C.Structure):
+    """l2b_sampling: logits of a batch, each row's settings and random number, and where the tokens go."""
+    _fields_ = [("type", C.c_int32), ("n_rows", C.c_int32), ("vocab", C.c_int32), ("reserved", C.c_int32), ("dev_logits", C.c_void_p),
+                ("stride", C.c_int64), ("dev_temperature", C.c_void_p), ("dev_top_k", C.c_void_p), ("dev_top_p", C.c_void_p), ("dev_min_p", C.c_void_p),
+                ("dev_uniform", C.c_void_p), ("dev_tokens", C.c_void_p), ("dev_probs", C.c_void_p)]
 
 
 _P = C.c_void_p
@@ -89,6 +122,10 @@ _SIGNATURES = {
     "l2b_swiglu": ([_P, _P, C.c_int64], C.c_int32),
     "l2b_argmax": ([_P, C.c_int64, C.POINTER(C.c_int32)], C.c_int32),
     "l2b_sample_temperature": ([_P, C.c_int64, C.c_float, C.c_double, C.POINTER(C.c_int32)], C.c_int32),
+    "l2b_paged_append_device": ([C.POINTER(PagedCache), C.POINTER(PagedBatch), C.POINTER(PagedRows), _P], C.c_int32),
+    "l2b_paged_attention_workspace": ([C.POINTER(PagedCache), C.POINTER(PagedBatch), C.POINTER(PagedQueries), C.POINTER(C.c_int64)], C.c_int32),
+    "l2b_paged_attention_device": ([C.POINTER(PagedCache), C.POINTER(PagedBatch), C.POINTER(PagedQueries), _P, C.c_int64, _P], C.c_int32),
+    "l2b_sample_device": ([C.POINTER(Sampling), _P], C.c_int32),
     "l2b_matrix_create": ([C.c_int32, _P, C.c_int64, C.c_int64, C.c_int32, C.POINTER(_P)], C.c_int32),
     "l2b_matrix_destroy": ([_P], C.c_int32),
     "l2b_matrix_matvec_device": ([_P, C.c_int32, _P, _P, C.c_int32, _P], C.c_int32),

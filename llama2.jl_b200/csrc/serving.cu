@@ -1,0 +1,311 @@
+// Entry points of the paged cache (append, attention) and of filtered sampling: argument checks, choice of kernel, launches.
+#include <atomic>
+#include <cmath>
+
+#include "filtered_sampling.cuh"
+#include "host_common.h"
+#include "paged_attention.cuh"
+
+using namespace l2b;
+
+namespace {
+
+constexpr int MAX_DEVICES = 64;
+
+// The device that a pointer's memory is on is the current one while this lives.
+struct OnDeviceOf {
+    int before = -1;
+    int32_t enter(const void* ptr, const char* what) {
+        int n = 0;
+        if (cudaGetDeviceCount(&n) != cudaSuccess || n == 0) {
+            (void)cudaGetLastError();
+            return fail(L2B_ERR_NO_DEVICE, "no CUDA device is visible; this library has no CPU path");
+        }
+        cudaPointerAttributes a;
+        const cudaError_t e = cudaPointerGetAttributes(&a, ptr);
+        if (e != cudaSuccess || (a.type != cudaMemoryTypeDevice && a.type != cudaMemoryTypeManaged)) {
+            (void)cudaGetLastError();
+            return fail(L2B_ERR_BAD_ARG, std::string(what) + " is not device memory");
+        }
+        int now = 0;
+        CU(cudaGetDevice(&now));
+        if (now != a.device) {
+            CU(cudaSetDevice(a.device));
+            before = now;
+        }
+        device = a.device;
+        return L2B_OK;
+    }
+    ~OnDeviceOf() {
+        if (before >= 0) (void)cudaSetDevice(before);
+    }
+    int device = 0;
+};
+
+int32_t sm_count(int device, int* sms) {
+    static std::atomic<int> known[MAX_DEVICES];
+    if (device >= 0 && device < MAX_DEVICES && (*sms = known[device].load()) > 0) return L2B_OK;
+    CU(cudaDeviceGetAttribute(sms, cudaDevAttrMultiProcessorCount, device));
+    if (device >= 0 && device < MAX_DEVICES) known[device].store(*sms);
+    return L2B_OK;
+}
+
+// A kernel may take all shared memory of an SM: said once per kernel and device.
+template <auto Kernel>
+int32_t allow_smem(int device) {
+    static std::atomic<uint64_t> said{0};
+    const uint64_t bit = device >= 0 && device < MAX_DEVICES ? 1ull << device : 0;
+    if (bit && (said.load() & bit)) return L2B_OK;
+    cudaFuncAttributes a;
+    CU(cudaFuncGetAttributes(&a, Kernel));
+    CU(cudaFuncSetAttribute(Kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, 227 * 1024 - (int)a.sharedSizeBytes));
+    said.fetch_or(bit);
+    return L2B_OK;
+}
+
+bool aligned(const void* p, size_t to = 16) { return ((uintptr_t)p & (to - 1)) == 0; }
+int type_bytes(int type) { return type == L2B_TYPE_F32 ? 4 : 2; }
+
+int32_t check_cache(const l2b_paged_cache* c, PagedPool& pool) {
+    if (!c || !c->dev_k || !c->dev_v) return fail(L2B_ERR_BAD_ARG, "null argument");
+    if (c->type != L2B_TYPE_F16 && c->type != L2B_TYPE_BF16) return fail(L2B_ERR_UNSUPPORTED_TYPE, "a paged cache holds f16 or bf16 values");
+    if (c->n_pages <= 0 || c->n_kv_heads <= 0 || c->n_kv_heads > 65535) return fail(L2B_ERR_BAD_ARG, "bad number of pages or key/value heads");
+    if (c->page_size < 8 || c->page_size > 1024 || (c->page_size & (c->page_size - 1))) return fail(L2B_ERR_BAD_ARG, "page_size must be a power of two, 8 to 1024");
+    if (c->head_size < 8 || c->head_size > PA_MAX_SIZE || c->head_size % 8) return fail(L2B_ERR_BAD_ARG, "head_size must be a multiple of 8, at most 128");
+    if (!aligned(c->dev_k) || !aligned(c->dev_v)) return fail(L2B_ERR_BAD_ARG, "pages must lie on a 16-byte boundary");
+    pool.k = c->dev_k;
+    pool.v = c->dev_v;
+    pool.n_pages = c->n_pages;
+    pool.n_kv = c->n_kv_heads;
+    pool.hs = c->head_size;
+    pool.page_shift = 0;
+    while ((1 << pool.page_shift) < c->page_size) ++pool.page_shift;
+    return L2B_OK;
+}
+
+int32_t check_batch(const l2b_paged_batch* b, const PagedPool& pool, PagedSeqs& s) {
+    if (!b) return fail(L2B_ERR_BAD_ARG, "null argument");
+    if (b->n_seq < 0 || b->n_query < 1 || b->pages_per_seq < 0 || b->prefix_len < 0) return fail(L2B_ERR_BAD_ARG, "bad batch shape");
+    if ((b->n_seq > 0 && !b->dev_lengths) || (b->n_seq > 0 && b->pages_per_seq > 0 && !b->dev_pages) || (b->prefix_len > 0 && !b->dev_prefix_pages))
+        return fail(L2B_ERR_BAD_ARG, "null argument");
+    if (((int64_t)b->pages_per_seq << pool.page_shift) + b->prefix_len > 0x7fffffff) return fail(L2B_ERR_BAD_ARG, "more than 2^31 - 1 positions");
+    if ((int64_t)b->n_seq * b->n_query > 0x7fffffff) return fail(L2B_ERR_BAD_ARG, "more than 2^31 - 1 rows");
+    s.lengths = b->dev_lengths;
+    s.counts = b->dev_counts;
+    s.pages = b->dev_pages;
+    s.prefix_pages = b->dev_prefix_pages;
+    s.n_seq = b->n_seq;
+    s.n_query = b->n_query;
+    s.width = b->pages_per_seq;
+    s.prefix_len = b->prefix_len;
+    return L2B_OK;
+}
+
+int32_t check_rows(const void* p, int64_t stride, int64_t width, int type, const char* what) {
+    if (!p) return fail(L2B_ERR_BAD_ARG, "null argument");
+    if (stride < width) return fail(L2B_ERR_BAD_ARG, std::string(what) + ": rows overlap");
+    if (!aligned(p) || stride * type_bytes(type) % 16) return fail(L2B_ERR_BAD_ARG, std::string(what) + ": rows must lie on 16-byte boundaries");
+    return L2B_OK;
+}
+
+int32_t check_row_type(int type, int cache_type) {
+    if (type != L2B_TYPE_F32 && type != cache_type) return fail(L2B_ERR_UNSUPPORTED_TYPE, "rows are f32 or of the cache's type");
+    return L2B_OK;
+}
+
+// f(cache type, row type) with the two as types
+template <typename F>
+int32_t by_types(int cache_type, int type, F&& f) {
+    if (cache_type == L2B_TYPE_F16) return type == L2B_TYPE_F32 ? f(__half(), float()) : f(__half(), __half());
+    return type == L2B_TYPE_F32 ? f(__nv_bfloat16(), float()) : f(__nv_bfloat16(), __nv_bfloat16());
+}
+
+// What an attention call needs of its workspace, all in floats, and how it is cut.
+struct AttnPlan {
+    int blocks, smem, rows16;
+    int64_t slots, whole, total;  // floats of the slots' sums, of one set of whole items, of everything
+};
+
+AttnPlan attention_plan(const PagedPool& pool, const PagedSeqs& s, int n_heads, int sms) {
+    AttnPlan a;
+    const int ks = (pool.hs + 31) / 32 * 2, group = n_heads / pool.n_kv;
+    const int64_t rows = (int64_t)s.n_query * group * (s.prefix_len ? s.n_seq : 1);
+    a.rows16 = (int)(rows < PT_ROWS ? rows : PT_ROWS);
+    a.smem = PT_WARPS * PT_STAGES * 2 * PT_WKEYS * (ks * 32 + 16) + PT_WARPS * a.rows16 * (pool.hs + 2) * 4;
+    a.blocks = sms * (2 * (a.smem + 1024) <= 228 * 1024 ? 2 : 1);
+    a.slots = (int64_t)2 * a.blocks * PT_ROWS * (pool.hs + 4);  // (maxima and totals behind the sums, on 16-byte boundaries)
+    a.whole = s.prefix_len ? (int64_t)s.n_seq * s.n_query * n_heads * (pool.hs + 4) : 0;
+    a.total = a.slots + 2 * a.whole;
+    return a;
+}
+
+int32_t check_queries(const l2b_paged_cache* c, const l2b_paged_queries* q, const PagedSeqs& s) {
+    if (!q) return fail(L2B_ERR_BAD_ARG, "null argument");
+    L2B_TRY(check_row_type(q->type, c->type));
+    if (q->n_heads <= 0 || q->n_heads > 65535 || q->n_heads % c->n_kv_heads) return fail(L2B_ERR_BAD_ARG, "n_heads must be a multiple of n_kv_heads");
+    if ((int64_t)s.n_seq * s.n_query * q->n_heads > 0x7fffffff) return fail(L2B_ERR_BAD_ARG, "more than 2^31 - 1 query heads");
+    return L2B_OK;
+}
+
+}  // namespace
+
+extern "C" int32_t l2b_paged_append_device(const l2b_paged_cache* cache, const l2b_paged_batch* batch, const l2b_paged_rows* rows, void* stream) {
+    AppendParams p;
+    memset(&p, 0, sizeof(p));
+    L2B_TRY(check_cache(cache, p.pool));
+    L2B_TRY(check_batch(batch, p.pool, p.seqs));
+    if (!rows) return fail(L2B_ERR_BAD_ARG, "null argument");
+    L2B_TRY(check_row_type(rows->type, cache->type));
+    const int hs = p.pool.hs;
+    if ((rows->dev_q == nullptr) != (rows->dev_q_out == nullptr)) return fail(L2B_ERR_BAD_ARG, "dev_q and dev_q_out go together");
+    if (rows->dev_q) {
+        if (rows->n_heads <= 0 || rows->n_heads > 65535) return fail(L2B_ERR_BAD_ARG, "bad number of heads");
+        L2B_TRY(check_rows(rows->dev_q, rows->q_stride, (int64_t)rows->n_heads * hs, rows->type, "dev_q"));
+        L2B_TRY(check_rows(rows->dev_q_out, rows->q_out_stride, (int64_t)rows->n_heads * hs, rows->type, "dev_q_out"));
+        if (rows->dev_q == rows->dev_q_out && rows->q_stride != rows->q_out_stride) return fail(L2B_ERR_BAD_ARG, "in place the strides must be the same");
+    }
+    L2B_TRY(check_rows(rows->dev_k, rows->k_stride, (int64_t)p.pool.n_kv * hs, rows->type, "dev_k"));
+    L2B_TRY(check_rows(rows->dev_v, rows->v_stride, (int64_t)p.pool.n_kv * hs, rows->type, "dev_v"));
+    if (!aligned(rows->dev_q_gain) || !aligned(rows->dev_k_gain)) return fail(L2B_ERR_BAD_ARG, "gains must lie on a 16-byte boundary");
+    if ((rows->dev_q_gain || rows->dev_k_gain) && !(rows->eps >= 0.f)) return fail(L2B_ERR_BAD_ARG, "eps must not be negative");
+    if (!(rows->rope_freq_base >= 0.f) || std::isinf(rows->rope_freq_base)) return fail(L2B_ERR_BAD_ARG, "rope_freq_base must be positive, or 0 for no rotation");
+    p.q = rows->dev_q; p.k = rows->dev_k; p.v = rows->dev_v; p.q_out = rows->dev_q_out;
+    p.q_stride = rows->q_stride; p.k_stride = rows->k_stride; p.v_stride = rows->v_stride; p.q_out_stride = rows->q_out_stride;
+    p.q_gain = rows->dev_q_gain; p.k_gain = rows->dev_k_gain; p.eps = rows->eps;
+    p.n_heads = rows->n_heads; p.neox = rows->rope_is_neox != 0; p.rotate = rows->rope_freq_base > 0.f;
+    if (p.rotate) {
+        const long double step = powl((long double)rows->rope_freq_base, -2.0L / hs);
+        long double f = 0.15915494309189533576888376337251436L;  // turns per radian
+        for (int i = 0; i < hs / 2; ++i, f *= step) p.turns[i] = (double)f;
+    }
+    OnDeviceOf on;
+    L2B_TRY(on.enter(cache->dev_k, "dev_k"));
+    const int64_t n = (int64_t)p.seqs.n_seq * p.seqs.n_query;
+    if (n == 0) return L2B_OK;
+    // Tokens of a block: their angles are worked out together, 256 at a time, so several tokens once there are blocks for every SM twice over;
+    // before that one token, and its heads over several blocks while that leaves SMs idle.
+    int sms = 0;
+    L2B_TRY(sm_count(on.device, &sms));
+    p.tokens = n >= (int64_t)16 * sms ? 8 : n >= (int64_t)8 * sms ? 4 : 1;
+    const int unit = hs % 16 ? 8 : 16, units = hs / unit;
+    int lanes = 1;
+    while (lanes < units) lanes *= 2;
+    const int64_t slots = ((p.q ? p.n_heads : 0) + 2 * p.pool.n_kv) * p.tokens, passes = (slots + PA_THREADS / lanes - 1) / (PA_THREADS / lanes), blocks = (n + p.tokens - 1) / p.tokens;
+    int64_t y = 1;
+    while (y < passes && y < 64 && blocks * y < 2 * sms) ++y;
+    const dim3 grid((unsigned)blocks, (unsigned)y);
+    return by_types(cache->type, rows->type, [&](auto t, auto io) -> int32_t {
+        using T = decltype(t);
+        using TIO = decltype(io);
+        cudaStream_t st = (cudaStream_t)stream;
+        if (unit == 16) CU(launch_kernel(paged_append_kernel<TIO, T, 16>, grid, dim3(PA_THREADS), 0, st, true, p));
+        else CU(launch_kernel(paged_append_kernel<TIO, T, 8>, grid, dim3(PA_THREADS), 0, st, true, p));
+        return L2B_OK;
+    });
+}
+
+extern "C" int32_t l2b_paged_attention_workspace(const l2b_paged_cache* cache, const l2b_paged_batch* batch, const l2b_paged_queries* queries, int64_t* bytes) {
+    PagedPool pool;
+    PagedSeqs seqs;
+    L2B_TRY(check_cache(cache, pool));
+    L2B_TRY(check_batch(batch, pool, seqs));
+    L2B_TRY(check_queries(cache, queries, seqs));
+    if (!bytes) return fail(L2B_ERR_BAD_ARG, "null argument");
+    OnDeviceOf on;
+    L2B_TRY(on.enter(cache->dev_k, "dev_k"));
+    int sms = 0;
+    L2B_TRY(sm_count(on.device, &sms));
+    *bytes = attention_plan(pool, seqs, queries->n_heads, sms).total * 4;
+    return L2B_OK;
+}
+
+extern "C" int32_t l2b_paged_attention_device(const l2b_paged_cache* cache, const l2b_paged_batch* batch, const l2b_paged_queries* queries, void* dev_workspace,
+                                              int64_t workspace_bytes, void* stream) {
+    PagedAttnParams p;
+    memset(&p, 0, sizeof(p));
+    L2B_TRY(check_cache(cache, p.pool));
+    L2B_TRY(check_batch(batch, p.pool, p.seqs));
+    L2B_TRY(check_queries(cache, queries, p.seqs));
+    const int hs = p.pool.hs;
+    L2B_TRY(check_rows(queries->dev_q, queries->q_stride, (int64_t)queries->n_heads * hs, queries->type, "dev_q"));
+    L2B_TRY(check_rows(queries->dev_out, queries->out_stride, (int64_t)queries->n_heads * hs, queries->type, "dev_out"));
+    if (!std::isfinite(queries->scale)) return fail(L2B_ERR_BAD_ARG, "scale must be finite, or 0 for 1 / sqrt(head_size)");
+    OnDeviceOf on;
+    L2B_TRY(on.enter(cache->dev_k, "dev_k"));
+    if (p.seqs.n_seq == 0) return L2B_OK;
+    int sms = 0;
+    L2B_TRY(sm_count(on.device, &sms));
+    const AttnPlan plan = attention_plan(p.pool, p.seqs, queries->n_heads, sms);
+    if (!dev_workspace || !aligned(dev_workspace) || workspace_bytes < plan.total * 4)
+        return fail(L2B_ERR_BAD_ARG, "the workspace must lie on a 16-byte boundary and hold l2b_paged_attention_workspace bytes");
+    p.q = queries->dev_q; p.out = queries->dev_out; p.q_stride = queries->q_stride; p.out_stride = queries->out_stride;
+    p.n_heads = queries->n_heads;
+    p.group = queries->n_heads / p.pool.n_kv;
+    p.scale2 = (queries->scale != 0.f ? queries->scale : 1.f / sqrtf((float)hs)) * 1.4426950408889634f;
+    p.thin_prefix = p.seqs.prefix_len > 0;
+    p.blocks = plan.blocks;
+    float* const w = (float*)dev_workspace;
+    const int64_t n_rows = (int64_t)p.seqs.n_seq * p.seqs.n_query * p.n_heads;
+    p.slot_acc = w;
+    p.slot_ml = w + (int64_t)2 * plan.blocks * PT_ROWS * hs;
+    if (p.seqs.prefix_len) {
+        p.own_acc = w + plan.slots;
+        p.own_ml = p.own_acc + n_rows * hs;
+        p.pre_acc = w + plan.slots + plan.whole;
+        p.pre_ml = p.pre_acc + n_rows * hs;
+    }
+    cudaStream_t st = (cudaStream_t)stream;
+    L2B_TRY(by_types(cache->type, queries->type, [&](auto t, auto io) -> int32_t {
+        using T = decltype(t);
+        using TIO = decltype(io);
+        auto go = [&](auto ks) -> int32_t {
+            constexpr int KS = decltype(ks)::value;
+            L2B_TRY((allow_smem<paged_attention_kernel<T, TIO, KS>>(on.device)));
+            CU(launch_kernel(paged_attention_kernel<T, TIO, KS>, dim3((unsigned)plan.blocks), dim3(PT_WARPS * 32), (size_t)plan.smem, st, true, p));
+            return L2B_OK;
+        };
+        switch ((hs + 31) / 32) {
+            case 1: L2B_TRY(go(std::integral_constant<int, 2>())); break;
+            case 2: L2B_TRY(go(std::integral_constant<int, 4>())); break;
+            case 3: L2B_TRY(go(std::integral_constant<int, 6>())); break;
+            default: L2B_TRY(go(std::integral_constant<int, 8>())); break;
+        }
+        JoinParams j;
+        j.a = p;
+        j.heads = n_rows >= 4096 ? 8 : n_rows >= 1024 ? 2 : 1;
+        const dim3 grid((unsigned)(p.seqs.n_seq * p.seqs.n_query), (unsigned)((p.n_heads + j.heads - 1) / j.heads));
+        CU(launch_kernel(paged_join_kernel<TIO>, grid, dim3(PJ_WARPS * 32), 0, st, true, j));
+        return L2B_OK;
+    }));
+    return L2B_OK;
+}
+
+extern "C" int32_t l2b_sample_device(const l2b_sampling* a, void* stream) {
+    if (!a || !a->dev_logits || !a->dev_tokens || !a->dev_uniform) return fail(L2B_ERR_BAD_ARG, "null argument");
+    if (a->type != L2B_TYPE_F32 && a->type != L2B_TYPE_F16 && a->type != L2B_TYPE_BF16) return fail(L2B_ERR_UNSUPPORTED_TYPE, "logits are f32, f16 or bf16");
+    if (a->n_rows < 0 || a->vocab < 1 || a->vocab > FS_CLUSTER * FS_SLICE) return fail(L2B_ERR_BAD_ARG, "bad number of rows, or a vocabulary of more than 393216");
+    if (a->n_rows > 0x7fffffff / FS_CLUSTER) return fail(L2B_ERR_BAD_ARG, "too many rows");
+    if (a->stride < a->vocab) return fail(L2B_ERR_BAD_ARG, "rows overlap");
+    if (!aligned(a->dev_logits, type_bytes(a->type)) || !aligned(a->dev_tokens, 4) || !aligned(a->dev_uniform, 8)) return fail(L2B_ERR_BAD_ARG, "misaligned pointer");
+    OnDeviceOf on;
+    L2B_TRY(on.enter(a->dev_logits, "dev_logits"));
+    if (a->n_rows == 0) return L2B_OK;
+    int sms = 0;
+    L2B_TRY(sm_count(on.device, &sms));
+    SampleParams p;
+    p.logits = a->dev_logits; p.stride = a->stride; p.vocab = a->vocab;
+    p.temperature = a->dev_temperature; p.top_p = a->dev_top_p; p.min_p = a->dev_min_p; p.top_k = a->dev_top_k;
+    p.uniform = a->dev_uniform; p.tokens = a->dev_tokens; p.probs = a->dev_probs;
+    // Blocks of a row: as many as keep a slice at 16384 logits (two blocks to an SM), more while SMs would be idle and a slice has work for the block.
+    int cluster = 1;
+    while (cluster < FS_CLUSTER && ((a->vocab + cluster - 1) / cluster > 16384 || ((int64_t)a->n_rows * cluster * 2 <= 2 * sms && a->vocab / cluster >= 4096))) cluster *= 2;
+    p.cluster = cluster;
+    p.slice = ((a->vocab + cluster - 1) / cluster + 7) / 8 * 8;
+    auto go = [&](auto t) -> int32_t {
+        using T = decltype(t);
+        L2B_TRY(allow_smem<filtered_sample_kernel<T>>(on.device));
+        CU(launch_kernel(filtered_sample_kernel<T>, dim3((unsigned)(a->n_rows * cluster)), dim3(FS_THREADS), (size_t)p.slice * 4, (cudaStream_t)stream, true, p, cluster));
+        return L2B_OK;
+    };
+    return a->type == L2B_TYPE_F32 ? go(float()) : a->type == L2B_TYPE_F16 ? go(__half()) : go(__nv_bfloat16());
+}
