@@ -58,6 +58,13 @@ L2B_HD PagedParts paged_parts(int64_t begin, int tiles, int64_t share) {
 L2B_HD int paged_slot(const PagedParts& p, int block) { return 2 * block + (block == p.first ? 1 : 0); }
 
 
+// How the prefix's kernel cuts its work: row tiles of `streams_share` * 128 rows; streams_share 2: two row tiles on the same keys, 1: one, whose keys
+// the two streams take in turn.  units 0: there is no such part.
+struct PrefixCut {
+    int64_t units, share, whole_rows;  // whole_rows: rows of the batch * heads
+    int tiles, row_tiles, streams_share;
+};
+
 constexpr int PT_KEYS = 64, PT_ROWS = 16;  // a tile
 
 // Rows of a group are the query heads of one key/value head, of all the group's rows one after the other.  Groups: the prefix first where it is one

@@ -8,8 +8,8 @@
 // warps meet at an item's end only.  Copies run ahead over the ends of items.  Rows of keys and values lie 16 bytes further apart in shared memory than
 // they are long, so that ldmatrix reads eight rows without bank conflicts.
 //
-// f32 rows over a 16-bit cache: a query is split into terms of the cache's type (three of bf16, two of f16 behind a power of two per row) and a weight
-// into two, which keeps the products' error at 2^-16 of a weight or less.  For 16-bit rows the weights are rounded once to the cache's type (at most
+// f32 rows over a 16-bit cache: a query and a weight are split into terms of the cache's type (three of bf16, two of f16, the query's behind a power of two
+// per row), which keeps the products' error at 2^-22 or less.  For 16-bit rows the weights are rounded once to the cache's type (at most
 // half a step of 2^-8 or 2^-11 relative, as the result itself is); scores, maxima, totals and sums are f32.
 #pragma once
 #include <type_traits>
@@ -30,6 +30,8 @@ struct PagedAttnParams : PagedWork {
     float *slot_acc, *slot_ml;  // [2 * blocks][16][hs], [2 * blocks][16][2]
     float *own_acc, *own_ml;    // items that one block did: [rows * n_heads][hs], [..][2]; null where nothing else is to be joined
     float *pre_acc, *pre_ml;    // the same of the prefix
+    PrefixCut cut;              // of the prefix's kernel (paged_prefix.cuh), which may be running still
+    float *cut_acc, *cut_ml;    // its slots: [2 * blocks][2][128][hs], [..][2]
 };
 
 __device__ __forceinline__ void cp_async16(void* dst, const void* src, bool real) {  // not real: zeros, and nothing is read
@@ -79,7 +81,7 @@ __device__ __forceinline__ uint32_t split_pair(float& a, float& b) {
 template <typename T, typename TIO, int KS>
 struct ThinTraits {
     static constexpr bool WIDE = sizeof(TIO) == 4;
-    static constexpr int QT = !WIDE ? 1 : sizeof(T) == 2 && std::is_same<T, __half>::value ? 2 : 3, PT = WIDE ? 2 : 1;
+    static constexpr int QT = !WIDE ? 1 : sizeof(T) == 2 && std::is_same<T, __half>::value ? 2 : 3, PT = QT;
     static constexpr int PITCH = KS * 32 + 16;               // bytes of a row in shared memory
     static constexpr int HALF_STAGE = PT_WKEYS * PITCH;      // keys of a stage, or values
     static constexpr int RING = PT_WARPS * PT_STAGES * 2 * HALF_STAGE;
@@ -101,8 +103,11 @@ __global__ void __launch_bounds__(PT_WARPS * 32, 2) paged_attention_kernel(const
         const int r = i / (KS * 2 - chunks), ch = chunks + i % (KS * 2 - chunks);
         *reinterpret_cast<uint4*>(ring + r * TR::PITCH + ch * 16) = make_uint4(0, 0, 0, 0);
     }
-    pdl_wait();
-    pdl_launch_dependents();  // (behind the wait: the joining kernel reads the lengths before it waits itself)
+    // The prefix's kernel in front has waited for what was before it, and nothing here hangs on it: then the wait is for the end, so that the joining
+    // kernel finds both done.
+    const bool late = p.cut.units > 0;
+    if (!late) pdl_wait();
+    pdl_launch_dependents();  // (behind a wait, here or there: the joining kernel reads the lengths before it waits itself)
 
     // this block's share; every warp finds it for itself
     int64_t units = 0;
@@ -110,9 +115,9 @@ __global__ void __launch_bounds__(PT_WARPS * 32, 2) paged_attention_kernel(const
     for (int o = 16; o > 0; o >>= 1) units += __shfl_xor_sync(0xffffffffu, units, o);
     const PagedShares sh = paged_shares(units, p.blocks);
     const int64_t begin = (int64_t)blockIdx.x * sh.share;
-    if (begin >= units) return;
     Cursor at;
-    {
+    at.left = 0;
+    if (begin < units) {
         int64_t sum = 0;  // units of the groups before
         int found = -1;
         for (int g0 = 0; found < 0 && g0 < groups; g0 += 32) {
@@ -131,8 +136,7 @@ __global__ void __launch_bounds__(PT_WARPS * 32, 2) paged_attention_kernel(const
                 sum += __shfl_sync(0xffffffffu, inc, 31);
             }
         }
-        if (found < 0) return;  // (begin < units: it is found)
-        at = cursor_at(p, found, begin - sum, min(sh.share, units - begin));
+        if (found >= 0) at = cursor_at(p, found, begin - sum, min(sh.share, units - begin));
     }
 
     Cursor ahead = at;
@@ -428,6 +432,7 @@ __global__ void __launch_bounds__(PT_WARPS * 32, 2) paged_attention_kernel(const
         }
         next_item(p, at, tiles);
     }
+    if (late) pdl_wait();
 }
 
 // Joins the partial results of a row: a block per token and `heads` heads, a warp's lanes along the head's values.  WARPS warps share a row's parts
@@ -463,7 +468,6 @@ __global__ void __launch_bounds__(PJ_WARPS * 32) paged_join_kernel(const __grid_
     const int64_t tok = blockIdx.x;
     const int seq = (int)(tok / p.seqs.n_query), j = (int)(tok % p.seqs.n_query), group = seq + p.thin_prefix;
     const int length = p.seqs.lengths[seq], count = paged_count(length, p.seqs.counts ? p.seqs.counts[seq] : p.seqs.n_query, p.seqs.n_query);
-    if (j >= count) return;
     // where the shares lie: units of all groups, and of those before this one
     int64_t all = 0, before = 0;
     for (int g = threadIdx.x; g < p.seqs.n_seq + p.thin_prefix; g += PJ_WARPS * 32) {
@@ -487,6 +491,7 @@ __global__ void __launch_bounds__(PJ_WARPS * 32) paged_join_kernel(const __grid_
     }
     const PagedShares sh = paged_shares(all, p.blocks);
     pdl_wait();
+    if (j >= count) return;
 
     const int per_row = PJ_WARPS / jp.heads, head = blockIdx.y * jp.heads + warp / per_row, sub = warp % per_row;
     const bool real = head < p.n_heads;
@@ -515,6 +520,18 @@ __global__ void __launch_bounds__(PJ_WARPS * 32) paged_join_kernel(const __grid_
     };
     if (real) {
         const int g = head - kv * p.group;
+        if (p.cut.units > 0) {
+            const int row = (int)(tok * p.group) + g, per_item = p.cut.streams_share * 128, row_tile = row / per_item, r128 = row % 128;
+            const int i0 = p.cut.streams_share == 2 ? row % per_item / 128 : 0, streams = p.cut.streams_share == 2 ? 1 : 2;
+            const PagedParts parts = paged_parts(((int64_t)kv * p.cut.row_tiles + row_tile) * p.cut.tiles, p.cut.tiles, p.cut.share);
+            const bool whole = parts.first == parts.last;
+            for (int n = sub; n < (parts.last - parts.first + 1) * streams; n += per_row) {
+                const int b = parts.first + n / streams, i = i0 + n % streams;
+                const int64_t at = whole ? (streams == 2 ? i * p.cut.whole_rows : 0) + at_row : ((int64_t)paged_slot(parts, b) * 2 + i) * 128 + r128;
+                const float2 ml = __ldcg(reinterpret_cast<const float2*>((whole ? p.pre_ml : p.cut_ml) + at * 2));
+                join(r, ml.x, ml.y, (whole ? p.pre_acc : p.cut_acc) + at * hs + d, d < hs);
+            }
+        }
         if (p.thin_prefix) item(0, group_shape(p, 0), (int)(tok * p.group) + g, p.pre_acc, p.pre_ml);
         item(before, group_shape(p, group), j * p.group + g, p.own_acc, p.own_ml);
     }

@@ -1,0 +1,364 @@
+// The shared prefix's part of the paged attention on the 5th-generation tensor cores: the rows of all sequences (every query head of a key/value
+// head, of every new token) against the same keys, which are read once per 256 (128) rows instead of once per sequence.
+//
+// A block runs two streams, each with its own 128 rows of scores and sums in tensor memory and its own four softmax warps (a thread per row), so that
+// one's products run beside the other's exponentials:  S = Q K^T,  P = exp2(S - m) as a tensor-memory operand in S's place,  O += P V.
+//   TILES = 2: the streams are two row tiles that share the tiles of keys (128 each);
+//   TILES = 1: one row tile, the streams take the tiles of keys in turn and leave a partial result each: for few rows, and for f32 rows, whose three (f16: two)
+//              terms of Q take the place of a second tile (64 keys a tile).
+//   warps 0-3, 4-7  the streams' softmax; before it they bring the block's rows of Q into shared memory, after it the sums to the workspace
+//   warp 8          issues the products; those of a stream follow one another: P V of a tile, then Q K^T of its next, which overwrites that P
+//   warp 9          TMA copies of keys and values straight from the pages: 8 rows or more at a time, V's rows behind the prefix's end through a map
+//                   that ends there, so that they are zeros; pages that are none lie outside the map and are zeros, too
+// Rows are rescaled only when a maximum has grown by more than 2^8.  The work, items (key/value head, row tile) of the prefix' key tiles, is cut
+// into equal shares of a block per SM (paged.h).  Every wait is bounded; a block whose wait ran out leaves NaN.
+#pragma once
+#include "paged_attention.cuh"
+#include "tcgen05.cuh"
+
+namespace l2b {
+
+constexpr int PX_ROWS = 128, PX_THREADS = 320, PX_MAX_STAGES = 8, PX_RING = 16;  // PX_RING: masks under way, more than stages
+
+struct PrefixParams : PagedWork {
+    const void* q;
+    int64_t q_stride;
+    int n_heads, rows, stages;
+    float scale2;  // not negative: a negative scale's sign goes to the queries
+    int negate;
+    PrefixCut cut;
+    float *slot_acc, *slot_ml;  // [2 * blocks][2][128][hs], [..][2]
+    float *pre_acc, *pre_ml;    // [2 / TILES][rows of the batch * n_heads][hs], [..][2]
+};
+
+template <typename T, typename TIO, int TILES>
+struct PrefixTraits {
+    static constexpr bool WIDE = sizeof(TIO) == 4, F16 = std::is_same<T, __half>::value;
+    static constexpr int QT = !WIDE ? 1 : F16 ? 2 : 3, PT = QT;
+    static constexpr int KEYS = WIDE ? 64 : 128;
+    static constexpr int SUB_Q = PX_ROWS * 128, SUB_K = KEYS * 128;  // bytes of 64 values of a tile's rows
+    // instruction descriptors: f32 sums, A and B of T; B's rows along K for P V
+    __host__ __device__ static constexpr uint32_t idesc(int n, int b_mn) {
+        return (1u << 4) | (F16 ? 0u : (1u << 7) | (1u << 10)) | ((uint32_t)b_mn << 16) | ((uint32_t)(n >> 3) << 17) | ((uint32_t)(PX_ROWS >> 4) << 24);
+    }
+};
+__device__ __forceinline__ void tmem_st16u(uint32_t taddr, const uint32_t (&v)[16]) {
+    asm volatile("tcgen05.st.sync.aligned.32x32b.x16.b32 [%0], {%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15,%16};" ::"r"(taddr), "r"(v[0]), "r"(v[1]), "r"(v[2]),
+                 "r"(v[3]), "r"(v[4]), "r"(v[5]), "r"(v[6]), "r"(v[7]), "r"(v[8]), "r"(v[9]), "r"(v[10]), "r"(v[11]), "r"(v[12]), "r"(v[13]), "r"(v[14]), "r"(v[15])
+                 : "memory");
+}
+
+// The softmax threads' part in bringing 128 * TILES rows of Q to shared memory, in operand layout, as terms of T.
+template <typename T, typename TIO, int TILES>
+__device__ __forceinline__ void load_queries(const PrefixParams& p, uint8_t* sq, int* s_exp, int kv, int row0, int nd) {
+    using TR = PrefixTraits<T, TIO, TILES>;
+    const int hs = p.pool.hs, per_row = nd * 8, tid = threadIdx.x;
+    for (int i = tid; i < TILES * PX_ROWS * per_row; i += 256) {  // (per_row is 8 or 16: a row's threads are of one warp)
+        const int r = i / per_row, ch = i - r * per_row, row = row0 + r;
+        float x[8] = {};
+        if (row < p.rows && ch * 8 < hs) {
+            const int t = row / p.group;
+            get((const TIO*)p.q + (int64_t)t * p.q_stride + (int64_t)(kv * p.group + row - t * p.group) * hs + ch * 8, x);
+        }
+        if (p.negate) {
+#pragma unroll
+            for (int e = 0; e < 8; ++e) x[e] = -x[e];
+        }
+        if (TR::WIDE && TR::F16) {  // f16 terms: the row's largest value between 1/2 and 1
+            float mx = 0.f;
+#pragma unroll
+            for (int e = 0; e < 8; ++e) mx = fmaxf(mx, fabsf(x[e]));
+            for (int o = per_row / 2; o > 0; o >>= 1) mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, o));
+            int ex = 0;
+            if (mx > 0.f && mx < INFINITY) frexpf(mx, &ex);
+            ex = max(-100, min(100, ex));
+            if (ch == 0) s_exp[r] = ex;
+#pragma unroll
+            for (int e = 0; e < 8; ++e) x[e] = ldexpf(x[e], -ex);
+        }
+#pragma unroll
+        for (int t = 0; t < TR::QT; ++t) {
+            uint4 w;
+            w.x = split_pair<T>(x[0], x[1]);
+            w.y = split_pair<T>(x[2], x[3]);
+            w.z = split_pair<T>(x[4], x[5]);
+            w.w = split_pair<T>(x[6], x[7]);
+            *reinterpret_cast<uint4*>(sq + ((t * TILES + r / PX_ROWS) * nd + (ch >> 3)) * TR::SUB_Q + sw128_chunk(r % PX_ROWS, ch & 7)) = w;
+        }
+    }
+}
+
+template <typename T, typename TIO, int TILES>
+__global__ void __launch_bounds__(PX_THREADS, 1) paged_prefix_kernel(const __grid_constant__ PrefixParams p, const __grid_constant__ CUtensorMap map_k,
+                                                                     const __grid_constant__ CUtensorMap map_v, const __grid_constant__ CUtensorMap map_end) {
+    using TR = PrefixTraits<T, TIO, TILES>;
+    constexpr int KEYS = TR::KEYS;
+    extern __shared__ __align__(1024) uint8_t px_raw[];
+    __shared__ __align__(8) uint64_t s_kfull[PX_MAX_STAGES], s_kfree[PX_MAX_STAGES], s_vfull[PX_MAX_STAGES], s_vfree[PX_MAX_STAGES], s_mask[PX_RING], s_q, s_seg, s_s[2], s_p[2];
+    __shared__ uint32_t s_tmem, s_valid[PX_RING][4];
+    __shared__ int s_exp[TILES * PX_ROWS];
+    uint8_t* const smem = px_raw + ((1024u - (smem_u32(px_raw) & 1023u)) & 1023u);
+    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, hs = p.pool.hs, nd = (hs + 63) / 64, vn = (hs + 15) / 16 * 16;
+    uint8_t* const sq = smem;
+    uint8_t* const sk = smem + TR::QT * TILES * nd * TR::SUB_Q;
+    uint8_t* const sv = sk + p.stages * nd * TR::SUB_K;
+    if (threadIdx.x == 0) {
+        for (int i = 0; i < p.stages; ++i) {
+            mbar_init(s_kfull + i, 1);
+            mbar_init(s_kfree + i, 1);
+            mbar_init(s_vfull + i, 1);
+            mbar_init(s_vfree + i, 1);
+        }
+        for (int i = 0; i < PX_RING; ++i) mbar_init(s_mask + i, 1);
+        mbar_init(&s_q, 8);
+        mbar_init(&s_seg, 1);
+        for (int i = 0; i < 2; ++i) {
+            mbar_init(s_s + i, 1);
+            mbar_init(s_p + i, 4);
+        }
+        fence_barrier_init();
+        fence_proxy_async();
+    }
+    if (warp == 8) tmem_alloc(&s_tmem, 512);
+    tc_fence_before();
+    __syncthreads();
+    tc_fence_after();
+    const uint32_t tmem = s_tmem;
+    pdl_wait();
+    pdl_launch_dependents();  // (behind the wait: what follows reads the lengths before it waits itself)
+
+    const int64_t begin = (int64_t)blockIdx.x * p.cut.share, end = min(begin + p.cut.share, p.cut.units);
+    if (warp == 9) {
+        // ---- copies
+        bool ok = true;
+        const int shift = min(p.pool.page_shift, KEYS == 128 ? 7 : 6), chunks = KEYS >> shift;  // a chunk: the map's box
+        const int outside = p.pool.n_pages * p.pool.n_kv, last_page = (p.seqs.prefix_len - 1) >> p.pool.page_shift;
+        int g = 0;  // tiles so far
+        for (int64_t u = begin; u < end && ok; ++u, ++g) {
+            const int item = (int)(u / p.cut.tiles), tile = (int)(u - (int64_t)item * p.cut.tiles), kv = item / p.cut.row_tiles;
+            const int stage = g % p.stages, use = g / p.stages;
+            // which keys are there: four to a lane (of one page)
+            const int key = tile * KEYS + lane * 4;
+            uint32_t nibble = 0;
+            if (lane * 4 < KEYS && key < p.seqs.prefix_len) {
+                const int page = p.seqs.prefix_pages[key >> p.pool.page_shift];
+                if (page >= 0 && page < p.pool.n_pages) nibble = p.seqs.prefix_len - key >= 4 ? 15u : (1u << (p.seqs.prefix_len - key)) - 1u;
+            }
+            uint32_t word = nibble << (4 * (lane & 7));
+            for (int o = 1; o < 8; o <<= 1) word |= __shfl_xor_sync(0xffffffffu, word, o);
+            // a chunk of rows of one page to a lane
+            const int first = tile * KEYS + (lane << shift), index = first >> p.pool.page_shift;
+            int page = -1;
+            if (lane < chunks && first < p.seqs.prefix_len) page = p.seqs.prefix_pages[index];
+            const bool there = page >= 0 && page < p.pool.n_pages;
+            const int z = there ? page * p.pool.n_kv + kv : outside, y = first & ((1 << p.pool.page_shift) - 1);
+            if (use > 0 && !mbar_wait_warp(s_kfree + stage, (uint32_t)((use - 1) & 1))) {
+                ok = false;
+                break;
+            }
+            if ((lane & 7) == 0) s_valid[g % PX_RING][lane >> 3] = word;
+            __syncwarp();
+            if (lane == 0) {
+                mbar_arrive(s_mask + g % PX_RING);
+                mbar_arrive_expect_tx(s_kfull + stage, (uint32_t)(nd * TR::SUB_K));
+            }
+            __syncwarp();
+            if (lane < chunks)
+                for (int d = 0; d < nd; ++d) tma_load_3d(sk + (stage * nd + d) * TR::SUB_K + (lane << shift) * 128, &map_k, 64 * d, y, z, s_kfull + stage);
+            if (use > 0 && !mbar_wait_warp(s_vfree + stage, (uint32_t)((use - 1) & 1))) {
+                ok = false;
+                break;
+            }
+            if (lane == 0) mbar_arrive_expect_tx(s_vfull + stage, (uint32_t)(nd * TR::SUB_K));
+            __syncwarp();
+            if (lane < chunks)
+                for (int d = 0; d < nd; ++d) tma_load_3d(sv + (stage * nd + d) * TR::SUB_K + (lane << shift) * 128, index == last_page ? &map_end : &map_v, 64 * d, y, z, s_vfull + stage);
+        }
+        if (!ok)
+            for (int i = 0; i < 2000; ++i) __nanosleep(1000);  // copies in flight land within microseconds
+    } else if (warp == 8) {
+        // ---- products
+        if (lane == 0) {
+            const uint32_t idesc_s = TR::idesc(KEYS, 0), idesc_o = TR::idesc(vn, 1);
+            bool ok = true;
+            int g = 0, segment = 0, np[2] = {0, 0};
+            auto qk = [&](int i, int gt) {  // scores of tile gt for stream i
+                const int stage = gt % p.stages, qtile = TILES == 2 ? i : 0;
+                bool more = false;
+#pragma unroll 1
+                for (int t = TR::QT - 1; t >= 0; --t)  // (small terms first)
+                    for (int kk = 0; 16 * kk < hs; ++kk) {
+                        umma_f16(tmem + (uint32_t)(i * 128), umma_desc_sw128(sq + ((t * TILES + qtile) * nd + (kk >> 2)) * TR::SUB_Q, (kk & 3) * 32),
+                                 umma_desc_sw128(sk + (stage * nd + (kk >> 2)) * TR::SUB_K, (kk & 3) * 32), idesc_s, more ? 1u : 0u);
+                        more = true;
+                    }
+                umma_commit(s_s + i);
+            };
+            auto pv = [&](int i, int gt, bool more) {
+                const int stage = gt % p.stages;
+#pragma unroll 1
+                for (int t = TR::PT - 1; t >= 0; --t)
+                    for (int kk = 0; kk < KEYS / 16; ++kk) {
+                        umma_f16_at(tmem + 256 + (uint32_t)(i * 128), tmem + (uint32_t)(i * 128 + t * (KEYS / 2) + kk * 8), umma_desc_sw128_mn(sv + stage * nd * TR::SUB_K, kk * 2048, TR::SUB_K), idesc_o,
+                                    more ? 1u : 0u);
+                        more = true;
+                    }
+            };
+            for (int64_t u = begin; u < end && ok; ++segment) {
+                const int item = (int)(u / p.cut.tiles), n = (int)min((int64_t)p.cut.tiles - (u - (int64_t)item * p.cut.tiles), end - u);
+                if (!mbar_wait_bounded(&s_q, (uint32_t)(segment & 1))) {
+                    ok = false;
+                    break;
+                }
+                const int lag = TILES == 2 ? 1 : 2;  // a stream's next tile
+                for (int s = 0; s < n + lag && ok; ++s)
+                    for (int i = TILES == 2 ? 0 : s & 1; i <= (TILES == 2 ? 1 : s & 1); ++i) {
+                        if (s >= lag) {
+                            const int gt = g + s - lag;
+                            if (!mbar_wait_bounded(s_p + i, (uint32_t)(np[i] & 1)) || !mbar_wait_bounded(s_vfull + gt % p.stages, (uint32_t)(gt / p.stages & 1))) {
+                                ok = false;
+                                break;
+                            }
+                            ++np[i];
+                            tc_fence_after();
+                            pv(i, gt, s >= 2 * lag);
+                            if (TILES == 1 || i == 1) umma_commit(s_vfree + gt % p.stages);
+                        }
+                        if (s < n) {
+                            const int gt = g + s;
+                            if (!mbar_wait_bounded(s_kfull + gt % p.stages, (uint32_t)(gt / p.stages & 1))) {
+                                ok = false;
+                                break;
+                            }
+                            tc_fence_after();
+                            qk(i, gt);
+                            if (TILES == 1 || i == 1) umma_commit(s_kfree + gt % p.stages);
+                        }
+                    }
+                if (ok) umma_commit(&s_seg);
+                g += n;
+                u += n;
+            }
+        }
+    } else {
+        // ---- softmax: a thread per row of its stream
+        const int i = warp >> 2, r = (warp & 3) * 32 + lane;
+        const uint32_t lanes = (uint32_t)((warp & 3) * 32) << 16, ts = tmem + lanes + (uint32_t)(i * 128), to = tmem + 256 + lanes + (uint32_t)(i * 128);
+        bool ok = true;
+        int g = 0, segment = 0, ns = 0;
+        for (int64_t u = begin; u < end; ++segment) {
+            const int item = (int)(u / p.cut.tiles), first_tile = (int)(u - (int64_t)item * p.cut.tiles), n = (int)min((int64_t)p.cut.tiles - first_tile, end - u);
+            const int kv = item / p.cut.row_tiles, row_tile = item - kv * p.cut.row_tiles;
+            load_queries<T, TIO, TILES>(p, sq, s_exp, kv, row_tile * TILES * PX_ROWS, nd);
+            fence_proxy_async();
+            __syncwarp();
+            if (lane == 0) mbar_arrive(&s_q);
+            float sc = p.scale2;
+            if (TR::WIDE && TR::F16) {
+                asm volatile("bar.sync 1, 256;" ::: "memory");  // (the row's exponent is another thread's)
+                sc = ldexpf(sc, s_exp[TILES == 2 ? i * PX_ROWS + r : r]);
+            }
+            float m = -INFINITY, l = 0.f;
+            bool some = false;
+            for (int t = TILES == 2 ? 0 : i; t < n; t += TILES == 2 ? 1 : 2) {
+                const int gt = g + t;
+                if (ok) ok = mbar_wait_warp(s_mask + gt % PX_RING, (uint32_t)(gt / PX_RING & 1));
+                if (ok) ok = mbar_wait_warp(s_s + i, (uint32_t)(ns & 1));
+                ++ns;
+                tc_fence_after();
+                float x[KEYS];
+#pragma unroll
+                for (int c = 0; c < KEYS; c += 32) tmem_ld32f(ts + (uint32_t)c, *reinterpret_cast<float(*)[32]>(x + c));
+                uint32_t there[KEYS / 32], all = ~0u;
+#pragma unroll
+                for (int c = 0; c < KEYS / 32; ++c) {
+                    there[c] = s_valid[gt % PX_RING][c];
+                    all &= there[c];
+                }
+                if (all != ~0u) {
+#pragma unroll
+                    for (int k = 0; k < KEYS; ++k) x[k] = there[k >> 5] >> (k & 31) & 1 ? x[k] : -INFINITY;
+                }
+                float m4[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
+#pragma unroll
+                for (int k = 0; k < KEYS; k += 2) m4[k >> 1 & 3] = fmaxf(fmaxf(x[k], x[k + 1]), m4[k >> 1 & 3]);
+                const float mx = fmaxf(fmaxf(m4[0], m4[1]), fmaxf(m4[2], m4[3])) * sc;
+                if (!some) {
+                    m = mx;
+                } else if (__any_sync(0xffffffffu, mx > m + 8.f)) {
+                    const float mn = mx > m + 8.f ? mx : m, corr = m == -INFINITY ? 0.f : exp2_approx(m - mn);  // (a row that has seen nothing has sums of zero)
+                    l *= corr;
+                    m = mn;
+#pragma unroll 1
+                    for (int c = 0; c < vn; c += 32) {
+                        float o[32];
+                        tmem_ld32f(to + (uint32_t)c, o);
+#pragma unroll
+                        for (int e = 0; e < 32; ++e) o[e] *= corr;
+                        tmem_st32f(to + (uint32_t)c, o);
+                    }
+                }
+                some = true;
+                const float use = m == -INFINITY ? 0.f : m;
+                float l4[4] = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+                for (int c = 0; c < KEYS; c += 32) {
+#pragma unroll
+                    for (int k = 0; k < 32; ++k) {
+                        x[c + k] = exp2_approx(fmaf(x[c + k], sc, -use));
+                        l4[k & 3] += x[c + k];
+                    }
+#pragma unroll
+                    for (int t2 = 0; t2 < TR::PT; ++t2) {
+                        uint32_t w[16];
+#pragma unroll
+                        for (int k = 0; k < 16; ++k) w[k] = TR::PT == 1 ? pair_of<T>(x[c + 2 * k], x[c + 2 * k + 1]) : split_pair<T>(x[c + 2 * k], x[c + 2 * k + 1]);
+                        tmem_st16u(ts + (uint32_t)(t2 * (KEYS / 2) + c / 2), w);
+                    }
+                }
+                l += (l4[0] + l4[1]) + (l4[2] + l4[3]);
+                tmem_wait_st();
+                tc_fence_before();
+                __syncwarp();
+                if (lane == 0) mbar_arrive(s_p + i);
+            }
+            // the segment's products are all done: this row's sums to the workspace
+            if (ok) ok = mbar_wait_warp(&s_seg, (uint32_t)(segment & 1));
+            tc_fence_after();
+            if (l != l && m == -INFINITY) m = 0.f;  // scores that are no numbers are not an empty row
+            if (!ok) {
+                m = 0.f;
+                l = NAN;
+            }
+            const int row = row_tile * TILES * PX_ROWS + (TILES == 2 ? i * PX_ROWS : 0) + r;
+            const bool whole = n == p.cut.tiles, real = row < p.rows;
+            int64_t at;
+            if (whole) {
+                const int t = row / p.group;
+                at = (TILES == 1 ? (int64_t)i * p.cut.whole_rows : 0) + (int64_t)t * p.n_heads + kv * p.group + row - t * p.group;
+            } else {
+                at = ((int64_t)(2 * blockIdx.x + (first_tile == 0 ? 1 : 0)) * 2 + i) * PX_ROWS + r;
+            }
+            if (real) *reinterpret_cast<float2*>((whole ? p.pre_ml : p.slot_ml) + at * 2) = make_float2(m, l);
+            if (some) {  // (the same for the whole warp)
+                float* const acc = (whole ? p.pre_acc : p.slot_acc) + at * hs;
+#pragma unroll 1
+                for (int c = 0; c < vn; c += 32) {
+                    float o[32];
+                    tmem_ld32f(to + (uint32_t)c, o);
+#pragma unroll
+                    for (int e = 0; e < 32; e += 4)
+                        if (real && c + e < hs) *reinterpret_cast<float4*>(acc + c + e) = make_float4(o[e], o[e + 1], o[e + 2], o[e + 3]);
+                }
+            }
+            tc_fence_before();  // (the next segment's products overwrite the sums)
+            g += n;
+            u += n;
+        }
+    }
+    tc_fence_before();
+    __syncthreads();
+    if (warp == 8) tmem_dealloc(tmem, 512);
+}
+
+}  // namespace l2b

@@ -5,6 +5,7 @@
 #include "filtered_sampling.cuh"
 #include "host_common.h"
 #include "paged_attention.cuh"
+#include "paged_prefix.cuh"
 
 using namespace l2b;
 
@@ -122,21 +123,59 @@ int32_t by_types(int cache_type, int type, F&& f) {
 
 // What an attention call needs of its workspace, all in floats, and how it is cut.
 struct AttnPlan {
-    int blocks, smem, rows16;
-    int64_t slots, whole, total;  // floats of the slots' sums, of one set of whole items, of everything
+    int blocks, smem, thin_prefix;
+    PrefixCut cut;              // the prefix's own kernel, a block per SM
+    int cut_blocks, stages, cut_smem;
+    int64_t slots, whole, cut_slots, pre, total;  // floats of the slots, of whole items, of the prefix's slots and whole items, of everything
 };
 
-AttnPlan attention_plan(const PagedPool& pool, const PagedSeqs& s, int n_heads, int sms) {
+// The prefix goes through the tensor cores' 128-row tiles when its rows fill more than one tile of 16; up to there it is one more group of the own
+// parts' kernel, without a launch of its own.
+AttnPlan attention_plan(const PagedPool& pool, const PagedSeqs& s, int n_heads, int type, int cache_type, int sms) {
     AttnPlan a;
+    memset(&a, 0, sizeof(a));
     const int ks = (pool.hs + 31) / 32 * 2, group = n_heads / pool.n_kv;
-    const int64_t rows = (int64_t)s.n_query * group * (s.prefix_len ? s.n_seq : 1);
-    a.rows16 = (int)(rows < PT_ROWS ? rows : PT_ROWS);
-    a.smem = PT_WARPS * PT_STAGES * 2 * PT_WKEYS * (ks * 32 + 16) + PT_WARPS * a.rows16 * (pool.hs + 2) * 4;
+    const int64_t n_tok = (int64_t)s.n_seq * s.n_query, rows = n_tok * group;
+    const bool tiled = s.prefix_len > 0 && rows > PT_ROWS && (int64_t)pool.n_pages * pool.n_kv < 0x7fffffff;
+    a.thin_prefix = s.prefix_len > 0 && !tiled;
+    const int64_t most = (int64_t)s.n_query * group * (a.thin_prefix ? s.n_seq : 1);
+    a.smem = PT_WARPS * PT_STAGES * 2 * PT_WKEYS * (ks * 32 + 16) + PT_WARPS * (int)(most < PT_ROWS ? most : PT_ROWS) * (pool.hs + 2) * 4;
     a.blocks = sms * (2 * (a.smem + 1024) <= 228 * 1024 ? 2 : 1);
-    a.slots = (int64_t)2 * a.blocks * PT_ROWS * (pool.hs + 4);  // (maxima and totals behind the sums, on 16-byte boundaries)
-    a.whole = s.prefix_len ? (int64_t)s.n_seq * s.n_query * n_heads * (pool.hs + 4) : 0;
-    a.total = a.slots + 2 * a.whole;
+    const int64_t row = pool.hs + 4;  // sums, then maximum and total, on 16-byte boundaries
+    a.slots = (int64_t)2 * a.blocks * PT_ROWS * row;
+    a.whole = a.pre = s.prefix_len ? n_tok * n_heads * row : 0;
+    if (tiled) {
+        const bool wide = type == L2B_TYPE_F32;
+        const int keys = wide ? 64 : 128, nd = (pool.hs + 63) / 64, terms = !wide ? 1 : cache_type == L2B_TYPE_F16 ? 2 : 3;
+        a.cut.streams_share = !wide && rows > PX_ROWS ? 2 : 1;
+        a.cut.tiles = (int)(((int64_t)s.prefix_len + keys - 1) / keys);
+        a.cut.row_tiles = (int)((rows + PX_ROWS * a.cut.streams_share - 1) / (PX_ROWS * a.cut.streams_share));
+        a.cut.units = (int64_t)a.cut.tiles * a.cut.row_tiles * pool.n_kv;
+        a.cut.whole_rows = n_tok * n_heads;
+        a.cut_blocks = a.cut.units < sms ? (int)a.cut.units : sms;
+        a.cut.share = (a.cut.units + a.cut_blocks - 1) / a.cut_blocks;
+        const int queries = terms * a.cut.streams_share * nd * PX_ROWS * 128, stage = 2 * nd * keys * 128;
+        a.stages = (222 * 1024 - queries) / stage;  // (of 227 KB, behind barriers and a start on 1 KB)
+        a.stages = a.stages < PX_MAX_STAGES ? a.stages : PX_MAX_STAGES;
+        a.cut_smem = queries + a.stages * stage + 1024;
+        a.cut_slots = (int64_t)2 * a.cut_blocks * 2 * PX_ROWS * row;
+        a.pre *= 2 / a.cut.streams_share;
+    }
+    a.total = a.slots + a.whole + a.cut_slots + a.pre;
     return a;
+}
+
+// Pages as rows of 64 values and as many slots as a tile takes of a page; `slots`: how many of a page's slots there are.
+int32_t encode_pages(CUtensorMap* map, void* pages, const PagedPool& p, int cache_type, int keys, int slots) {
+    const EncodeTiledFn fn = encode_tiled_fn();
+    if (!fn) return fail(L2B_ERR_CUDA, "cuTensorMapEncodeTiled is not available");
+    const int page = 1 << p.page_shift;
+    const cuuint64_t dims[3] = {(cuuint64_t)p.hs, (cuuint64_t)slots, (cuuint64_t)p.n_pages * p.n_kv}, strides[2] = {(cuuint64_t)p.hs * 2, (cuuint64_t)p.hs * 2 * page};
+    const cuuint32_t box[3] = {64, (cuuint32_t)(page < keys ? page : keys), 1}, one[3] = {1, 1, 1};
+    if (fn(map, cache_type == L2B_TYPE_F16 ? CU_TENSOR_MAP_DATA_TYPE_FLOAT16 : CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, 3, pages, dims, strides, box, one, CU_TENSOR_MAP_INTERLEAVE_NONE,
+           CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) != CUDA_SUCCESS)
+        return fail(L2B_ERR_CUDA, "cuTensorMapEncodeTiled failed");
+    return L2B_OK;
 }
 
 int32_t check_queries(const l2b_paged_cache* c, const l2b_paged_queries* q, const PagedSeqs& s) {
@@ -215,7 +254,7 @@ extern "C" int32_t l2b_paged_attention_workspace(const l2b_paged_cache* cache, c
     L2B_TRY(on.enter(cache->dev_k, "dev_k"));
     int sms = 0;
     L2B_TRY(sm_count(on.device, &sms));
-    *bytes = attention_plan(pool, seqs, queries->n_heads, sms).total * 4;
+    *bytes = attention_plan(pool, seqs, queries->n_heads, queries->type, cache->type, sms).total * 4;
     return L2B_OK;
 }
 
@@ -235,14 +274,15 @@ extern "C" int32_t l2b_paged_attention_device(const l2b_paged_cache* cache, cons
     if (p.seqs.n_seq == 0) return L2B_OK;
     int sms = 0;
     L2B_TRY(sm_count(on.device, &sms));
-    const AttnPlan plan = attention_plan(p.pool, p.seqs, queries->n_heads, sms);
+    const AttnPlan plan = attention_plan(p.pool, p.seqs, queries->n_heads, queries->type, cache->type, sms);
     if (!dev_workspace || !aligned(dev_workspace) || workspace_bytes < plan.total * 4)
         return fail(L2B_ERR_BAD_ARG, "the workspace must lie on a 16-byte boundary and hold l2b_paged_attention_workspace bytes");
     p.q = queries->dev_q; p.out = queries->dev_out; p.q_stride = queries->q_stride; p.out_stride = queries->out_stride;
     p.n_heads = queries->n_heads;
     p.group = queries->n_heads / p.pool.n_kv;
     p.scale2 = (queries->scale != 0.f ? queries->scale : 1.f / sqrtf((float)hs)) * 1.4426950408889634f;
-    p.thin_prefix = p.seqs.prefix_len > 0;
+    p.thin_prefix = plan.thin_prefix;
+    p.cut = plan.cut;
     p.blocks = plan.blocks;
     float* const w = (float*)dev_workspace;
     const int64_t n_rows = (int64_t)p.seqs.n_seq * p.seqs.n_query * p.n_heads;
@@ -251,13 +291,45 @@ extern "C" int32_t l2b_paged_attention_device(const l2b_paged_cache* cache, cons
     if (p.seqs.prefix_len) {
         p.own_acc = w + plan.slots;
         p.own_ml = p.own_acc + n_rows * hs;
-        p.pre_acc = w + plan.slots + plan.whole;
-        p.pre_ml = p.pre_acc + n_rows * hs;
+        p.cut_acc = p.own_acc + plan.whole;
+        p.cut_ml = p.cut_acc + (int64_t)2 * plan.cut_blocks * 2 * PX_ROWS * hs;
+        p.pre_acc = p.cut_acc + plan.cut_slots;
+        p.pre_ml = p.pre_acc + n_rows * hs * (plan.cut.streams_share == 1 ? 2 : 1);
     }
     cudaStream_t st = (cudaStream_t)stream;
     L2B_TRY(by_types(cache->type, queries->type, [&](auto t, auto io) -> int32_t {
         using T = decltype(t);
         using TIO = decltype(io);
+        if (plan.cut.units > 0) {
+            PrefixParams x;
+            memset(&x, 0, sizeof(x));
+            static_cast<PagedWork&>(x) = p;
+            x.q = p.q; x.q_stride = p.q_stride; x.n_heads = p.n_heads;
+            x.rows = p.seqs.n_seq * p.seqs.n_query * p.group;
+            x.stages = plan.stages;
+            x.scale2 = fabsf(p.scale2);
+            x.negate = p.scale2 < 0.f;
+            x.cut = plan.cut;
+            x.slot_acc = p.cut_acc; x.slot_ml = p.cut_ml; x.pre_acc = p.pre_acc; x.pre_ml = p.pre_ml;
+            const int keys = sizeof(TIO) == 4 ? 64 : 128, page = 1 << p.pool.page_shift;
+            CUtensorMap mk, mv, me;
+            L2B_TRY(encode_pages(&mk, p.pool.k, p.pool, cache->type, keys, page));
+            L2B_TRY(encode_pages(&mv, p.pool.v, p.pool, cache->type, keys, page));
+            L2B_TRY(encode_pages(&me, p.pool.v, p.pool, cache->type, keys, (p.seqs.prefix_len - 1) % page + 1));
+            auto tiled = [&](auto tiles) -> int32_t {
+                constexpr int TILES = decltype(tiles)::value;
+                L2B_TRY((allow_smem<paged_prefix_kernel<T, TIO, TILES>>(on.device)));
+                CU(launch_kernel_args(paged_prefix_kernel<T, TIO, TILES>, dim3((unsigned)plan.cut_blocks), dim3(PX_THREADS), (size_t)plan.cut_smem, st, true, 1, x, mk, mv, me));
+                return L2B_OK;
+            };
+            if constexpr (sizeof(TIO) == 4) {
+                L2B_TRY(tiled(std::integral_constant<int, 1>()));
+            } else if (plan.cut.streams_share == 2) {
+                L2B_TRY(tiled(std::integral_constant<int, 2>()));
+            } else {
+                L2B_TRY(tiled(std::integral_constant<int, 1>()));
+            }
+        }
         auto go = [&](auto ks) -> int32_t {
             constexpr int KS = decltype(ks)::value;
             L2B_TRY((allow_smem<paged_attention_kernel<T, TIO, KS>>(on.device)));
