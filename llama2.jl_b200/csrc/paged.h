@@ -34,20 +34,21 @@ L2B_HD int64_t paged_offset(int page, int head, int slot, const PagedPool& p) {
 }
 
 // The attention's work in units of one tile of keys: items (a tile of rows of one key/value head of one group, a group being a sequence or the
-// shared prefix) lie one behind the other, each as long as its group has key tiles, and block c of n takes units c * share ..  An item that falls into
-// one block is done there; of a longer one each block leaves a partial result: the block in which it begins in its second slot, the others in their
-// first.  A block has at most one item of either kind.
+// shared prefix) lie one behind the other, each as long as its group has key tiles, and worker c of n (a warp, or a block) takes units c * share ..  An item that
+// falls into one share is done there; of a longer one each worker leaves a partial result: the one with which it begins in its second slot, the others
+// in their first.  A worker has at most one item of either kind.
 struct PagedShares {
     int64_t units, share;
 };
-L2B_HD PagedShares paged_shares(int64_t units, int blocks) {
+L2B_HD PagedShares paged_shares(int64_t units, int workers, int least) {
     PagedShares s;
     s.units = units;
-    s.share = units > 0 ? (units + blocks - 1) / blocks : 1;
+    s.share = (units + workers - 1) / workers;
+    if (s.share < least) s.share = least;
     return s;
 }
 struct PagedParts {
-    int first, last;  // blocks
+    int first, last;  // workers
 };
 L2B_HD PagedParts paged_parts(int64_t begin, int tiles, int64_t share) {
     PagedParts p;
@@ -55,7 +56,7 @@ L2B_HD PagedParts paged_parts(int64_t begin, int tiles, int64_t share) {
     p.last = (int)((begin + tiles - 1) / share);
     return p;
 }
-L2B_HD int paged_slot(const PagedParts& p, int block) { return 2 * block + (block == p.first ? 1 : 0); }
+L2B_HD int paged_slot(const PagedParts& p, int worker) { return 2 * worker + (worker == p.first ? 1 : 0); }
 
 
 // How the prefix's kernel cuts its work: row tiles of `streams_share` * 128 rows; streams_share 2: two row tiles on the same keys, 1: one, whose keys
@@ -65,7 +66,7 @@ struct PrefixCut {
     int tiles, row_tiles, streams_share;
 };
 
-constexpr int PT_KEYS = 64, PT_ROWS = 16;  // a tile
+constexpr int PT_KEYS = 16, PT_ROWS = 16;  // a tile of the own parts' kernel
 
 // Rows of a group are the query heads of one key/value head, of all the group's rows one after the other.  Groups: the prefix first where it is one
 // (thin_prefix), then the sequences.
@@ -78,37 +79,36 @@ struct PagedWork {
 struct GroupShape {
     int keys, tiles, row_tiles;
 };
-L2B_HD GroupShape group_shape(const PagedWork& p, int g) {
+L2B_HD GroupShape group_shape(const PagedWork& p, int g, int length) {  // length: of the sequence; none of the prefix
     GroupShape s;
-    if (p.thin_prefix && g == 0) {
-        s.keys = p.seqs.prefix_len;
-        s.row_tiles = (int)(((int64_t)p.seqs.n_seq * p.seqs.n_query * p.group + PT_ROWS - 1) / PT_ROWS);
-    } else {
-        s.keys = paged_keys(p.seqs.lengths[g - p.thin_prefix], p.seqs.width, p.pool.page_shift);
-        s.row_tiles = (int)(((int64_t)p.seqs.n_query * p.group + PT_ROWS - 1) / PT_ROWS);
-    }
+    const bool pre = p.thin_prefix && g == 0;
+    s.keys = pre ? p.seqs.prefix_len : paged_keys(length, p.seqs.width, p.pool.page_shift);
+    s.row_tiles = (int)(((int64_t)(pre ? p.seqs.n_seq : 1) * p.seqs.n_query * p.group + PT_ROWS - 1) / PT_ROWS);
     s.tiles = (int)(((int64_t)s.keys + PT_KEYS - 1) / PT_KEYS);
     return s;
 }
+L2B_HD int group_length(const PagedWork& p, int g) { return p.thin_prefix && g == 0 ? 0 : p.seqs.lengths[g - p.thin_prefix]; }
+L2B_HD GroupShape group_shape(const PagedWork& p, int g) { return group_shape(p, g, group_length(p, g)); }
 L2B_HD int64_t group_units(const PagedWork& p, const GroupShape& s) { return (int64_t)s.tiles * s.row_tiles * p.pool.n_kv; }
 
-// A place in a block's share: unit `tile` of item `item` (key/value head * row_tiles + row tile) of group `g`.
+// A place in a worker's share: unit `tile` of item `item` (key/value head * row_tiles + row tile) of group `g`.
 struct Cursor {
     int g, item, tile;
     GroupShape s;
     int64_t left;  // units of the share from here on
 };
-L2B_HD Cursor cursor_at(const PagedWork& p, int g, int64_t unit_of_group, int64_t left) {
+L2B_HD Cursor cursor_at(const PagedWork& p, int g, const GroupShape& s, int64_t unit_of_group, int64_t left) {
     Cursor c;
     c.g = g;
-    c.s = group_shape(p, g);
-    c.item = (int)(unit_of_group / c.s.tiles);
-    c.tile = (int)(unit_of_group % c.s.tiles);
+    c.s = s;
+    c.item = (int)(unit_of_group / s.tiles);
+    c.tile = (int)(unit_of_group % s.tiles);
     c.left = left;
     return c;
 }
-// `tiles` of the item on, to the next item (of a group that has any) at its end.
-L2B_HD void next_item(const PagedWork& p, Cursor& c, int tiles) {
+// `tiles` of the item on, to the next item (of a group that has any) at its end.  length(g): as group_length.
+template <class Length>
+L2B_HD void next_item(const PagedWork& p, Cursor& c, int tiles, Length&& length) {
     c.left -= tiles;
     c.tile += tiles;
     if (c.tile < c.s.tiles) return;
@@ -117,9 +117,8 @@ L2B_HD void next_item(const PagedWork& p, Cursor& c, int tiles) {
     c.item = 0;
     while (c.left > 0) {
         if (++c.g >= p.seqs.n_seq + p.thin_prefix) c.left = 0;  // (not while the lengths are what they were)
-        else if ((c.s = group_shape(p, c.g)).tiles > 0) return;
+        else if ((c.s = group_shape(p, c.g, length(c.g))).tiles > 0) return;
     }
 }
-L2B_HD void next_tile(const PagedWork& p, Cursor& c) { next_item(p, c, 1); }
 
 }  // namespace l2b

@@ -2,11 +2,11 @@
 // sequence's own positions up to the token's.
 //
 // Rows: the query heads of one key/value head, of all new tokens of a group (a sequence, or all of them for the prefix), in tiles of 16: the M of
-// m16n8k16.  What a step of single tokens reads is the cache, once, so memory bounds it; the work is cut into equal shares of 64-key tiles over all
-// blocks whatever the sequences' lengths (paged.h), and the partial results (f32 sums, each row's maximum and total) are joined by a second kernel.
-// A block is four warps, each with 16 keys of a tile, its own ring of asynchronous 16-byte copies and its own running maximum, total and sums: the
-// warps meet at an item's end only.  Copies run ahead over the ends of items.  Rows of keys and values lie 16 bytes further apart in shared memory than
-// they are long, so that ldmatrix reads eight rows without bank conflicts.
+// m16n8k16.  What a step of single tokens reads is the cache, once, so memory bounds it; the work is cut into equal shares of 16-key tiles over all
+// warps whatever the sequences' lengths (paged.h), and the partial results (f32 sums, each row's maximum and total) are joined by a second kernel.
+// Every warp works by itself: its own share, its own ring of asynchronous 16-byte copies, its own running maximum, total and sums; there is no barrier.  Copies run
+// ahead over the ends of items; the page of a tile's keys is looked up one tile before it is needed, and the lengths of 32 sequences at a time.  Rows
+// of keys and values lie 16 bytes further apart in shared memory than they are long, so that ldmatrix reads eight rows without bank conflicts.
 //
 // f32 rows over a 16-bit cache: a query and a weight are split into terms of the cache's type (three of bf16, two of f16, the query's behind a power of two
 // per row), which keeps the products' error at 2^-22 or less.  For 16-bit rows the weights are rounded once to the cache's type (at most
@@ -18,7 +18,7 @@
 
 namespace l2b {
 
-constexpr int PT_WARPS = 4, PT_WKEYS = PT_KEYS / PT_WARPS, PT_STAGES = 3;
+constexpr int PT_WARPS = 4, PT_STAGES = 3, PT_LEAST = 2;
 
 struct PagedAttnParams : PagedWork {
     const void* q;
@@ -26,9 +26,10 @@ struct PagedAttnParams : PagedWork {
     int64_t q_stride, out_stride;
     int n_heads;
     float scale2;          // scale * log2(e)
-    int blocks;            // of the own parts' kernel
-    float *slot_acc, *slot_ml;  // [2 * blocks][16][hs], [2 * blocks][16][2]
-    float *own_acc, *own_ml;    // items that one block did: [rows * n_heads][hs], [..][2]; null where nothing else is to be joined
+    int workers;                // warps of the own parts' kernel
+    int slot_rows;              // rows of a slot: 16, or fewer when no tile has as many
+    float *slot_acc, *slot_ml;  // [2 * workers][slot_rows][hs], [..][2]
+    float *own_acc, *own_ml;    // items that one warp did: [rows * n_heads][hs], [..][2]; null where nothing else is to be joined
     float *pre_acc, *pre_ml;    // the same of the prefix
     PrefixCut cut;              // of the prefix's kernel (paged_prefix.cuh), which may be running still
     float *cut_acc, *cut_ml;    // its slots: [2 * blocks][2][128][hs], [..][2]
@@ -83,23 +84,31 @@ struct ThinTraits {
     static constexpr bool WIDE = sizeof(TIO) == 4;
     static constexpr int QT = !WIDE ? 1 : sizeof(T) == 2 && std::is_same<T, __half>::value ? 2 : 3, PT = QT;
     static constexpr int PITCH = KS * 32 + 16;               // bytes of a row in shared memory
-    static constexpr int HALF_STAGE = PT_WKEYS * PITCH;      // keys of a stage, or values
+    static constexpr int HALF_STAGE = PT_KEYS * PITCH;      // keys of a stage, or values
     static constexpr int RING = PT_WARPS * PT_STAGES * 2 * HALF_STAGE;
 };
-// shared memory: the rings, then each warp's sums, maxima and totals of up to 16 rows
-template <typename TR>
-__host__ __device__ constexpr int thin_smem(int hs, int rows) { return TR::RING + PT_WARPS * rows * (hs + 2) * 4; }
+// The sequences' lengths as a warp needs them one after the other: 32 at a time.
+struct Lengths {
+    int base, mine;
+    __device__ __forceinline__ int operator()(const PagedWork& p, int g) {
+        if (g < base || g >= base + 32) {
+            const int lane = threadIdx.x & 31;
+            base = g;
+            mine = g + lane < p.seqs.n_seq + p.thin_prefix ? group_length(p, g + lane) : 0;
+        }
+        return __shfl_sync(0xffffffffu, mine, g - base);
+    }
+};
 
 template <typename T, typename TIO, int KS>
 __global__ void __launch_bounds__(PT_WARPS * 32, 2) paged_attention_kernel(const __grid_constant__ PagedAttnParams p) {
     using TR = ThinTraits<T, TIO, KS>;
     extern __shared__ __align__(16) uint8_t pt_smem[];
     const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, hs = p.pool.hs, chunks = hs / 8, groups = p.seqs.n_seq + p.thin_prefix;
+    const int worker = warp * (int)gridDim.x + (int)blockIdx.x;  // (few shares: spread over the SMs)
     uint8_t* const ring = pt_smem + warp * PT_STAGES * 2 * TR::HALF_STAGE;
-    const int most_rows = min(PT_ROWS, p.seqs.n_query * p.group * (p.thin_prefix ? p.seqs.n_seq : 1));
-    float* const merge = reinterpret_cast<float*>(pt_smem + TR::RING);
     // the values between a head's end and the next multiple of 32: zero once and for all
-    for (int i = lane; i < PT_STAGES * 2 * PT_WKEYS * (KS * 2 - chunks); i += 32) {
+    for (int i = lane; i < PT_STAGES * 2 * PT_KEYS * (KS * 2 - chunks); i += 32) {
         const int r = i / (KS * 2 - chunks), ch = chunks + i % (KS * 2 - chunks);
         *reinterpret_cast<uint4*>(ring + r * TR::PITCH + ch * 16) = make_uint4(0, 0, 0, 0);
     }
@@ -109,12 +118,12 @@ __global__ void __launch_bounds__(PT_WARPS * 32, 2) paged_attention_kernel(const
     if (!late) pdl_wait();
     pdl_launch_dependents();  // (behind a wait, here or there: the joining kernel reads the lengths before it waits itself)
 
-    // this block's share; every warp finds it for itself
+    // this warp's share
     int64_t units = 0;
     for (int g = lane; g < groups; g += 32) units += group_units(p, group_shape(p, g));
     for (int o = 16; o > 0; o >>= 1) units += __shfl_xor_sync(0xffffffffu, units, o);
-    const PagedShares sh = paged_shares(units, p.blocks);
-    const int64_t begin = (int64_t)blockIdx.x * sh.share;
+    const PagedShares sh = paged_shares(units, p.workers, PT_LEAST);
+    const int64_t begin = worker * sh.share;
     Cursor at;
     at.left = 0;
     if (begin < units) {
@@ -136,23 +145,30 @@ __global__ void __launch_bounds__(PT_WARPS * 32, 2) paged_attention_kernel(const
                 sum += __shfl_sync(0xffffffffu, inc, 31);
             }
         }
-        if (found >= 0) at = cursor_at(p, found, begin - sum, min(sh.share, units - begin));
+        if (found >= 0) at = cursor_at(p, found, group_shape(p, found), begin - sum, min(sh.share, units - begin));
     }
+    Lengths ahead_lengths = {-64, 0}, at_lengths = {-64, 0};
 
     Cursor ahead = at;
     uint64_t seen = 0;  // 16 bits per stage under way: which of its keys are there
     int in_flight = 0, put_stage = 0, get_stage = 0;
-    auto load = [&]() {  // the next tile's 16 keys and values of this warp, or an empty group of copies
+    int page = -1;  // of this lane's key of the tile that is copied next
+    auto look_up = [&]() {
+        const int key = ahead.tile * PT_KEYS + (lane & 15);
+        page = -1;
+        if (ahead.left > 0 && key < ahead.s.keys)
+            page = p.thin_prefix && ahead.g == 0 ? p.seqs.prefix_pages[key >> p.pool.page_shift] : p.seqs.pages[(int64_t)(ahead.g - p.thin_prefix) * p.seqs.width + (key >> p.pool.page_shift)];
+    };
+    look_up();
+    auto load = [&]() {  // the next tile's 16 keys and values, or an empty group of copies
         if (ahead.left > 0) {
-            const bool pre = p.thin_prefix && ahead.g == 0;
-            const int kv = ahead.item / ahead.s.row_tiles, key = ahead.tile * PT_KEYS + warp * PT_WKEYS + (lane & 15);
-            int page = -1;
-            if (key < ahead.s.keys)
-                page = pre ? p.seqs.prefix_pages[key >> p.pool.page_shift] : p.seqs.pages[(int64_t)(ahead.g - p.thin_prefix) * p.seqs.width + (key >> p.pool.page_shift)];
+            const int kv = ahead.item / ahead.s.row_tiles, key = ahead.tile * PT_KEYS + (lane & 15);
             const bool there = page >= 0 && page < p.pool.n_pages;
             seen |= (uint64_t)(__ballot_sync(0xffffffffu, there) & 0xffffu) << (16 * in_flight);
             const int64_t off = there ? paged_offset(page, kv, key & ((1 << p.pool.page_shift) - 1), p.pool) : 0;
             uint8_t* const st = ring + put_stage * 2 * TR::HALF_STAGE;
+            next_item(p, ahead, 1, [&](int g) { return ahead_lengths(p, g); });
+            look_up();
 #pragma unroll
             for (int i = 0; i < KS; ++i) {
                 const int r = (i * 32 + lane) / (KS * 2), ch = (i * 32 + lane) % (KS * 2);
@@ -163,7 +179,6 @@ __global__ void __launch_bounds__(PT_WARPS * 32, 2) paged_attention_kernel(const
                     cp_async16(st + TR::HALF_STAGE + r * TR::PITCH + ch * 16, (const T*)p.pool.v + o + ch * 8, real);
                 }
             }
-            next_tile(p, ahead);
         }
         cp_async_commit();
         ++in_flight;
@@ -174,7 +189,7 @@ __global__ void __launch_bounds__(PT_WARPS * 32, 2) paged_attention_kernel(const
 
     const int r0 = lane >> 2, c0 = (lane & 3) * 2;
     while (at.left > 0) {
-        // one item, or as much of it as is this block's
+        // one item, or as much of it as is this warp's
         const bool pre = p.thin_prefix && at.g == 0;
         const int kv = at.item / at.s.row_tiles, row_tile = at.item - kv * at.s.row_tiles, first_tile = at.tile;
         const int tiles = (int)min((int64_t)(at.s.tiles - at.tile), at.left);
@@ -195,13 +210,9 @@ __global__ void __launch_bounds__(PT_WARPS * 32, 2) paged_attention_kernel(const
                 head[i] = kv * p.group + r - t * p.group;
                 lim[i] = -1;
                 low[i] = 0x7fffffff;
-                if (r0 + 8 * i < n_rows) {
-                    const int seq = seq0 + t / p.seqs.n_query, j = t % p.seqs.n_query, length = p.seqs.lengths[seq];
-                    const int count = paged_count(length, p.seqs.counts ? p.seqs.counts[seq] : p.seqs.n_query, p.seqs.n_query);
-                    if (j < count) low[i] = lim[i] = pre ? p.seqs.prefix_len - 1 : length - count + j;
-                }
+                const bool any = r0 + 8 * i < n_rows;  // (other rows: zeros do)
+                const int seq = any ? seq0 + t / p.seqs.n_query : 0, j = t % p.seqs.n_query, length = p.seqs.lengths[seq], given = p.seqs.counts ? p.seqs.counts[seq] : p.seqs.n_query;
                 const TIO* const src = (const TIO*)p.q + token[i] * p.q_stride + (int64_t)head[i] * hs;
-                const bool any = lim[i] >= 0;  // (a row without keys here: zeros do)
 #pragma unroll
                 for (int ks = 0; ks < KS; ++ks) {
 #pragma unroll
@@ -213,6 +224,8 @@ __global__ void __launch_bounds__(PT_WARPS * 32, 2) paged_attention_kernel(const
                         qv[i][ks][2 * h + 1] = x[1];
                     }
                 }
+                const int count = paged_count(length, given, p.seqs.n_query);
+                if (any && j < count) low[i] = lim[i] = pre ? p.seqs.prefix_len - 1 : length - count + j;
                 if (TR::WIDE && std::is_same<T, __half>::value) {  // f16 terms: the row's largest value between 1/2 and 1
                     float mx = 0.f;
 #pragma unroll
@@ -262,7 +275,7 @@ __global__ void __launch_bounds__(PT_WARPS * 32, 2) paged_attention_kernel(const
             const uint8_t* const sk = ring + get_stage * 2 * TR::HALF_STAGE;
             const uint8_t* const sv = sk + TR::HALF_STAGE;
             get_stage = get_stage + 1 == PT_STAGES ? 0 : get_stage + 1;
-            const int k0 = tile * PT_KEYS + warp * PT_WKEYS;
+            const int k0 = tile * PT_KEYS;
             if (k0 > most || !there) {  // nobody sees any of it
                 __syncwarp();
                 continue;
@@ -278,7 +291,7 @@ __global__ void __launch_bounds__(PT_WARPS * 32, 2) paged_attention_kernel(const
                     mma16<T>(s[1], qa[t][ks], b[2], b[3]);
                 }
             }
-            const bool cut = there != 0xffffu || k0 + PT_WKEYS - 1 > least;
+            const bool cut = there != 0xffffu || k0 + PT_KEYS - 1 > least;
 #pragma unroll
             for (int n = 0; n < 2; ++n)
 #pragma unroll
@@ -321,8 +334,8 @@ __global__ void __launch_bounds__(PT_WARPS * 32, 2) paged_attention_kernel(const
                 }
             // A key that one row sees and another does not may hold values that are no numbers: then no product, 0 * inf would spread.
             bool odd = false;
-            if (k0 + PT_WKEYS - 1 > least) {
-                for (int i = lane; i < PT_WKEYS * KS * 2 && !odd; i += 32) {
+            if (k0 + PT_KEYS - 1 > least) {
+                for (int i = lane; i < PT_KEYS * KS * 2 && !odd; i += 32) {
                     const T* v = reinterpret_cast<const T*>(sv + i / (KS * 2) * TR::PITCH + i % (KS * 2) * 16);
                     for (int e = 0; e < 8; ++e) odd |= !(fabsf(to_f32(v[e])) < INFINITY);
                 }
@@ -348,7 +361,7 @@ __global__ void __launch_bounds__(PT_WARPS * 32, 2) paged_attention_kernel(const
                     }
                 }
             } else {
-                for (int key = 0; key < PT_WKEYS; ++key) {
+                for (int key = 0; key < PT_KEYS; ++key) {
                     const int src = (lane & ~3) | ((key & 7) >> 1);
                     float wk[2];
 #pragma unroll
@@ -367,97 +380,47 @@ __global__ void __launch_bounds__(PT_WARPS * 32, 2) paged_attention_kernel(const
             __syncwarp();  // the stage may be written again
         }
 
-        // the warps' results together
-#pragma unroll
-        for (int i = 0; i < 2; ++i) {
-            l[i] += __shfl_xor_sync(0xffffffffu, l[i], 1);
-            l[i] += __shfl_xor_sync(0xffffffffu, l[i], 2);
-            if (l[i] != l[i] && m[i] == -INFINITY) m[i] = 0.f;  // scores that are no numbers are not an empty row
-        }
-        __syncthreads();  // (the last item's have been read)
+        // the rows' results: done, or to the workspace
+        const bool whole = first_tile == 0 && ends;
+        float* const whole_acc = pre ? p.pre_acc : p.own_acc;
+        float* const whole_ml = pre ? p.pre_ml : p.own_ml;
 #pragma unroll
         for (int i = 0; i < 2; ++i) {
             const int r = r0 + 8 * i;
-            if (r < most_rows) {
-                float* const row = merge + (warp * most_rows + r) * (hs + 2);
-#pragma unroll
-                for (int n = 0; n < KS * 2; ++n)
-                    if (n * 8 < hs) {
-                        row[n * 8 + c0] = acc[n][2 * i];
-                        row[n * 8 + c0 + 1] = acc[n][2 * i + 1];
-                    }
-                if ((lane & 3) == 0) {
-                    row[hs] = m[i];
-                    row[hs + 1] = l[i];
-                }
-            }
-        }
-        __syncthreads();
-        const bool whole = first_tile == 0 && ends;
-        const int slot = 2 * (int)blockIdx.x + (first_tile == 0 ? 1 : 0);
-        float* const whole_acc = pre ? p.pre_acc : p.own_acc;
-        float* const whole_ml = pre ? p.pre_ml : p.own_ml;
-        for (int i = threadIdx.x; i < n_rows * chunks * 2; i += PT_WARPS * 32) {  // four values each
-            const int r = i / (chunks * 2), d = (i - r * chunks * 2) * 4;
-            float mw[PT_WARPS], top = -INFINITY, sum = 0.f, o[4] = {};
-#pragma unroll
-            for (int w = 0; w < PT_WARPS; ++w) {
-                mw[w] = merge[(w * most_rows + r) * (hs + 2) + hs];
-                top = fmaxf(top, mw[w]);
-            }
-#pragma unroll
-            for (int w = 0; w < PT_WARPS; ++w) {
-                const float* const row = merge + (w * most_rows + r) * (hs + 2);
-                const float f = mw[w] == -INFINITY ? 0.f : exp2_approx(mw[w] - top);
-                sum = fmaf(f, row[hs + 1], sum);
-#pragma unroll
-                for (int e = 0; e < 4; ++e) o[e] += mw[w] == -INFINITY ? 0.f : f * row[d + e];
-            }
-            const int rr = row_tile * PT_ROWS + r, t = rr / p.group;
-            const int64_t tok = (int64_t)seq0 * p.seqs.n_query + t;
-            const int h = kv * p.group + rr - t * p.group;
+            l[i] += __shfl_xor_sync(0xffffffffu, l[i], 1);
+            l[i] += __shfl_xor_sync(0xffffffffu, l[i], 2);
+            if (l[i] != l[i] && m[i] == -INFINITY) m[i] = 0.f;  // scores that are no numbers are not an empty row
+            if (r >= n_rows) continue;
             if (whole && !whole_acc) {  // all there is of these rows
-                const int length = p.seqs.lengths[seq0];
-                if (t < paged_count(length, p.seqs.counts ? p.seqs.counts[seq0] : p.seqs.n_query, p.seqs.n_query)) {
-                    const float inv = sum > 0.f ? 1.f / sum : sum == 0.f ? 0.f : sum;
+                if (low[i] == 0x7fffffff) continue;  // (no token)
+                const float inv = l[i] > 0.f ? 1.f / l[i] : l[i] == 0.f ? 0.f : l[i];
+                TIO* const dst = (TIO*)p.out + token[i] * p.out_stride + (int64_t)head[i] * hs;
 #pragma unroll
-                    for (int e = 0; e < 4; ++e) o[e] *= inv;
-                    put((TIO*)p.out + tok * p.out_stride + (int64_t)h * hs + d, o);
+                for (int n = 0; n < KS * 2; ++n) {
+                    const float o[2] = {acc[n][2 * i] * inv, acc[n][2 * i + 1] * inv};
+                    if (n * 8 < hs) put(dst + n * 8 + c0, o);
                 }
             } else {
-                const int64_t at_row = whole ? tok * p.n_heads + h : (int64_t)slot * PT_ROWS + r;
-                *reinterpret_cast<float4*>((whole ? whole_acc : p.slot_acc) + at_row * hs + d) = make_float4(o[0], o[1], o[2], o[3]);
-                if (d == 0) *reinterpret_cast<float2*>((whole ? whole_ml : p.slot_ml) + at_row * 2) = make_float2(top, sum);
+                const int64_t at_row = whole ? token[i] * p.n_heads + head[i] : (int64_t)(2 * worker + (first_tile == 0 ? 1 : 0)) * p.slot_rows + r;
+                float* const dst = (whole ? whole_acc : p.slot_acc) + at_row * hs;
+#pragma unroll
+                for (int n = 0; n < KS * 2; ++n)
+                    if (n * 8 < hs) *reinterpret_cast<float2*>(dst + n * 8 + c0) = make_float2(acc[n][2 * i], acc[n][2 * i + 1]);
+                if ((lane & 3) == 0) *reinterpret_cast<float2*>((whole ? whole_ml : p.slot_ml) + at_row * 2) = make_float2(m[i], l[i]);
             }
         }
-        next_item(p, at, tiles);
+        next_item(p, at, tiles, [&](int g) { return at_lengths(p, g); });
     }
     if (late) pdl_wait();
 }
 
-// Joins the partial results of a row: a block per token and `heads` heads, a warp's lanes along the head's values.  WARPS warps share a row's parts
-// where there are few rows and so many parts of each.
+// Joins the partial results of a row (a token's head): a block per token and `heads` heads.  Lanes look up a part each, its maximum and total; then they
+// lie along the head's values and add the parts up, so that the loads of many parts are under way at once.  Several warps share a row where there are few.
 struct JoinParams {
     PagedAttnParams a;
     int heads;  // of a block
 };
 constexpr int PJ_WARPS = 8;
-
-struct Joined {
-    float m, l, o[4];
-};
-__device__ __forceinline__ void join(Joined& j, float m, float l, const float* acc, bool read) {
-    if (m == -INFINITY) return;
-    const float mn = fmaxf(j.m, m), a = j.m == -INFINITY ? 0.f : exp2_approx(j.m - mn), b = exp2_approx(m - mn);
-    float4 v = make_float4(0.f, 0.f, 0.f, 0.f);
-    if (read) v = __ldcg(reinterpret_cast<const float4*>(acc));
-    j.l = j.l * a + l * b;
-    j.o[0] = j.o[0] * a + v.x * b;
-    j.o[1] = j.o[1] * a + v.y * b;
-    j.o[2] = j.o[2] * a + v.z * b;
-    j.o[3] = j.o[3] * a + v.w * b;
-    j.m = mn;
-}
 
 template <typename TIO>
 __global__ void __launch_bounds__(PJ_WARPS * 32) paged_join_kernel(const __grid_constant__ JoinParams jp) {
@@ -489,75 +452,100 @@ __global__ void __launch_bounds__(PJ_WARPS * 32) paged_join_kernel(const __grid_
         all += s_units[0][w];
         before += s_units[1][w];
     }
-    const PagedShares sh = paged_shares(all, p.blocks);
+    const PagedShares sh = paged_shares(all, p.workers, PT_LEAST);
+    const int per_row = PJ_WARPS / jp.heads, head = blockIdx.y * jp.heads + warp / per_row, sub = warp % per_row;
+    const bool real = head < p.n_heads;
+    const int kv = head / p.group, g = head - kv * p.group, d = lane * 4;
+    const int64_t at_row = tok * p.n_heads + head;
+
+    // the parts of this row: of the prefix's kernel, of the prefix as a group of the own parts' kernel, of the own positions
+    const GroupShape own = group_shape(p, group, length), pre = group_shape(p, 0, length);
+    const int own_row = j * p.group + g, pre_row = (int)(tok * p.group) + g;
+    PagedParts of[3] = {};
+    int n_parts[3] = {};
+    const int per_item = p.cut.streams_share * 128, streams = p.cut.streams_share == 2 ? 1 : 2;
+    if (p.cut.units > 0) {
+        of[0] = paged_parts(((int64_t)kv * p.cut.row_tiles + pre_row / per_item) * p.cut.tiles, p.cut.tiles, p.cut.share);
+        n_parts[0] = (of[0].last - of[0].first + 1) * streams;
+    }
+    if (p.thin_prefix) {
+        of[1] = paged_parts(((int64_t)kv * pre.row_tiles + pre_row / PT_ROWS) * pre.tiles, pre.tiles, sh.share);
+        n_parts[1] = of[1].last - of[1].first + 1;
+    }
+    if (own.tiles > 0) {
+        of[2] = paged_parts(before + ((int64_t)kv * own.row_tiles + own_row / PT_ROWS) * own.tiles, own.tiles, sh.share);
+        n_parts[2] = of[2].last - of[2].first + 1;
+    }
+    const bool done = own.tiles > 0 && n_parts[2] == 1 && !p.own_acc;  // written already
+    const int parts = !real || done ? 0 : n_parts[0] + n_parts[1] + n_parts[2];
     pdl_wait();
     if (j >= count) return;
 
-    const int per_row = PJ_WARPS / jp.heads, head = blockIdx.y * jp.heads + warp / per_row, sub = warp % per_row;
-    const bool real = head < p.n_heads;
-    const int kv = head / p.group, d = lane * 4;
-    const int64_t at_row = tok * p.n_heads + head;
-    Joined r = {-INFINITY, 0.f, {0.f, 0.f, 0.f, 0.f}};
-    bool done = false;
-    auto item = [&](int64_t first_unit, const GroupShape& s, int row, const float* whole_acc, const float* whole_ml) {
-        if (s.tiles == 0) return;
-        const int row_tile = row / PT_ROWS;
-        const int64_t begin = first_unit + ((int64_t)kv * s.row_tiles + row_tile) * s.tiles;
-        const PagedParts parts = paged_parts(begin, s.tiles, sh.share);
-        if (parts.first == parts.last) {
-            if (!whole_acc) done = true;  // written already
-            else if (sub == 0) {
-                const float2 ml = __ldcg(reinterpret_cast<const float2*>(whole_ml + at_row * 2));
-                join(r, ml.x, ml.y, whole_acc + at_row * hs + d, d < hs);
-            }
-            return;
-        }
-        for (int b = parts.first + sub; b <= parts.last; b += per_row) {
-            const int64_t at = (int64_t)paged_slot(parts, b) * PT_ROWS + row % PT_ROWS;
-            const float2 ml = __ldcg(reinterpret_cast<const float2*>(p.slot_ml + at * 2));
-            join(r, ml.x, ml.y, p.slot_acc + at * hs + d, d < hs);
-        }
-    };
-    if (real) {
-        const int g = head - kv * p.group;
-        if (p.cut.units > 0) {
-            const int row = (int)(tok * p.group) + g, per_item = p.cut.streams_share * 128, row_tile = row / per_item, r128 = row % 128;
-            const int i0 = p.cut.streams_share == 2 ? row % per_item / 128 : 0, streams = p.cut.streams_share == 2 ? 1 : 2;
-            const PagedParts parts = paged_parts(((int64_t)kv * p.cut.row_tiles + row_tile) * p.cut.tiles, p.cut.tiles, p.cut.share);
-            const bool whole = parts.first == parts.last;
-            for (int n = sub; n < (parts.last - parts.first + 1) * streams; n += per_row) {
-                const int b = parts.first + n / streams, i = i0 + n % streams;
-                const int64_t at = whole ? (streams == 2 ? i * p.cut.whole_rows : 0) + at_row : ((int64_t)paged_slot(parts, b) * 2 + i) * 128 + r128;
-                const float2 ml = __ldcg(reinterpret_cast<const float2*>((whole ? p.pre_ml : p.cut_ml) + at * 2));
-                join(r, ml.x, ml.y, (whole ? p.pre_acc : p.cut_acc) + at * hs + d, d < hs);
+    float m = -INFINITY, l = 0.f, o[4] = {0.f, 0.f, 0.f, 0.f};
+    for (int first = sub; first < parts; first += 32 * per_row) {  // (the same for the whole warp)
+        int n = first + lane * per_row;
+        const float *acc = nullptr, *ml = nullptr;
+        if (n < parts) {
+            if (n < n_parts[0]) {
+                const int b = of[0].first + n / streams, i = streams == 1 ? pre_row % per_item / 128 : n % streams;
+                const bool whole = of[0].first == of[0].last;
+                const int64_t at = whole ? (streams == 2 ? i * p.cut.whole_rows : 0) + at_row : ((int64_t)paged_slot(of[0], b) * 2 + i) * 128 + pre_row % 128;
+                acc = (whole ? p.pre_acc : p.cut_acc) + at * hs;
+                ml = (whole ? p.pre_ml : p.cut_ml) + at * 2;
+            } else {
+                const bool of_pre = n < n_parts[0] + n_parts[1];
+                const PagedParts& q = of[of_pre ? 1 : 2];
+                const bool whole = q.first == q.last;
+                n -= of_pre ? n_parts[0] : n_parts[0] + n_parts[1];
+                const int64_t at = whole ? at_row : (int64_t)paged_slot(q, q.first + n) * p.slot_rows + (of_pre ? pre_row : own_row) % PT_ROWS;
+                acc = (whole ? of_pre ? p.pre_acc : p.own_acc : p.slot_acc) + at * hs;
+                ml = (whole ? of_pre ? p.pre_ml : p.own_ml : p.slot_ml) + at * 2;
             }
         }
-        if (p.thin_prefix) item(0, group_shape(p, 0), (int)(tok * p.group) + g, p.pre_acc, p.pre_ml);
-        item(before, group_shape(p, group), j * p.group + g, p.own_acc, p.own_ml);
+        float2 v = make_float2(-INFINITY, 0.f);
+        if (ml) v = __ldcg(reinterpret_cast<const float2*>(ml));
+        const float mn = fmaxf(m, warp_max(v.x)), keep = m == -INFINITY ? 0.f : exp2_approx(m - mn), w = v.x == -INFINITY ? 0.f : exp2_approx(v.x - mn);
+        l = l * keep + warp_sum(w * v.y);
+#pragma unroll
+        for (int e = 0; e < 4; ++e) o[e] *= keep;
+        m = mn;
+        const unsigned some = __ballot_sync(0xffffffffu, v.x != -INFINITY);
+        const int last = 32 - __clz(some);
+#pragma unroll 4
+        for (int i = 0; i < last; ++i) {
+            const float wi = __shfl_sync(0xffffffffu, w, i);
+            const float* const a = reinterpret_cast<const float*>(__shfl_sync(0xffffffffu, (unsigned long long)acc, i));
+            if ((some >> i & 1) && d < hs) {
+                const float4 x = __ldcg(reinterpret_cast<const float4*>(a + d));
+                o[0] = fmaf(x.x, wi, o[0]);
+                o[1] = fmaf(x.y, wi, o[1]);
+                o[2] = fmaf(x.z, wi, o[2]);
+                o[3] = fmaf(x.w, wi, o[3]);
+            }
+        }
     }
     if (per_row > 1) {
         if (d < hs)
-            for (int e = 0; e < 4; ++e) s_part[warp][d + e] = r.o[e];
+            for (int e = 0; e < 4; ++e) s_part[warp][d + e] = o[e];
         if (lane == 0) {
-            s_part[warp][hs] = r.m;
-            s_part[warp][hs + 1] = r.l;
+            s_part[warp][hs] = m;
+            s_part[warp][hs + 1] = l;
         }
         __syncthreads();
         if (sub == 0) {
             for (int w = warp + 1; w < warp + per_row; ++w) {
-                const float m = s_part[w][hs], l = s_part[w][hs + 1];
-                if (m == -INFINITY) continue;
-                const float mn = fmaxf(r.m, m), a = r.m == -INFINITY ? 0.f : exp2_approx(r.m - mn), b = exp2_approx(m - mn);
-                r.l = r.l * a + l * b;
-                for (int e = 0; e < 4; ++e) r.o[e] = r.o[e] * a + (d < hs ? s_part[w][d + e] * b : 0.f);
-                r.m = mn;
+                const float mw = s_part[w][hs], lw = s_part[w][hs + 1];
+                if (mw == -INFINITY) continue;
+                const float mn = fmaxf(m, mw), a = m == -INFINITY ? 0.f : exp2_approx(m - mn), b = exp2_approx(mw - mn);
+                l = l * a + lw * b;
+                for (int e = 0; e < 4; ++e) o[e] = o[e] * a + (d < hs ? s_part[w][d + e] * b : 0.f);
+                m = mn;
             }
         }
     }
     if (real && sub == 0 && !done && d < hs) {
-        const float inv = r.l > 0.f ? 1.f / r.l : r.l == 0.f ? 0.f : r.l;
-        float o[4];
-        for (int e = 0; e < 4; ++e) o[e] = r.o[e] * inv;
+        const float inv = l > 0.f ? 1.f / l : l == 0.f ? 0.f : l;
+        for (int e = 0; e < 4; ++e) o[e] *= inv;
         put((TIO*)p.out + tok * p.out_stride + (int64_t)head * hs + d, o);
     }
 }

@@ -37,6 +37,8 @@ struct PrefixTraits {
     static constexpr int QT = !WIDE ? 1 : F16 ? 2 : 3, PT = QT;
     static constexpr int KEYS = WIDE ? 64 : 128;
     static constexpr int SUB_Q = PX_ROWS * 128, SUB_K = KEYS * 128;  // bytes of 64 values of a tile's rows
+    // bytes of Q's place: its terms, or 4 KB for each of the eight warps that take the sums out
+    __host__ __device__ static constexpr int queries(int nd) { return QT * TILES * nd * SUB_Q > 8 * 4096 ? QT * TILES * nd * SUB_Q : 8 * 4096; }
     // instruction descriptors: f32 sums, A and B of T; B's rows along K for P V
     __host__ __device__ static constexpr uint32_t idesc(int n, int b_mn) {
         return (1u << 4) | (F16 ? 0u : (1u << 7) | (1u << 10)) | ((uint32_t)b_mn << 16) | ((uint32_t)(n >> 3) << 17) | ((uint32_t)(PX_ROWS >> 4) << 24);
@@ -53,6 +55,7 @@ template <typename T, typename TIO, int TILES>
 __device__ __forceinline__ void load_queries(const PrefixParams& p, uint8_t* sq, int* s_exp, int kv, int row0, int nd) {
     using TR = PrefixTraits<T, TIO, TILES>;
     const int hs = p.pool.hs, per_row = nd * 8, tid = threadIdx.x;
+#pragma unroll 4
     for (int i = tid; i < TILES * PX_ROWS * per_row; i += 256) {  // (per_row is 8 or 16: a row's threads are of one warp)
         const int r = i / per_row, ch = i - r * per_row, row = row0 + r;
         float x[8] = {};
@@ -100,7 +103,7 @@ __global__ void __launch_bounds__(PX_THREADS, 1) paged_prefix_kernel(const __gri
     uint8_t* const smem = px_raw + ((1024u - (smem_u32(px_raw) & 1023u)) & 1023u);
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, hs = p.pool.hs, nd = (hs + 63) / 64, vn = (hs + 15) / 16 * 16;
     uint8_t* const sq = smem;
-    uint8_t* const sk = smem + TR::QT * TILES * nd * TR::SUB_Q;
+    uint8_t* const sk = smem + TR::queries(nd);
     uint8_t* const sv = sk + p.stages * nd * TR::SUB_K;
     if (threadIdx.x == 0) {
         for (int i = 0; i < p.stages; ++i) {
@@ -262,8 +265,8 @@ __global__ void __launch_bounds__(PX_THREADS, 1) paged_prefix_kernel(const __gri
             bool some = false;
             for (int t = TILES == 2 ? 0 : i; t < n; t += TILES == 2 ? 1 : 2) {
                 const int gt = g + t;
-                if (ok) ok = mbar_wait_warp(s_mask + gt % PX_RING, (uint32_t)(gt / PX_RING & 1));
-                if (ok) ok = mbar_wait_warp(s_s + i, (uint32_t)(ns & 1));
+                if (ok) ok = __all_sync(0xffffffffu, mbar_wait_bounded(s_mask + gt % PX_RING, (uint32_t)(gt / PX_RING & 1)));
+                if (ok) ok = __all_sync(0xffffffffu, mbar_wait_bounded(s_s + i, (uint32_t)(ns & 1)));
                 ++ns;
                 tc_fence_after();
                 float x[KEYS];
@@ -323,7 +326,7 @@ __global__ void __launch_bounds__(PX_THREADS, 1) paged_prefix_kernel(const __gri
                 if (lane == 0) mbar_arrive(s_p + i);
             }
             // the segment's products are all done: this row's sums to the workspace
-            if (ok) ok = mbar_wait_warp(&s_seg, (uint32_t)(segment & 1));
+            if (ok) ok = __all_sync(0xffffffffu, mbar_wait_bounded(&s_seg, (uint32_t)(segment & 1)));
             tc_fence_after();
             if (l != l && m == -INFINITY) m = 0.f;  // scores that are no numbers are not an empty row
             if (!ok) {
@@ -340,17 +343,27 @@ __global__ void __launch_bounds__(PX_THREADS, 1) paged_prefix_kernel(const __gri
                 at = ((int64_t)(2 * blockIdx.x + (first_tile == 0 ? 1 : 0)) * 2 + i) * PX_ROWS + r;
             }
             if (real) *reinterpret_cast<float2*>((whole ? p.pre_ml : p.slot_ml) + at * 2) = make_float2(m, l);
+            // The sums go through shared memory, in Q's place, so that a row's 32 values are written together: 4 KB per warp, 16-byte chunks swizzled.
             if (some) {  // (the same for the whole warp)
-                float* const acc = (whole ? p.pre_acc : p.slot_acc) + at * hs;
+                float* const acc = whole ? p.pre_acc : p.slot_acc;
+                uint8_t* const st = sq + warp * 4096;
 #pragma unroll 1
-                for (int c = 0; c < vn; c += 32) {
+                for (int c = 0; c < hs; c += 32) {
                     float o[32];
                     tmem_ld32f(to + (uint32_t)c, o);
 #pragma unroll
-                    for (int e = 0; e < 32; e += 4)
-                        if (real && c + e < hs) *reinterpret_cast<float4*>(acc + c + e) = make_float4(o[e], o[e + 1], o[e + 2], o[e + 3]);
+                    for (int e = 0; e < 8; ++e) *reinterpret_cast<float4*>(st + sw128_chunk(lane, e)) = make_float4(o[4 * e], o[4 * e + 1], o[4 * e + 2], o[4 * e + 3]);
+                    __syncwarp();
+#pragma unroll
+                    for (int e = 0; e < 8; ++e) {
+                        const int rr = e * 4 + (lane >> 3), ch = lane & 7;
+                        const int64_t to_row = __shfl_sync(0xffffffffu, real ? at : -1, rr);
+                        if (to_row >= 0 && c + ch * 4 < hs) *reinterpret_cast<float4*>(acc + to_row * hs + c + ch * 4) = *reinterpret_cast<const float4*>(st + sw128_chunk(rr, ch));
+                    }
+                    __syncwarp();
                 }
             }
+            asm volatile("bar.sync 1, 256;" ::: "memory");  // (the next segment's Q comes where other warps' sums may be still)
             tc_fence_before();  // (the next segment's products overwrite the sums)
             g += n;
             u += n;

@@ -123,7 +123,7 @@ int32_t by_types(int cache_type, int type, F&& f) {
 
 // What an attention call needs of its workspace, all in floats, and how it is cut.
 struct AttnPlan {
-    int blocks, smem, thin_prefix;
+    int blocks, smem, thin_prefix, slot_rows;
     PrefixCut cut;              // the prefix's own kernel, a block per SM
     int cut_blocks, stages, cut_smem;
     int64_t slots, whole, cut_slots, pre, total;  // floats of the slots, of whole items, of the prefix's slots and whole items, of everything
@@ -139,10 +139,11 @@ AttnPlan attention_plan(const PagedPool& pool, const PagedSeqs& s, int n_heads, 
     const bool tiled = s.prefix_len > 0 && rows > PT_ROWS && (int64_t)pool.n_pages * pool.n_kv < 0x7fffffff;
     a.thin_prefix = s.prefix_len > 0 && !tiled;
     const int64_t most = (int64_t)s.n_query * group * (a.thin_prefix ? s.n_seq : 1);
-    a.smem = PT_WARPS * PT_STAGES * 2 * PT_WKEYS * (ks * 32 + 16) + PT_WARPS * (int)(most < PT_ROWS ? most : PT_ROWS) * (pool.hs + 2) * 4;
-    a.blocks = sms * (2 * (a.smem + 1024) <= 228 * 1024 ? 2 : 1);
+    a.slot_rows = (int)(most < PT_ROWS ? most : PT_ROWS);
+    a.smem = PT_WARPS * PT_STAGES * 2 * PT_KEYS * (ks * 32 + 16);
+    a.blocks = sms * 2;
     const int64_t row = pool.hs + 4;  // sums, then maximum and total, on 16-byte boundaries
-    a.slots = (int64_t)2 * a.blocks * PT_ROWS * row;
+    a.slots = (int64_t)2 * a.blocks * PT_WARPS * a.slot_rows * row;
     a.whole = a.pre = s.prefix_len ? n_tok * n_heads * row : 0;
     if (tiled) {
         const bool wide = type == L2B_TYPE_F32;
@@ -154,7 +155,7 @@ AttnPlan attention_plan(const PagedPool& pool, const PagedSeqs& s, int n_heads, 
         a.cut.whole_rows = n_tok * n_heads;
         a.cut_blocks = a.cut.units < sms ? (int)a.cut.units : sms;
         a.cut.share = (a.cut.units + a.cut_blocks - 1) / a.cut_blocks;
-        const int queries = terms * a.cut.streams_share * nd * PX_ROWS * 128, stage = 2 * nd * keys * 128;
+        const int terms_bytes = terms * a.cut.streams_share * nd * PX_ROWS * 128, queries = terms_bytes > 32768 ? terms_bytes : 32768, stage = 2 * nd * keys * 128;  // (PrefixTraits)
         a.stages = (222 * 1024 - queries) / stage;  // (of 227 KB, behind barriers and a start on 1 KB)
         a.stages = a.stages < PX_MAX_STAGES ? a.stages : PX_MAX_STAGES;
         a.cut_smem = queries + a.stages * stage + 1024;
@@ -283,11 +284,12 @@ extern "C" int32_t l2b_paged_attention_device(const l2b_paged_cache* cache, cons
     p.scale2 = (queries->scale != 0.f ? queries->scale : 1.f / sqrtf((float)hs)) * 1.4426950408889634f;
     p.thin_prefix = plan.thin_prefix;
     p.cut = plan.cut;
-    p.blocks = plan.blocks;
+    p.workers = plan.blocks * PT_WARPS;
+    p.slot_rows = plan.slot_rows;
     float* const w = (float*)dev_workspace;
     const int64_t n_rows = (int64_t)p.seqs.n_seq * p.seqs.n_query * p.n_heads;
     p.slot_acc = w;
-    p.slot_ml = w + (int64_t)2 * plan.blocks * PT_ROWS * hs;
+    p.slot_ml = w + (int64_t)2 * p.workers * p.slot_rows * hs;
     if (p.seqs.prefix_len) {
         p.own_acc = w + plan.slots;
         p.own_ml = p.own_acc + n_rows * hs;

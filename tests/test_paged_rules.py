@@ -92,9 +92,9 @@ SIMULATE = r"""
 #include "paged.h"
 #include <vector>
 using namespace l2b;
-// Walks every block's share as the kernel does.  out: blocks that did each unit of (group, item, tile), in that order; returns the number of units, or a
+// Walks every worker's share as the kernel does.  out: blocks that did each unit of (group, item, tile), in that order; returns the number of units, or a
 // negative number where a slot is used twice or a part is missing.
-extern "C" long long walk(const int* lengths, int n_seq, int n_query, int width, int page_shift, int prefix_len, int thin_prefix, int n_kv, int group, int blocks, int* out, long long room) {
+extern "C" long long walk(const int* lengths, int n_seq, int n_query, int width, int page_shift, int prefix_len, int thin_prefix, int n_kv, int group, int blocks, int least, int* out, long long room) {
     PagedWork w;
     w.pool = {nullptr, nullptr, 1, page_shift, n_kv, 64};
     w.seqs = {lengths, nullptr, nullptr, nullptr, n_seq, n_query, width, prefix_len};
@@ -105,14 +105,15 @@ extern "C" long long walk(const int* lengths, int n_seq, int n_query, int width,
     for (int g = 0; g < groups; ++g) first[g + 1] = first[g] + group_units(w, group_shape(w, g));
     const long long units = first[groups];
     if (units > room) return -1;
-    const PagedShares sh = paged_shares(units, blocks);
+    const PagedShares sh = paged_shares(units, blocks, least);
     std::vector<int> slots(2 * blocks, 0);
     for (int b = 0; b < blocks; ++b) {
         const long long begin = b * sh.share;
         if (begin >= units) continue;
         int g = 0;
         while (first[g + 1] <= begin) ++g;
-        Cursor at = cursor_at(w, g, begin - first[g], units - begin < sh.share ? units - begin : sh.share), tile = at;
+        auto length = [&](int g) { return group_length(w, g); };
+        Cursor at = cursor_at(w, g, group_shape(w, g), begin - first[g], units - begin < sh.share ? units - begin : sh.share), tile = at;
         long long done = 0;
         while (at.left > 0) {
             const int tiles = at.s.tiles - at.tile < at.left ? at.s.tiles - at.tile : (int)at.left;
@@ -120,7 +121,7 @@ extern "C" long long walk(const int* lengths, int n_seq, int n_query, int width,
             for (int t = 0; t < tiles; ++t) {
                 if (tile.g != at.g || tile.item != at.item || tile.tile != at.tile + t || tile.left <= 0) return -2;  // the copies run ahead over the same tiles
                 ++out[unit + t];
-                next_tile(w, tile);
+                next_item(w, tile, 1, length);
             }
             const PagedParts parts = paged_parts(unit - at.tile, at.s.tiles, sh.share);
             const bool whole = at.tile == 0 && tiles == at.s.tiles;
@@ -130,7 +131,7 @@ extern "C" long long walk(const int* lengths, int n_seq, int n_query, int width,
                 if (slot != paged_slot(parts, b) || slots[slot]++) return -4;
             }
             done += tiles;
-            next_item(w, at, tiles);
+            next_item(w, at, tiles, length);
         }
         if (done != (units - begin < sh.share ? units - begin : sh.share)) return -5;
     }
@@ -154,7 +155,7 @@ def sim(tmp_path_factory):
     return lib
 
 
-@pytest.mark.parametrize("blocks", [1, 7, 148, 296])
+@pytest.mark.parametrize("blocks", [1, 7, 148, 1184])
 def test_every_tile_belongs_to_one_share(sim, blocks):
     rng = np.random.default_rng(blocks)
     for trial in range(60):
@@ -164,10 +165,10 @@ def test_every_tile_belongs_to_one_share(sim, blocks):
         lengths[rng.random(n_seq) < 0.3] = rng.choice([-1, 0, 1, 63, 64, 65])
         prefix = int(rng.choice([0, 1, 63, 64, 65, 1000]))
         thin = int(prefix > 0)
-        out = np.zeros(1 << 20, np.int32)
-        units = sim.walk(lengths.ctypes.data_as(C.c_void_p), n_seq, n_query, width, shift, prefix, thin, n_kv, group, blocks, out.ctypes.data_as(C.c_void_p), out.size)
+        out, least = np.zeros(1 << 22, np.int32), int(rng.choice([1, 2, 4]))
+        units = sim.walk(lengths.ctypes.data_as(C.c_void_p), n_seq, n_query, width, shift, prefix, thin, n_kv, group, blocks, least, out.ctypes.data_as(C.c_void_p), out.size)
         up = lambda a, b: -(-a // b)  # noqa: E731
-        want = sum(up(min(max(int(n), 0), width << shift), 64) for n in lengths) * up(n_query * group, 16) * n_kv + thin * up(prefix, 64) * up(n_seq * n_query * group, 16) * n_kv
+        want = sum(up(min(max(int(n), 0), width << shift), 16) for n in lengths) * up(n_query * group, 16) * n_kv + thin * up(prefix, 16) * up(n_seq * n_query * group, 16) * n_kv
         assert units == want
         assert (out[:units] == 1).all() and (out[units:] == 0).all()
 
