@@ -43,7 +43,7 @@ struct PagedShares {
 L2B_HD PagedShares paged_shares(int64_t units, int workers, int least) {
     PagedShares s;
     s.units = units;
-    s.share = (units + workers - 1) / workers;
+    s.share = units + workers <= 0xffffffffll ? ((uint32_t)units + (uint32_t)workers - 1u) / (uint32_t)workers : (units + workers - 1) / workers;
     if (s.share < least) s.share = least;
     return s;
 }
@@ -52,8 +52,14 @@ struct PagedParts {
 };
 L2B_HD PagedParts paged_parts(int64_t begin, int tiles, int64_t share) {
     PagedParts p;
-    p.first = (int)(begin / share);
-    p.last = (int)((begin + tiles - 1) / share);
+    if (begin + tiles <= 0xffffffffll) {  // (a 64-bit division is a hundred instructions; the share is no larger than all units)
+        const uint32_t b = (uint32_t)begin, s = share <= 0xffffffffll ? (uint32_t)share : 0xffffffffu;
+        p.first = (int)(b / s);
+        p.last = (int)((b + (uint32_t)tiles - 1u) / s);
+    } else {
+        p.first = (int)(begin / share);
+        p.last = (int)((begin + tiles - 1) / share);
+    }
     return p;
 }
 L2B_HD int paged_slot(const PagedParts& p, int worker) { return 2 * worker + (worker == p.first ? 1 : 0); }

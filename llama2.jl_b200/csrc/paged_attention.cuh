@@ -26,6 +26,7 @@ struct PagedAttnParams : PagedWork {
     int64_t q_stride, out_stride;
     int n_heads;
     float scale2;          // scale * log2(e)
+    int64_t* starts;            // [groups + 1]: first unit of each group, left by the own parts' kernel for the joining one
     int workers;                // warps of the own parts' kernel
     int slot_rows;              // rows of a slot: 16, or fewer when no tile has as many
     float *slot_acc, *slot_ml;  // [2 * workers][slot_rows][hs], [..][2]
@@ -126,10 +127,11 @@ __global__ void __launch_bounds__(PT_WARPS * 32, 2) paged_attention_kernel(const
     const int64_t begin = worker * sh.share;
     Cursor at;
     at.left = 0;
-    if (begin < units) {
+    if (begin < units || worker == 0) {
         int64_t sum = 0;  // units of the groups before
         int found = -1;
-        for (int g0 = 0; found < 0 && g0 < groups; g0 += 32) {
+        if (worker == 0 && lane == 0) p.starts[groups] = units;
+        for (int g0 = 0; (found < 0 || worker == 0) && g0 < groups; g0 += 32) {
             const int64_t n = g0 + lane < groups ? group_units(p, group_shape(p, g0 + lane)) : 0;
             int64_t inc = n;
             for (int o = 1; o < 32; o <<= 1) {
@@ -137,15 +139,14 @@ __global__ void __launch_bounds__(PT_WARPS * 32, 2) paged_attention_kernel(const
                 if (lane >= o) inc += v;
             }
             const unsigned hit = __ballot_sync(0xffffffffu, sum + inc > begin);
-            if (hit) {
+            if (hit && found < 0) {
                 const int l = __ffs(hit) - 1;
-                sum += __shfl_sync(0xffffffffu, inc - n, l);
                 found = g0 + l;
-            } else {
-                sum += __shfl_sync(0xffffffffu, inc, 31);
+                at = cursor_at(p, found, group_shape(p, found), begin - sum - __shfl_sync(0xffffffffu, inc - n, l), min(sh.share, units - begin));
             }
+            if (worker == 0 && g0 + lane < groups) p.starts[g0 + lane] = sum + inc - n;
+            sum += __shfl_sync(0xffffffffu, inc, 31);
         }
-        if (found >= 0) at = cursor_at(p, found, group_shape(p, found), begin - sum, min(sh.share, units - begin));
     }
     Lengths ahead_lengths = {-64, 0}, at_lengths = {-64, 0};
 
@@ -425,34 +426,11 @@ constexpr int PJ_WARPS = 8;
 template <typename TIO>
 __global__ void __launch_bounds__(PJ_WARPS * 32) paged_join_kernel(const __grid_constant__ JoinParams jp) {
     const PagedAttnParams& p = jp.a;
-    __shared__ int64_t s_units[2][PJ_WARPS];
     __shared__ float s_part[PJ_WARPS][PA_MAX_SIZE + 2];
     const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, hs = p.pool.hs;
     const int64_t tok = blockIdx.x;
     const int seq = (int)(tok / p.seqs.n_query), j = (int)(tok % p.seqs.n_query), group = seq + p.thin_prefix;
     const int length = p.seqs.lengths[seq], count = paged_count(length, p.seqs.counts ? p.seqs.counts[seq] : p.seqs.n_query, p.seqs.n_query);
-    // where the shares lie: units of all groups, and of those before this one
-    int64_t all = 0, before = 0;
-    for (int g = threadIdx.x; g < p.seqs.n_seq + p.thin_prefix; g += PJ_WARPS * 32) {
-        const int64_t n = group_units(p, group_shape(p, g));
-        all += n;
-        before += g < group ? n : 0;
-    }
-    for (int o = 16; o > 0; o >>= 1) {
-        all += __shfl_xor_sync(0xffffffffu, all, o);
-        before += __shfl_xor_sync(0xffffffffu, before, o);
-    }
-    if (lane == 0) {
-        s_units[0][warp] = all;
-        s_units[1][warp] = before;
-    }
-    __syncthreads();
-    all = before = 0;
-    for (int w = 0; w < PJ_WARPS; ++w) {
-        all += s_units[0][w];
-        before += s_units[1][w];
-    }
-    const PagedShares sh = paged_shares(all, p.workers, PT_LEAST);
     const int per_row = PJ_WARPS / jp.heads, head = blockIdx.y * jp.heads + warp / per_row, sub = warp % per_row;
     const bool real = head < p.n_heads;
     const int kv = head / p.group, g = head - kv * p.group, d = lane * 4;
@@ -461,25 +439,26 @@ __global__ void __launch_bounds__(PJ_WARPS * 32) paged_join_kernel(const __grid_
     // the parts of this row: of the prefix's kernel, of the prefix as a group of the own parts' kernel, of the own positions
     const GroupShape own = group_shape(p, group, length), pre = group_shape(p, 0, length);
     const int own_row = j * p.group + g, pre_row = (int)(tok * p.group) + g;
+    const int per_item = p.cut.streams_share * 128, streams = p.cut.streams_share == 2 ? 1 : 2;
     PagedParts of[3] = {};
     int n_parts[3] = {};
-    const int per_item = p.cut.streams_share * 128, streams = p.cut.streams_share == 2 ? 1 : 2;
     if (p.cut.units > 0) {
         of[0] = paged_parts(((int64_t)kv * p.cut.row_tiles + pre_row / per_item) * p.cut.tiles, p.cut.tiles, p.cut.share);
         n_parts[0] = (of[0].last - of[0].first + 1) * streams;
     }
+    pdl_wait();
+    if (j >= count) return;
+    const int64_t units = __ldcg(p.starts + p.seqs.n_seq + p.thin_prefix), share = paged_shares(units, p.workers, PT_LEAST).share;
     if (p.thin_prefix) {
-        of[1] = paged_parts(((int64_t)kv * pre.row_tiles + pre_row / PT_ROWS) * pre.tiles, pre.tiles, sh.share);
+        of[1] = paged_parts(((int64_t)kv * pre.row_tiles + pre_row / PT_ROWS) * pre.tiles, pre.tiles, share);
         n_parts[1] = of[1].last - of[1].first + 1;
     }
     if (own.tiles > 0) {
-        of[2] = paged_parts(before + ((int64_t)kv * own.row_tiles + own_row / PT_ROWS) * own.tiles, own.tiles, sh.share);
+        of[2] = paged_parts(__ldcg(p.starts + group) + ((int64_t)kv * own.row_tiles + own_row / PT_ROWS) * own.tiles, own.tiles, share);
         n_parts[2] = of[2].last - of[2].first + 1;
     }
     const bool done = own.tiles > 0 && n_parts[2] == 1 && !p.own_acc;  // written already
     const int parts = !real || done ? 0 : n_parts[0] + n_parts[1] + n_parts[2];
-    pdl_wait();
-    if (j >= count) return;
 
     float m = -INFINITY, l = 0.f, o[4] = {0.f, 0.f, 0.f, 0.f};
     for (int first = sub; first < parts; first += 32 * per_row) {  // (the same for the whole warp)

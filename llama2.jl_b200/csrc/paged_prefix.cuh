@@ -24,8 +24,7 @@ struct PrefixParams : PagedWork {
     const void* q;
     int64_t q_stride;
     int n_heads, rows, stages;
-    float scale2;  // not negative: a negative scale's sign goes to the queries
-    int negate;
+    float scale2;  // positive
     PrefixCut cut;
     float *slot_acc, *slot_ml;  // [2 * blocks][2][128][hs], [..][2]
     float *pre_acc, *pre_ml;    // [2 / TILES][rows of the batch * n_heads][hs], [..][2]
@@ -44,50 +43,85 @@ struct PrefixTraits {
         return (1u << 4) | (F16 ? 0u : (1u << 7) | (1u << 10)) | ((uint32_t)b_mn << 16) | ((uint32_t)(n >> 3) << 17) | ((uint32_t)(PX_ROWS >> 4) << 24);
     }
 };
-__device__ __forceinline__ void tmem_st16u(uint32_t taddr, const uint32_t (&v)[16]) {
-    asm volatile("tcgen05.st.sync.aligned.32x32b.x16.b32 [%0], {%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15,%16};" ::"r"(taddr), "r"(v[0]), "r"(v[1]), "r"(v[2]),
-                 "r"(v[3]), "r"(v[4]), "r"(v[5]), "r"(v[6]), "r"(v[7]), "r"(v[8]), "r"(v[9]), "r"(v[10]), "r"(v[11]), "r"(v[12]), "r"(v[13]), "r"(v[14]), "r"(v[15])
-                 : "memory");
+// 64 consecutive columns of this thread's tensor-memory lane, and a store of 32
+__device__ __forceinline__ void tmem_ld64f(uint32_t taddr, float (&v)[64]) {
+    asm volatile(
+        "tcgen05.ld.sync.aligned.32x32b.x64.b32 {"
+        "%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15,%16,%17,%18,%19,%20,%21,%22,%23,%24,%25,%26,%27,%28,%29,%30,%31,"
+        "%32,%33,%34,%35,%36,%37,%38,%39,%40,%41,%42,%43,%44,%45,%46,%47,%48,%49,%50,%51,%52,%53,%54,%55,%56,%57,%58,%59,%60,%61,%62,%63"
+        "}, [%64];\n\ttcgen05.wait::ld.sync.aligned;"
+        : "=f"(v[0]), "=f"(v[1]), "=f"(v[2]), "=f"(v[3]), "=f"(v[4]), "=f"(v[5]), "=f"(v[6]), "=f"(v[7]), "=f"(v[8]), "=f"(v[9]), "=f"(v[10]), "=f"(v[11]),
+          "=f"(v[12]), "=f"(v[13]), "=f"(v[14]), "=f"(v[15]), "=f"(v[16]), "=f"(v[17]), "=f"(v[18]), "=f"(v[19]), "=f"(v[20]), "=f"(v[21]), "=f"(v[22]), "=f"(v[23]),
+          "=f"(v[24]), "=f"(v[25]), "=f"(v[26]), "=f"(v[27]), "=f"(v[28]), "=f"(v[29]), "=f"(v[30]), "=f"(v[31]), "=f"(v[32]), "=f"(v[33]), "=f"(v[34]), "=f"(v[35]),
+          "=f"(v[36]), "=f"(v[37]), "=f"(v[38]), "=f"(v[39]), "=f"(v[40]), "=f"(v[41]), "=f"(v[42]), "=f"(v[43]), "=f"(v[44]), "=f"(v[45]), "=f"(v[46]), "=f"(v[47]),
+          "=f"(v[48]), "=f"(v[49]), "=f"(v[50]), "=f"(v[51]), "=f"(v[52]), "=f"(v[53]), "=f"(v[54]), "=f"(v[55]), "=f"(v[56]), "=f"(v[57]), "=f"(v[58]), "=f"(v[59]),
+          "=f"(v[60]), "=f"(v[61]), "=f"(v[62]), "=f"(v[63])
+        : "r"(taddr)
+        : "memory");
+}
+__device__ __forceinline__ void tmem_st32u(uint32_t taddr, const uint32_t (&v)[32]) {
+    asm volatile(
+        "tcgen05.st.sync.aligned.32x32b.x32.b32 [%0], {"
+        "%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15,%16,%17,%18,%19,%20,%21,%22,%23,%24,%25,%26,%27,%28,%29,%30,%31,%32"
+        "};" ::"r"(taddr),
+        "r"(v[0]), "r"(v[1]), "r"(v[2]), "r"(v[3]), "r"(v[4]), "r"(v[5]), "r"(v[6]), "r"(v[7]), "r"(v[8]), "r"(v[9]), "r"(v[10]), "r"(v[11]),
+        "r"(v[12]), "r"(v[13]), "r"(v[14]), "r"(v[15]), "r"(v[16]), "r"(v[17]), "r"(v[18]), "r"(v[19]), "r"(v[20]), "r"(v[21]), "r"(v[22]), "r"(v[23]),
+        "r"(v[24]), "r"(v[25]), "r"(v[26]), "r"(v[27]), "r"(v[28]), "r"(v[29]), "r"(v[30]), "r"(v[31])
+        : "memory");
 }
 
-// The softmax threads' part in bringing 128 * TILES rows of Q to shared memory, in operand layout, as terms of T.
+// The softmax threads' part in bringing 128 * TILES rows of Q to shared memory, in operand layout, as terms of T.  Rows of T come by asynchronous copies,
+// all of them under way at once.
 template <typename T, typename TIO, int TILES>
 __device__ __forceinline__ void load_queries(const PrefixParams& p, uint8_t* sq, int* s_exp, int kv, int row0, int nd) {
     using TR = PrefixTraits<T, TIO, TILES>;
-    const int hs = p.pool.hs, per_row = nd * 8, tid = threadIdx.x;
+    const int hs = p.pool.hs, shift = nd == 1 ? 3 : 4, tid = threadIdx.x;  // 8 or 16 threads to a row, a chunk of 8 values each
+    const int ch = tid & ((1 << shift) - 1), step = 256 >> shift;
+    int r = tid >> shift, t = (row0 + r) / p.group, g = (row0 + r) - t * p.group;  // row of the block, token and head of it
+    const int t_step = step / p.group, g_step = step - t_step * p.group;
+    const TIO* const base = (const TIO*)p.q + (int64_t)kv * p.group * hs + ch * 8;
 #pragma unroll 4
-    for (int i = tid; i < TILES * PX_ROWS * per_row; i += 256) {  // (per_row is 8 or 16: a row's threads are of one warp)
-        const int r = i / per_row, ch = i - r * per_row, row = row0 + r;
-        float x[8] = {};
-        if (row < p.rows && ch * 8 < hs) {
-            const int t = row / p.group;
-            get((const TIO*)p.q + (int64_t)t * p.q_stride + (int64_t)(kv * p.group + row - t * p.group) * hs + ch * 8, x);
-        }
-        if (p.negate) {
+    for (; r < TILES * PX_ROWS; r += step) {
+        const bool real = row0 + r < p.rows && ch * 8 < hs;
+        const TIO* const src = base + (int64_t)(real ? t : 0) * p.q_stride + (real ? g : 0) * hs;
+        uint8_t* const dst = sq + ((r / PX_ROWS) * nd + (ch >> 3)) * TR::SUB_Q + sw128_chunk(r % PX_ROWS, ch & 7);
+        if constexpr (!TR::WIDE) {
+            cp_async16(dst, real ? src : (const TIO*)p.q, real);
+        } else {
+            float x[8] = {};
+            if (real) get(src, x);
+            if (TR::F16) {  // f16 terms: the row's largest value between 1/2 and 1
+                float mx = 0.f;
 #pragma unroll
-            for (int e = 0; e < 8; ++e) x[e] = -x[e];
-        }
-        if (TR::WIDE && TR::F16) {  // f16 terms: the row's largest value between 1/2 and 1
-            float mx = 0.f;
+                for (int e = 0; e < 8; ++e) mx = fmaxf(mx, fabsf(x[e]));
+                for (int o = 1 << shift >> 1; o > 0; o >>= 1) mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, o));
+                int ex = 0;
+                if (mx > 0.f && mx < INFINITY) ex = max(-100, min(100, ilogbf(mx) + 1));
+                if (ch == 0) s_exp[r] = ex;
+                const float f = ldexpf(1.f, -ex);
 #pragma unroll
-            for (int e = 0; e < 8; ++e) mx = fmaxf(mx, fabsf(x[e]));
-            for (int o = per_row / 2; o > 0; o >>= 1) mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, o));
-            int ex = 0;
-            if (mx > 0.f && mx < INFINITY) frexpf(mx, &ex);
-            ex = max(-100, min(100, ex));
-            if (ch == 0) s_exp[r] = ex;
+                for (int e = 0; e < 8; ++e) x[e] *= f;
+            }
 #pragma unroll
-            for (int e = 0; e < 8; ++e) x[e] = ldexpf(x[e], -ex);
+            for (int k = 0; k < TR::QT; ++k) {
+                uint4 w;
+                w.x = split_pair<T>(x[0], x[1]);
+                w.y = split_pair<T>(x[2], x[3]);
+                w.z = split_pair<T>(x[4], x[5]);
+                w.w = split_pair<T>(x[6], x[7]);
+                *reinterpret_cast<uint4*>(dst + k * TILES * nd * TR::SUB_Q) = w;
+            }
         }
-#pragma unroll
-        for (int t = 0; t < TR::QT; ++t) {
-            uint4 w;
-            w.x = split_pair<T>(x[0], x[1]);
-            w.y = split_pair<T>(x[2], x[3]);
-            w.z = split_pair<T>(x[4], x[5]);
-            w.w = split_pair<T>(x[6], x[7]);
-            *reinterpret_cast<uint4*>(sq + ((t * TILES + r / PX_ROWS) * nd + (ch >> 3)) * TR::SUB_Q + sw128_chunk(r % PX_ROWS, ch & 7)) = w;
+        t += t_step;
+        g += g_step;
+        if (g >= p.group) {
+            g -= p.group;
+            ++t;
         }
+    }
+    if (!TR::WIDE) {
+        cp_async_commit();
+        cp_async_wait<0>();
     }
 }
 
@@ -269,22 +303,19 @@ __global__ void __launch_bounds__(PX_THREADS, 1) paged_prefix_kernel(const __gri
                 if (ok) ok = __all_sync(0xffffffffu, mbar_wait_bounded(s_s + i, (uint32_t)(ns & 1)));
                 ++ns;
                 tc_fence_after();
-                float x[KEYS];
-#pragma unroll
-                for (int c = 0; c < KEYS; c += 32) tmem_ld32f(ts + (uint32_t)c, *reinterpret_cast<float(*)[32]>(x + c));
-                uint32_t there[KEYS / 32], all = ~0u;
-#pragma unroll
-                for (int c = 0; c < KEYS / 32; ++c) {
-                    there[c] = s_valid[gt % PX_RING][c];
-                    all &= there[c];
-                }
-                if (all != ~0u) {
-#pragma unroll
-                    for (int k = 0; k < KEYS; ++k) x[k] = there[k >> 5] >> (k & 31) & 1 ? x[k] : -INFINITY;
-                }
                 float m4[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
+#pragma unroll 1
+                for (int c = 0; c < KEYS; c += 64) {
+                    float x[64];
+                    tmem_ld64f(ts + (uint32_t)c, x);
+                    const uint32_t v0 = s_valid[gt % PX_RING][c >> 5], v1 = s_valid[gt % PX_RING][(c >> 5) + 1];
+                    if ((v0 & v1) != ~0u) {
 #pragma unroll
-                for (int k = 0; k < KEYS; k += 2) m4[k >> 1 & 3] = fmaxf(fmaxf(x[k], x[k + 1]), m4[k >> 1 & 3]);
+                        for (int k = 0; k < 64; ++k) x[k] = (k < 32 ? v0 : v1) >> (k & 31) & 1 ? x[k] : -INFINITY;
+                    }
+#pragma unroll
+                    for (int k = 0; k < 64; k += 2) m4[k >> 1 & 3] = fmaxf(fmaxf(x[k], x[k + 1]), m4[k >> 1 & 3]);
+                }
                 const float mx = fmaxf(fmaxf(m4[0], m4[1]), fmaxf(m4[2], m4[3])) * sc;
                 if (!some) {
                     m = mx;
@@ -304,19 +335,25 @@ __global__ void __launch_bounds__(PX_THREADS, 1) paged_prefix_kernel(const __gri
                 some = true;
                 const float use = m == -INFINITY ? 0.f : m;
                 float l4[4] = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll 1
+                for (int c = 0; c < KEYS; c += 64) {
+                    float x[64];
+                    tmem_ld64f(ts + (uint32_t)c, x);
+                    const uint32_t v0 = s_valid[gt % PX_RING][c >> 5], v1 = s_valid[gt % PX_RING][(c >> 5) + 1];
 #pragma unroll
-                for (int c = 0; c < KEYS; c += 32) {
+                    for (int k = 0; k < 64; ++k) x[k] = exp2_approx(fmaf(x[k], sc, -use));
+                    if ((v0 & v1) != ~0u) {
 #pragma unroll
-                    for (int k = 0; k < 32; ++k) {
-                        x[c + k] = exp2_approx(fmaf(x[c + k], sc, -use));
-                        l4[k & 3] += x[c + k];
+                        for (int k = 0; k < 64; ++k) x[k] = (k < 32 ? v0 : v1) >> (k & 31) & 1 ? x[k] : 0.f;
                     }
 #pragma unroll
-                    for (int t2 = 0; t2 < TR::PT; ++t2) {
-                        uint32_t w[16];
+                    for (int k = 0; k < 64; ++k) l4[k & 3] += x[k];
 #pragma unroll
-                        for (int k = 0; k < 16; ++k) w[k] = TR::PT == 1 ? pair_of<T>(x[c + 2 * k], x[c + 2 * k + 1]) : split_pair<T>(x[c + 2 * k], x[c + 2 * k + 1]);
-                        tmem_st16u(ts + (uint32_t)(t2 * (KEYS / 2) + c / 2), w);
+                    for (int t2 = 0; t2 < TR::PT; ++t2) {
+                        uint32_t w[32];
+#pragma unroll
+                        for (int k = 0; k < 32; ++k) w[k] = TR::PT == 1 ? pair_of<T>(x[2 * k], x[2 * k + 1]) : split_pair<T>(x[2 * k], x[2 * k + 1]);
+                        tmem_st32u(ts + (uint32_t)(t2 * 32 + c / 2), w);  // (columns of scores that have been read)
                     }
                 }
                 l += (l4[0] + l4[1]) + (l4[2] + l4[3]);

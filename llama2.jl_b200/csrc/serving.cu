@@ -126,17 +126,17 @@ struct AttnPlan {
     int blocks, smem, thin_prefix, slot_rows;
     PrefixCut cut;              // the prefix's own kernel, a block per SM
     int cut_blocks, stages, cut_smem;
-    int64_t slots, whole, cut_slots, pre, total;  // floats of the slots, of whole items, of the prefix's slots and whole items, of everything
+    int64_t starts, slots, whole, cut_slots, pre, total;  // floats of the slots, of whole items, of the prefix's slots and whole items, of everything
 };
 
 // The prefix goes through the tensor cores' 128-row tiles when its rows fill more than one tile of 16; up to there it is one more group of the own
-// parts' kernel, without a launch of its own.
-AttnPlan attention_plan(const PagedPool& pool, const PagedSeqs& s, int n_heads, int type, int cache_type, int sms) {
+// parts' kernel, without a launch of its own.  (So it is with a negative scale, which the tiles' maxima do not allow for.)
+AttnPlan attention_plan(const PagedPool& pool, const PagedSeqs& s, const l2b_paged_queries& q, int cache_type, int sms) {
     AttnPlan a;
     memset(&a, 0, sizeof(a));
-    const int ks = (pool.hs + 31) / 32 * 2, group = n_heads / pool.n_kv;
+    const int ks = (pool.hs + 31) / 32 * 2, n_heads = q.n_heads, group = n_heads / pool.n_kv;
     const int64_t n_tok = (int64_t)s.n_seq * s.n_query, rows = n_tok * group;
-    const bool tiled = s.prefix_len > 0 && rows > PT_ROWS && (int64_t)pool.n_pages * pool.n_kv < 0x7fffffff;
+    const bool tiled = s.prefix_len > 0 && rows > PT_ROWS && q.scale >= 0.f && (int64_t)pool.n_pages * pool.n_kv < 0x7fffffff;
     a.thin_prefix = s.prefix_len > 0 && !tiled;
     const int64_t most = (int64_t)s.n_query * group * (a.thin_prefix ? s.n_seq : 1);
     a.slot_rows = (int)(most < PT_ROWS ? most : PT_ROWS);
@@ -146,7 +146,7 @@ AttnPlan attention_plan(const PagedPool& pool, const PagedSeqs& s, int n_heads, 
     a.slots = (int64_t)2 * a.blocks * PT_WARPS * a.slot_rows * row;
     a.whole = a.pre = s.prefix_len ? n_tok * n_heads * row : 0;
     if (tiled) {
-        const bool wide = type == L2B_TYPE_F32;
+        const bool wide = q.type == L2B_TYPE_F32;
         const int keys = wide ? 64 : 128, nd = (pool.hs + 63) / 64, terms = !wide ? 1 : cache_type == L2B_TYPE_F16 ? 2 : 3;
         a.cut.streams_share = !wide && rows > PX_ROWS ? 2 : 1;
         a.cut.tiles = (int)(((int64_t)s.prefix_len + keys - 1) / keys);
@@ -162,7 +162,8 @@ AttnPlan attention_plan(const PagedPool& pool, const PagedSeqs& s, int n_heads, 
         a.cut_slots = (int64_t)2 * a.cut_blocks * 2 * PX_ROWS * row;
         a.pre *= 2 / a.cut.streams_share;
     }
-    a.total = a.slots + a.whole + a.cut_slots + a.pre;
+    a.starts = ((int64_t)s.n_seq + a.thin_prefix + 1 + 1) / 2 * 4;  // 64-bit numbers, to a 16-byte boundary
+    a.total = a.starts + a.slots + a.whole + a.cut_slots + a.pre;
     return a;
 }
 
@@ -184,6 +185,7 @@ int32_t check_queries(const l2b_paged_cache* c, const l2b_paged_queries* q, cons
     L2B_TRY(check_row_type(q->type, c->type));
     if (q->n_heads <= 0 || q->n_heads > 65535 || q->n_heads % c->n_kv_heads) return fail(L2B_ERR_BAD_ARG, "n_heads must be a multiple of n_kv_heads");
     if ((int64_t)s.n_seq * s.n_query * q->n_heads > 0x7fffffff) return fail(L2B_ERR_BAD_ARG, "more than 2^31 - 1 query heads");
+    if (!std::isfinite(q->scale)) return fail(L2B_ERR_BAD_ARG, "scale must be finite, or 0 for 1 / sqrt(head_size)");
     return L2B_OK;
 }
 
@@ -255,7 +257,7 @@ extern "C" int32_t l2b_paged_attention_workspace(const l2b_paged_cache* cache, c
     L2B_TRY(on.enter(cache->dev_k, "dev_k"));
     int sms = 0;
     L2B_TRY(sm_count(on.device, &sms));
-    *bytes = attention_plan(pool, seqs, queries->n_heads, queries->type, cache->type, sms).total * 4;
+    *bytes = attention_plan(pool, seqs, *queries, cache->type, sms).total * 4;
     return L2B_OK;
 }
 
@@ -269,13 +271,12 @@ extern "C" int32_t l2b_paged_attention_device(const l2b_paged_cache* cache, cons
     const int hs = p.pool.hs;
     L2B_TRY(check_rows(queries->dev_q, queries->q_stride, (int64_t)queries->n_heads * hs, queries->type, "dev_q"));
     L2B_TRY(check_rows(queries->dev_out, queries->out_stride, (int64_t)queries->n_heads * hs, queries->type, "dev_out"));
-    if (!std::isfinite(queries->scale)) return fail(L2B_ERR_BAD_ARG, "scale must be finite, or 0 for 1 / sqrt(head_size)");
     OnDeviceOf on;
     L2B_TRY(on.enter(cache->dev_k, "dev_k"));
     if (p.seqs.n_seq == 0) return L2B_OK;
     int sms = 0;
     L2B_TRY(sm_count(on.device, &sms));
-    const AttnPlan plan = attention_plan(p.pool, p.seqs, queries->n_heads, queries->type, cache->type, sms);
+    const AttnPlan plan = attention_plan(p.pool, p.seqs, *queries, cache->type, sms);
     if (!dev_workspace || !aligned(dev_workspace) || workspace_bytes < plan.total * 4)
         return fail(L2B_ERR_BAD_ARG, "the workspace must lie on a 16-byte boundary and hold l2b_paged_attention_workspace bytes");
     p.q = queries->dev_q; p.out = queries->dev_out; p.q_stride = queries->q_stride; p.out_stride = queries->out_stride;
@@ -286,7 +287,8 @@ extern "C" int32_t l2b_paged_attention_device(const l2b_paged_cache* cache, cons
     p.cut = plan.cut;
     p.workers = plan.blocks * PT_WARPS;
     p.slot_rows = plan.slot_rows;
-    float* const w = (float*)dev_workspace;
+    p.starts = (int64_t*)dev_workspace;
+    float* const w = (float*)dev_workspace + plan.starts;
     const int64_t n_rows = (int64_t)p.seqs.n_seq * p.seqs.n_query * p.n_heads;
     p.slot_acc = w;
     p.slot_ml = w + (int64_t)2 * p.workers * p.slot_rows * hs;
@@ -309,8 +311,7 @@ extern "C" int32_t l2b_paged_attention_device(const l2b_paged_cache* cache, cons
             x.q = p.q; x.q_stride = p.q_stride; x.n_heads = p.n_heads;
             x.rows = p.seqs.n_seq * p.seqs.n_query * p.group;
             x.stages = plan.stages;
-            x.scale2 = fabsf(p.scale2);
-            x.negate = p.scale2 < 0.f;
+            x.scale2 = p.scale2;
             x.cut = plan.cut;
             x.slot_acc = p.cut_acc; x.slot_ml = p.cut_ml; x.pre_acc = p.pre_acc; x.pre_ml = p.pre_ml;
             const int keys = sizeof(TIO) == 4 ? 64 : 128, page = 1 << p.pool.page_shift;

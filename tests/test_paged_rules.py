@@ -50,7 +50,7 @@ REFUSED = [
     ("rows", "dev_k", A + 4, BAD, "a"), ("rows", "dev_q_gain", A + 4, BAD, "a"), ("rows", "eps", -1.0, BAD, "a"), ("rows", "eps", float("nan"), BAD, "a"), ("rows", "rope_freq_base", -2.0, BAD, "a"),
     ("rows", "rope_freq_base", float("inf"), BAD, "a"),
     ("queries", "type", 1, TYPE, "wt"), ("queries", "n_heads", 3, BAD, "wt"), ("queries", "n_heads", 0, BAD, "wt"), ("queries", "dev_q", None, BAD, "t"), ("queries", "dev_out", A + 2, BAD, "t"),
-    ("queries", "q_stride", 100, BAD, "t"), ("queries", "out_stride", 257, BAD, "t"), ("queries", "scale", float("nan"), BAD, "t"), ("queries", "scale", float("inf"), BAD, "t"),
+    ("queries", "q_stride", 100, BAD, "t"), ("queries", "out_stride", 257, BAD, "t"), ("queries", "scale", float("nan"), BAD, "wt"), ("queries", "scale", float("inf"), BAD, "wt"),
     ("sampling", "type", 12, TYPE, "s"), ("sampling", "n_rows", -1, BAD, "s"), ("sampling", "vocab", 0, BAD, "s"), ("sampling", "vocab", 393217, BAD, "s"), ("sampling", "stride", 99, BAD, "s"),
     ("sampling", "dev_logits", None, BAD, "s"), ("sampling", "dev_logits", A + 2, BAD, "s"), ("sampling", "dev_uniform", None, BAD, "s"), ("sampling", "dev_uniform", A + 4, BAD, "s"),
     ("sampling", "dev_tokens", None, BAD, "s"), ("sampling", "n_rows", 1 << 29, BAD, "s"),
