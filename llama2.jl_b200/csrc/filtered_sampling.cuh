@@ -5,10 +5,13 @@
 //
 // A cluster of up to eight blocks holds a row in its shared memory, read once; every pass after that is over shared memory.  Masses are whole numbers of
 // 2^-44 of the largest weight (weights computed in 64 bits), so that sums do not depend on their order and no cut or choice hangs on the blocks or on atomics.
-// Cuts: equal bins of the distance from the maximum are counted; only the bin that holds the k-th value (or the nucleus' border) is ordered,
-// by counting, a thread per value.  With a top-k whose bins hold at most LIST values everything else happens among those.  The nucleus' bin is first guessed from
-// f32 masses per bin and then checked with exact sums.  More than LIST values in one bin (many equal logits): bisection on (value, index), a pass per bit.
-// Bound by the passes over shared memory and by the cluster's barriers; the logits' read is the floor.
+//   top-k up to FS_FAST: every block takes its share of the k-th place among its threads' maxima, so that the lowest of the blocks' values has at least k
+//     values above it; the few that are no smaller are brought together, and everything else happens among those.
+//   other cuts: equal bins of the distance from the maximum are counted, or weighed; only the bin with the k-th value, or the nucleus' border, is listed and
+//     ordered, by counting.  More than FS_LIST values in one bin (many equal logits): bisection on (value, index), a pass per bit.
+//   the choice: masses of stretches of the row, then inside the stretch that holds it.
+// What every block needs it works out for itself from the others' shared memory: a barrier of the cluster costs more than that.
+// A pass that weighs all logits is bound by 64-bit arithmetic, one over a few candidates by the barriers; the logits' read is the floor.
 #pragma once
 #include <cooperative_groups.h>
 
@@ -16,7 +19,7 @@
 
 namespace l2b {
 
-constexpr int FS_THREADS = 512, FS_WARPS = FS_THREADS / 32, FS_BINS = 1024, FS_LIST = 1024, FS_CLUSTER = 8;
+constexpr int FS_THREADS = 512, FS_WARPS = FS_THREADS / 32, FS_BINS = 1024, FS_LIST = 1024, FS_FAST = 512, FS_CLUSTER = 8, FS_TABLE = 128;
 constexpr int FS_SLICE = 48 * 1024;  // most logits of a block
 constexpr double FS_ONE = 17592186044416.0;  // 2^44
 
@@ -32,23 +35,26 @@ struct SampleParams {
 };
 
 struct SampleShared {
-    uint32_t count[FS_BINS];
-    float mass[FS_BINS];
+    union {
+        struct {
+            uint32_t low[FS_BINS], high[FS_BINS];  // of each bin: the count in `low`, or the mass
+        };
+        uint64_t w[FS_LIST];  // weights of `all`, once all blocks have read the bins (a gathering's barrier is behind that)
+    };
     uint64_t list[FS_LIST];
-    uint64_t all[FS_LIST], w[FS_LIST];  // block 0: the lists of all blocks, and their weights
+    uint64_t all[FS_LIST];                 // the lists of all blocks
+    double table[FS_TABLE];                // 2^(-i / FS_TABLE)
     uint64_t sums[FS_WARPS];
-    float wmax[FS_WARPS], wmin[FS_WARPS];
+    float wmax[FS_WARPS], wmin[FS_WARPS], tmax[FS_THREADS];
     uint32_t widx[FS_WARPS], wcnt[FS_WARPS];
     // what other blocks read
-    float max, min;
+    float max, min, tau;
     uint32_t idx, usable, listed;
     uint64_t total[2];
-    uint64_t cut;
     // found by one thread, used by all
     int bin;
-    uint32_t before;
-    uint32_t choice;
-    uint64_t found;
+    uint32_t survivors, choice;
+    uint64_t before, found;
 };
 
 __device__ __forceinline__ uint32_t ordered_bits(float x) {  // larger value, larger number; -0 and 0 are equal
@@ -59,23 +65,30 @@ __device__ __forceinline__ float from_ordered(uint32_t u) { return __uint_as_flo
 __device__ __forceinline__ uint64_t order_key(float x, uint32_t index) { return (uint64_t)ordered_bits(x) << 32 | (0xffffffffu - index); }
 
 struct SampleRow {
-    float max;
-    double dmax, rate, floor_t;  // w = 2^-((max - x) * rate); floor_t: no weight beyond
+    float top;
+    double shift, rate, floor_t;  // w = 2^-t, t = shift - x * rate; floor_t: no weight beyond
     double min_p;
     uint64_t first;  // key of the first token: always kept
+    const double* table;
+    // 2^-t: t to the nearest 1/128 from the table, the rest (a = rest * ln 2 up to 0.0027) by the exponential series up to a^4 / 24; a^5 / 120 is 1.2e-15.
     __device__ __forceinline__ double weight(float x) const {
-        if (x == max) return 1.0;
-        const double t = (dmax - (double)x) * rate;
-        return t < floor_t ? exp2(-t) : 0.0;  // (NaN: infinite minus infinite)
+        if (x == top) return 1.0;
+        const double t = fma(-(double)x, rate, shift);
+        if (!(t < floor_t)) return 0.0;  // (also: infinite minus infinite)
+        constexpr double magic = 6755399441055744.0 / FS_TABLE;  // 1.5 * 2^52 / 128: the sum's last bit is 1/128
+        const double u = t + magic;
+        const int k = max(0, (int)(__double_as_longlong(u) & 0xffffffff));
+        const double a = (t - (u - magic)) * -0.6931471805599453;
+        const double q = fma(a, fma(a, fma(a, fma(a, 1.0 / 24, 1.0 / 6), 0.5), 1.0), 1.0) * table[k & (FS_TABLE - 1)];
+        return __longlong_as_double(__double_as_longlong(q) - ((long long)(k / FS_TABLE) << 52));  // (2^-46 at least)
     }
-    // mass of a value that the order keeps
-    __device__ __forceinline__ uint64_t mass(float x) const {
-        const double w = weight(x);
-        return (uint64_t)__double2ll_rn(w * FS_ONE);
-    }
+    // In units of 2^-44, to the nearest: the last bits of w + 2^8.
+    static __device__ __forceinline__ uint64_t units(double w) { return (uint64_t)(__double_as_longlong(w + 256.0) - __double_as_longlong(256.0)); }
+    __device__ __forceinline__ uint64_t mass(float x) const { return units(weight(x)); }
+    // of a value that the order keeps
     __device__ __forceinline__ uint64_t kept_mass(float x, uint64_t key) const {
         const double w = weight(x);
-        return w >= min_p || key == first ? (uint64_t)__double2ll_rn(w * FS_ONE) : 0;
+        return w >= min_p || key == first ? units(w) : 0;
     }
 };
 
@@ -110,6 +123,40 @@ __device__ __forceinline__ uint64_t block_before(uint64_t v, SampleShared& s) {
     return b;
 }
 
+// Exact mass of a bin: two 32-bit words, the carry by hand.
+__device__ __forceinline__ void add_mass(SampleShared& s, int bin, uint64_t w) {
+    const uint32_t lo = (uint32_t)w, old = atomicAdd(&s.low[bin], lo), hi = (uint32_t)(w >> 32) + (old + lo < old ? 1u : 0u);
+    if (hi) atomicAdd(&s.high[bin], hi);
+}
+
+// For every one of n keys in s.all: how many are above it, and their mass.  Several threads share a key when there are few: `lanes` of them, and all get the
+// sums.  body(e, i, place, above): i = the key's number, n or more for none; e counts this thread's keys.
+template <class Body>
+__device__ __forceinline__ void for_each_above(SampleShared& s, int n, Body&& body) {
+    int lanes = 16;
+    while (lanes > 1 && FS_THREADS / lanes < n) lanes /= 2;
+    const int q = threadIdx.x % lanes;
+#pragma unroll
+    for (int e = 0; e < FS_LIST / FS_THREADS; ++e) {
+        const int i = (int)threadIdx.x / lanes + e * (FS_THREADS / lanes);
+        if (e > 0 && FS_THREADS / lanes >= n) break;  // (the same for all threads)
+        const uint64_t key = i < n ? s.all[i] : ~0ull;
+        uint32_t place = 0;
+        uint64_t above = 0;
+#pragma unroll 4
+        for (int j = q; j < n; j += lanes) {
+            const bool yes = s.all[j] > key;
+            place += yes;
+            above += yes ? s.w[j] : 0;
+        }
+        for (int o = 1; o < lanes; o <<= 1) {
+            place += __shfl_xor_sync(0xffffffffu, place, o);
+            above += __shfl_xor_sync(0xffffffffu, above, o);
+        }
+        body(e, i, key, place, above, q == 0);
+    }
+}
+
 template <typename T>
 __global__ void __launch_bounds__(FS_THREADS) filtered_sample_kernel(const __grid_constant__ SampleParams p) {
     namespace cg = cooperative_groups;
@@ -118,7 +165,14 @@ __global__ void __launch_bounds__(FS_THREADS) filtered_sample_kernel(const __gri
     const cg::cluster_group cluster = cg::this_cluster();
     const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, rank = (int)blockIdx.x % p.cluster, row = (int)(blockIdx.x / p.cluster);
     const int first = rank * p.slice, n = max(0, min(p.slice, p.vocab - first));
+    if (tid < FS_TABLE) s.table[tid] = exp2(-(double)tid / FS_TABLE);
+    for (int i = tid; i < FS_BINS; i += FS_THREADS) s.low[i] = s.high[i] = 0;
+    if (tid == 0) s.survivors = 0;
     pdl_wait();
+    const float temperature = p.temperature ? p.temperature[row] : 1.f;
+    const int k = p.top_k ? p.top_k[row] : 0;
+    const float top_p = p.top_p ? p.top_p[row] : 1.f, min_p = p.min_p && p.min_p[row] > 0.f ? p.min_p[row] : 0.f;
+    double u = p.uniform[row];
 
     // the slice, its maximum (first of equals), its smallest finite value and how many values are choices at all
     float mx = -INFINITY, mn = INFINITY;
@@ -138,13 +192,16 @@ __global__ void __launch_bounds__(FS_THREADS) filtered_sample_kernel(const __gri
     const T* const src = (const T*)p.logits + row * p.stride + first;
     constexpr int V = 16 / sizeof(T);
     const int nv = ((uintptr_t)src & 15) == 0 ? n / V : 0;
+#pragma unroll 4
     for (int i = tid; i < nv; i += FS_THREADS) {
         float x[V];
         get(src + i * V, x);
 #pragma unroll
         for (int e = 0; e < V; ++e) take(i * V + e, x[e]);
     }
+#pragma unroll 4
     for (int i = nv * V + tid; i < n; i += FS_THREADS) take(i, to_f32(src[i]));
+    const float own_max = mx;
     for (int o = 16; o > 0; o >>= 1) {
         const float v = __shfl_xor_sync(0xffffffffu, mx, o);
         const uint32_t i = __shfl_xor_sync(0xffffffffu, mi, o);
@@ -162,7 +219,12 @@ __global__ void __launch_bounds__(FS_THREADS) filtered_sample_kernel(const __gri
         s.wcnt[warp] = usable;
     }
     __syncthreads();
+    float weakest = INFINITY;
+    for (int w = 0; w < FS_WARPS; ++w) weakest = fminf(weakest, s.wmax[w]);
     if (tid == 0) {
+        mx = -INFINITY;
+        mn = INFINITY;
+        mi = 0xffffffffu;
         usable = 0;
         for (int w = 0; w < FS_WARPS; ++w) {
             if (s.wmax[w] > mx || (s.wmax[w] == mx && s.widx[w] < mi)) {
@@ -177,12 +239,31 @@ __global__ void __launch_bounds__(FS_THREADS) filtered_sample_kernel(const __gri
         s.min = mn;
         s.usable = usable;
         s.listed = 0;
+        s.tau = -INFINITY;
     }
-    for (int i = tid; i < FS_BINS; i += FS_THREADS) {
-        s.count[i] = 0;
-        s.mass[i] = 0.f;
+    // The block's share of the k-th place: the value at that place among its threads' maxima (of up to 16: only those as large as the weakest warp's
+    // count, there are 16 of them at least).
+    const bool fast = k > 1 && k <= FS_FAST;
+    if (fast) {
+        const int place = (k + p.cluster - 1) / p.cluster - 1;
+        const bool in = place >= FS_WARPS || own_max >= weakest;
+        const unsigned v = __ballot_sync(0xffffffffu, in);
+        uint32_t at = 0;
+        if (lane == 0) at = atomicAdd(&s.survivors, __popc(v));
+        at = __shfl_sync(0xffffffffu, at, 0) + __popc(v & ((1u << lane) - 1u));
+        if (in) s.tmax[at] = own_max;
+        __syncthreads();
+        const int m = (int)s.survivors;
+        if (tid < m) {
+            const float mine = s.tmax[tid];
+            int above = 0;
+#pragma unroll 8
+            for (int j = 0; j < m; ++j) above += s.tmax[j] > mine || (s.tmax[j] == mine && j < tid);
+            if (above == place) s.tau = mine;
+        }
     }
     cluster.sync();
+    float tau = INFINITY;
     mx = -INFINITY;
     mn = INFINITY;
     mi = 0xffffffffu;
@@ -195,12 +276,10 @@ __global__ void __launch_bounds__(FS_THREADS) filtered_sample_kernel(const __gri
             mi = o->idx;
         }
         mn = fminf(mn, o->min);
+        tau = fminf(tau, o->tau);
         usable += o->usable;
     }
 
-    const float temperature = p.temperature ? p.temperature[row] : 1.f;
-    const int k = p.top_k ? p.top_k[row] : 0;
-    const float top_p = p.top_p ? p.top_p[row] : 1.f, min_p = p.min_p && p.min_p[row] > 0.f ? p.min_p[row] : 0.f;
     const bool has_k = k > 0 && (uint32_t)k < usable, has_p = top_p < 1.f;
     if (usable == 0 || !(temperature > 0.f) || k == 1 || top_p <= 0.f) {  // nothing to choose from, or to choose
         if (rank == 0 && tid == 0) {
@@ -211,24 +290,24 @@ __global__ void __launch_bounds__(FS_THREADS) filtered_sample_kernel(const __gri
         return;
     }
     SampleRow r;
-    r.max = mx;
-    r.dmax = (double)mx;
+    r.top = mx;
     r.rate = 1.4426950408889634 / (double)temperature;
+    r.shift = (double)mx * r.rate;
     r.floor_t = 46.0;
     r.min_p = (double)min_p;
     r.first = order_key(mx, mi);
-    double u = p.uniform[row];
+    r.table = s.table;
     u = u > 0.0 ? fmin(u, 1.0) : 0.0;
     // the last of the mass counts as not reached: u * whole rounds to at most whole, and the token is there where the sum exceeds it
     auto border = [&](uint64_t whole) { return min((uint64_t)(u * (double)whole), whole - 1); };
-
     const float span = fminf(mx - mn, 32.f * temperature);
     const float per = span > 1e-30f ? (float)FS_BINS / span : 1e30f;  // (an infinite span: everything in bin 0)
     auto bin_of = [&](float x) { return min(FS_BINS - 1, (int)((mx - x) * per)); };
     uint64_t cut = 0;  // key of the last that is kept
 
-    // Values of one kind, listed by every block, brought together by block 0.  Returns how many there are (all blocks know; more than FS_LIST: no list).
-    auto gather = [&](auto&& wanted) -> uint32_t {
+    // Values of one kind, listed by every block and brought together.  Returns how many there are (more than FS_LIST: no list).  everyone: for all
+    // blocks, else for block 0.
+    auto gather = [&](bool everyone, auto&& wanted) -> uint32_t {
         if (tid == 0) s.listed = 0;
         __syncthreads();
         for (int i0 = 0; i0 < n; i0 += FS_THREADS) {
@@ -243,18 +322,24 @@ __global__ void __launch_bounds__(FS_THREADS) filtered_sample_kernel(const __gri
             }
         }
         cluster.sync();
-        uint32_t all = 0, mine = 0;
-        for (int b = 0; b < p.cluster; ++b) all += cluster.map_shared_rank(&s, b)->listed;
-        if (rank == 0 && all <= FS_LIST) {
-            for (int b = 0; b < p.cluster; ++b) {
-                const SampleShared* o = cluster.map_shared_rank(&s, b);
-                const uint32_t c = o->listed;
-                for (uint32_t i = tid; i < c; i += FS_THREADS) {
-                    const uint64_t key = o->list[i];
-                    s.all[mine + i] = key;
-                    s.w[mine + i] = r.mass(from_ordered((uint32_t)(key >> 32)));
-                }
-                mine += c;
+        uint32_t all = 0, of[FS_CLUSTER];
+#pragma unroll
+        for (int b = 0; b < FS_CLUSTER; ++b) {
+            of[b] = b < p.cluster ? cluster.map_shared_rank(&s, b)->listed : 0;
+            all += of[b];
+        }
+        if (all <= FS_LIST && (everyone || rank == 0)) {
+            for (uint32_t i = tid; i < all; i += FS_THREADS) {
+                uint32_t b = 0, at = i;
+#pragma unroll
+                for (int c = 0; c < FS_CLUSTER - 1; ++c)
+                    if (b == (uint32_t)c && at >= of[c]) {
+                        at -= of[c];
+                        ++b;
+                    }
+                const uint64_t key = cluster.map_shared_rank(&s, b)->list[at];
+                s.all[i] = key;
+                s.w[i] = r.mass(from_ordered((uint32_t)(key >> 32)));
             }
             __syncthreads();
         }
@@ -283,30 +368,30 @@ __global__ void __launch_bounds__(FS_THREADS) filtered_sample_kernel(const __gri
         cluster.sync();
         return lo;
     };
-
-    bool chosen = false;
-    if (has_k) {
-        for (int i = tid; i < n; i += FS_THREADS) {
-            const int b = fs_x[i] > -INFINITY ? bin_of(fs_x[i]) : FS_BINS - 1;
-            if (b < FS_BINS - 1) atomicAdd(&s.count[b], 1u);  // (the last bin has the rest)
-        }
-        if (tid == 0) {
-            s.bin = FS_BINS - 1;
-            s.before = 0xffffffffu;
-        }
-        cluster.sync();
-        uint32_t c[FS_BINS / FS_THREADS], sum = 0;
+    // The bin at which the running measure (counts, or masses) reaches `most`, and the measure before it and with it; the last bin, which is not measured, has the rest.
+    auto reach = [&](double most) {
+        uint64_t c[FS_BINS / FS_THREADS], sum = 0;
 #pragma unroll
         for (int e = 0; e < FS_BINS / FS_THREADS; ++e) {
             c[e] = 0;
-            for (int b = 0; b < p.cluster; ++b) c[e] += cluster.map_shared_rank(&s, b)->count[tid * (FS_BINS / FS_THREADS) + e];
+            const int bin = tid * (FS_BINS / FS_THREADS) + e;
+            for (int b = 0; b < p.cluster; ++b) {
+                const SampleShared* o = cluster.map_shared_rank(&s, b);
+                c[e] += (uint64_t)o->high[bin] << 32;
+                c[e] += o->low[bin];
+            }
             sum += c[e];
         }
-        uint32_t before = (uint32_t)block_before(sum, s);
-        const uint32_t binned = (uint32_t)block_total(sum, s);
+        uint64_t before = block_before(sum, s);
+        if (tid == FS_THREADS - 1) {
+            s.bin = FS_BINS - 1;
+            s.before = before + sum;
+            s.found = ~0ull;
+        }
+        __syncthreads();
 #pragma unroll
         for (int e = 0; e < FS_BINS / FS_THREADS; ++e) {
-            if (before < (uint32_t)k && before + c[e] >= (uint32_t)k) {
+            if ((double)before < most && (double)(before + c[e]) >= most) {
                 s.bin = tid * (FS_BINS / FS_THREADS) + e;
                 s.before = before;
                 s.found = before + c[e];
@@ -314,86 +399,77 @@ __global__ void __launch_bounds__(FS_THREADS) filtered_sample_kernel(const __gri
             before += c[e];
         }
         __syncthreads();
-        const int bk = s.bin;
-        const uint32_t ahead = s.before != 0xffffffffu ? s.before : binned, upto = s.before != 0xffffffffu ? (uint32_t)s.found : usable;
-        if (upto <= FS_LIST) {
+    };
+
+    if (has_k) {
+        uint32_t m = FS_LIST + 1;
+        if (fast) m = gather(false, [&](float x, uint32_t) { return x >= tau; });
+        if (m <= FS_LIST) {
             // everything that is kept is among these
-            gather([&](float x, uint32_t) { return bin_of(x) <= bk; });
             if (rank == 0) {
-                const int m = (int)upto;
-                uint64_t key[FS_LIST / FS_THREADS], w[FS_LIST / FS_THREADS], above[FS_LIST / FS_THREADS] = {}, mass_k = 0;
-                uint32_t place[FS_LIST / FS_THREADS] = {};
-#pragma unroll
-                for (int e = 0; e < FS_LIST / FS_THREADS; ++e) {
-                    const int i = tid + e * FS_THREADS;
-                    key[e] = i < m ? s.all[i] : 0;
-                    w[e] = i < m ? s.w[i] : 0;
-                }
-                for (int j = 0; j < m; ++j) {
-                    const uint64_t kj = s.all[j], wj = s.w[j];
-#pragma unroll
-                    for (int e = 0; e < FS_LIST / FS_THREADS; ++e) {
-                        place[e] += kj > key[e];
-                        above[e] += kj > key[e] ? wj : 0;
-                    }
-                }
-#pragma unroll
-                for (int e = 0; e < FS_LIST / FS_THREADS; ++e) mass_k += place[e] < (uint32_t)k ? w[e] : 0;
-                mass_k = block_total(mass_k, s);
-                const double most = (double)top_p * (double)mass_k;
+                constexpr int E = FS_LIST / FS_THREADS;
+                uint64_t above[E] = {}, key[E] = {}, w[E] = {}, mass_k = 0;
+                uint32_t place[E] = {};
+                bool mine[E] = {};  // (one of the threads that share a key)
+                for_each_above(s, (int)m, [&](int e, int i, uint64_t ke, uint32_t pl, uint64_t ab, bool one) {
+                    mine[e] = one && i < (int)m;
+                    key[e] = ke;
+                    place[e] = pl;
+                    above[e] = ab;
+                    w[e] = mine[e] && pl < (uint32_t)k ? s.w[i] : 0;
+                    mass_k += w[e];
+                });
+                const double most = (double)top_p * (double)block_total(mass_k, s);
                 uint64_t whole = 0;
 #pragma unroll
-                for (int e = 0; e < FS_LIST / FS_THREADS; ++e) {
-                    const int i = tid + e * FS_THREADS;
-                    const bool keep = i < m && place[e] < (uint32_t)k && (!has_p || (double)above[e] < most || key[e] == r.first);
+                for (int e = 0; e < E; ++e) {
+                    const bool keep = mine[e] && place[e] < (uint32_t)k && (!has_p || (double)above[e] < most || key[e] == r.first);
                     w[e] = keep ? r.kept_mass(from_ordered((uint32_t)(key[e] >> 32)), key[e]) : 0;
                     whole += w[e];
                 }
-                whole = block_total(whole, s);  // (its barriers: everyone has read s.w)
+                whole = block_total(whole, s);  // (its barriers: everyone has read s.all and s.w)
+                // the kept ones again, ordered by index: keys with the index in front
 #pragma unroll
-                for (int e = 0; e < FS_LIST / FS_THREADS; ++e)
-                    if (tid + e * FS_THREADS < m) s.w[tid + e * FS_THREADS] = w[e];
-                if (tid == 0) s.choice = 0xffffffffu;
+                for (int e = 0; e < E; ++e)
+                    if (mine[e]) {
+                        s.all[place[e]] = w[e] ? (key[e] & 0xffffffffu) : 0;  // (higher for a lower index)
+                        s.w[place[e]] = w[e];
+                    }
                 __syncthreads();
                 const uint64_t most_u = border(whole);
-                uint64_t run[FS_LIST / FS_THREADS] = {};  // mass up to this one, by index
-                for (int j = 0; j < m; ++j) {
-                    const uint32_t kj = (uint32_t)s.all[j];  // (the higher the lower the index)
-                    const uint64_t wj = s.w[j];
-#pragma unroll
-                    for (int e = 0; e < FS_LIST / FS_THREADS; ++e) run[e] += kj >= (uint32_t)key[e] ? wj : 0;
-                }
-#pragma unroll
-                for (int e = 0; e < FS_LIST / FS_THREADS; ++e)
-                    if (w[e] && run[e] > most_u) atomicMin(&s.choice, 0xffffffffu - (uint32_t)key[e]);
-                __syncthreads();
-#pragma unroll
-                for (int e = 0; e < FS_LIST / FS_THREADS; ++e)
-                    if (w[e] && 0xffffffffu - (uint32_t)key[e] == s.choice) {
-                        p.tokens[row] = (int)s.choice;
-                        if (p.probs) p.probs[row] = (float)((double)w[e] / (double)whole);
+                for_each_above(s, (int)m, [&](int e, int i, uint64_t ke, uint32_t, uint64_t ab, bool one) {
+                    if (one && i < (int)m && ke && ab <= most_u && most_u < ab + s.w[i]) {  // (of one key only)
+                        p.tokens[row] = (int)(0xffffffffu - (uint32_t)ke);
+                        if (p.probs) p.probs[row] = (float)((double)s.w[i] / (double)whole);
                     }
-            }
-            chosen = true;
-        } else if (upto - ahead <= FS_LIST) {
-            gather([&](float x, uint32_t) { return bin_of(x) == bk; });
-            if (rank == 0) {
-                const int m = (int)(upto - ahead);
-                for (int i = tid; i < m; i += FS_THREADS) {
-                    uint32_t place = ahead;
-                    for (int j = 0; j < m; ++j) place += s.all[j] > s.all[i];
-                    if (place == (uint32_t)k - 1) s.cut = s.all[i];
-                }
+                });
             }
             cluster.sync();
-            cut = cluster.map_shared_rank(&s, 0)->cut;
+            return;
+        }
+        for (int i = tid; i < n; i += FS_THREADS) {
+            const int b = fs_x[i] > -INFINITY ? bin_of(fs_x[i]) : FS_BINS - 1;
+            if (b < FS_BINS - 1) atomicAdd(&s.low[b], 1u);
+        }
+        cluster.sync();
+        reach((double)k);
+        const int bk = s.bin;
+        const uint32_t ahead = (uint32_t)s.before, upto = s.found != ~0ull ? (uint32_t)s.found : usable;
+        if (upto - ahead <= FS_LIST) {
+            m = gather(true, [&](float x, uint32_t) { return bin_of(x) == bk; });
+            for_each_above(s, (int)m, [&](int, int i, uint64_t key, uint32_t place, uint64_t, bool one) {
+                if (one && i < (int)m && ahead + place == (uint32_t)k - 1) s.found = key;
+            });
+            __syncthreads();
+            cut = s.found;
         } else {
             cut = bisect([](float, uint64_t) { return (uint64_t)1; }, (double)k);
         }
-    }
-    if (chosen) {
-        cluster.sync();
-        return;
+        if (has_p) {
+            cluster.sync();  // (all have read the counts)
+            for (int i = tid; i < FS_BINS; i += FS_THREADS) s.low[i] = s.high[i] = 0;
+            __syncthreads();
+        }
     }
 
     if (has_p) {
@@ -404,82 +480,27 @@ __global__ void __launch_bounds__(FS_THREADS) filtered_sample_kernel(const __gri
                 const uint64_t w = r.mass(x);
                 const int b = bin_of(x);
                 sum += w;
-                if (b < FS_BINS - 1) atomicAdd(&s.mass[b], (float)w);  // (a guess: its rounding hangs on the order)
+                if (w && b < FS_BINS - 1) add_mass(s, b, w);
             }
         }
         sum = block_total(sum, s);
-        if (tid == 0) {
-            s.total[0] = sum;
-            s.bin = FS_BINS - 1;
-        }
+        if (tid == 0) s.total[0] = sum;
         cluster.sync();
         uint64_t whole = 0;
         for (int b = 0; b < p.cluster; ++b) whole += cluster.map_shared_rank(&s, b)->total[0];
         const double most = (double)top_p * (double)whole;
-        if (rank == 0) {  // the guess
-            float c[FS_BINS / FS_THREADS];
-            uint64_t mine = 0;
-#pragma unroll
-            for (int e = 0; e < FS_BINS / FS_THREADS; ++e) {
-                c[e] = 0.f;
-                for (int b = 0; b < p.cluster; ++b) c[e] += cluster.map_shared_rank(&s, b)->mass[tid * (FS_BINS / FS_THREADS) + e];
-                mine += (uint64_t)c[e];
-            }
-            uint64_t before = block_before(mine, s);
-#pragma unroll
-            for (int e = 0; e < FS_BINS / FS_THREADS; ++e) {
-                const uint64_t after = before + (uint64_t)c[e];
-                if ((double)before < most && (double)after >= most) s.bin = tid * (FS_BINS / FS_THREADS) + e;
-                before = after;
-            }
-        }
-        cluster.sync();
-        int bp = cluster.map_shared_rank(&s, 0)->bin;
-        uint64_t ahead = 0;
-        uint32_t listed;
-        for (;;) {  // one way only: down while too much lies before the bin, up while too little lies before its end
-            uint64_t before = 0, in = 0;
-            listed = gather([&](float x, uint32_t index) {
-                if (order_key(x, index) < cut) return false;
-                const int b = bin_of(x);
-                if (b > bp) return false;
-                const uint64_t w = r.mass(x);
-                before += b < bp ? w : 0;
-                in += b == bp ? w : 0;
-                return b == bp;
+        reach(most);
+        const int bp = s.bin;
+        const uint64_t ahead = s.before;
+        const uint32_t m = gather(true, [&](float x, uint32_t index) { return bin_of(x) == bp && order_key(x, index) >= cut; });
+        if (m <= FS_LIST) {
+            if (tid == 0) s.found = r.first;  // (the first is always kept)
+            __syncthreads();
+            for_each_above(s, (int)m, [&](int, int i, uint64_t key, uint32_t, uint64_t above, bool one) {
+                if (one && i < (int)m && (double)(ahead + above) < most) atomicMin((unsigned long long*)&s.found, (unsigned long long)key);
             });
-            before = block_total(before, s);
-            in = block_total(in, s);
-            if (tid == 0) {
-                s.total[0] = before;
-                s.total[1] = in;
-            }
-            cluster.sync();
-            before = in = 0;
-            for (int b = 0; b < p.cluster; ++b) {
-                before += cluster.map_shared_rank(&s, b)->total[0];
-                in += cluster.map_shared_rank(&s, b)->total[1];
-            }
-            cluster.sync();  // (all have read before any writes again)
-            ahead = before;
-            if ((double)before >= most && bp > 0) --bp;
-            else if ((double)(before + in) < most && bp < FS_BINS - 1) ++bp;
-            else break;
-        }
-        if (listed <= FS_LIST) {
-            if (rank == 0) {
-                if (tid == 0) s.found = ~0ull;
-                __syncthreads();
-                for (uint32_t i = tid; i < listed; i += FS_THREADS) {
-                    uint64_t above = ahead;
-                    for (uint32_t j = 0; j < listed; ++j) above += s.all[j] > s.all[i] ? s.w[j] : 0;
-                    if ((double)above < most) atomicMin((unsigned long long*)&s.found, (unsigned long long)s.all[i]);
-                }
-                __syncthreads();
-                if (tid == 0) s.cut = min(s.found, r.first);  // (the first is always kept)
-            }
-            cluster.sync();
-            cut = max(cut, cluster.map_shared_rank(&s, 0)->cut);
+            __syncthreads();
+            cut = max(cut, s.found);
         } else {
             const uint64_t old = cut;
             cut = max(old, bisect([&](float x, uint64_t key) { return key >= old ? r.mass(x) : (uint64_t)0; }, most));
@@ -504,11 +525,11 @@ __global__ void __launch_bounds__(FS_THREADS) filtered_sample_kernel(const __gri
     __syncthreads();
     sum = 0;
     for (int w = 0; w < FS_WARPS; ++w) sum += s.sums[w];
-    if (tid == 0) s.total[0] = sum;
+    if (tid == 0) s.total[1] = sum;
     cluster.sync();
     uint64_t whole = 0, ahead = 0;
     for (int b = 0; b < p.cluster; ++b) {
-        const uint64_t t = cluster.map_shared_rank(&s, b)->total[0];
+        const uint64_t t = cluster.map_shared_rank(&s, b)->total[1];
         whole += t;
         ahead += b < rank ? t : 0;
     }
