@@ -6,13 +6,17 @@
 // A cluster of up to eight blocks holds a row in its shared memory, read once; every pass after that is over shared memory.  Masses are whole numbers of
 // 2^-44 of the largest weight (weights computed in 64 bits), so that sums do not depend on their order and no cut or choice hangs on the blocks or on atomics.
 //   top-k up to FS_FAST: every block takes its share of the k-th place among its threads' maxima, so that the lowest of the blocks' values has at least k
-//     values above it; the few that are no smaller are brought together, and everything else happens among those.
+//     values that are no smaller; those few go to the first block, which does the rest alone while the others leave.
 //   other cuts: equal bins of the distance from the maximum are counted, or weighed; only the bin with the k-th value, or the nucleus' border, is listed and
 //     ordered, by counting.  More than FS_LIST values in one bin (many equal logits): bisection on (value, index), a pass per bit.
 //   the choice: masses of stretches of the row, then inside the stretch that holds it.
-// What every block needs it works out for itself from the others' shared memory: a barrier of the cluster costs more than that.
-// A pass that weighs all logits is bound by 64-bit arithmetic, one over a few candidates by the barriers; the logits' read is the floor.
+// Blocks write what the others need into the others' shared memory in front of a barrier, so that it is at hand behind it; nothing is fetched from a block
+// after the last barrier, so blocks leave at once.
+// Passes that compare take four logits at a time.  A pass that weighs all logits is bound by 64-bit arithmetic (about 40 issue slots per logit and
+// scheduler); with a cut below it the kept logits are collected 32 at a time first.  With a top-k the barriers are what is left over the logits' read.
 #pragma once
+#include <cfloat>
+
 #include <cooperative_groups.h>
 
 #include "paged_append.cuh"
@@ -39,21 +43,23 @@ struct SampleShared {
         struct {
             uint32_t low[FS_BINS], high[FS_BINS];  // of each bin: the count in `low`, or the mass
         };
-        uint64_t w[FS_LIST];  // weights of `all`, once all blocks have read the bins (a gathering's barrier is behind that)
+        uint64_t w[FS_LIST];  // masses of `all`, once all blocks have read the bins (a gathering's barrier is behind that)
     };
-    uint64_t list[FS_LIST];
-    uint64_t all[FS_LIST];                 // the lists of all blocks
-    double table[FS_TABLE];                // 2^(-i / FS_TABLE)
+    uint64_t all[FS_LIST];     // keys that the blocks have listed
+    uint64_t sorted[FS_FAST];
+    double table[FS_TABLE];    // 2^(-i / FS_TABLE)
     uint64_t sums[FS_WARPS];
     float wmax[FS_WARPS], wmin[FS_WARPS], tmax[FS_THREADS];
-    uint32_t widx[FS_WARPS], wcnt[FS_WARPS];
-    // what other blocks read
-    float max, min, tau;
-    uint32_t idx, usable, listed;
-    uint64_t total[2];
+    float queue[FS_WARPS][64];
+    // of each block of the cluster, written by it
+    float max[FS_CLUSTER], min[FS_CLUSTER], tau[FS_CLUSTER];
+    uint32_t count[3][FS_CLUSTER];  // listed for a top-k, for the bin with the k-th value, for the nucleus' bin
+    uint64_t total[3][FS_CLUSTER];  // two in turn, and the last one
+    uint32_t listed[3];             // of the first block: where the next keys go
     // found by one thread, used by all
+    float own_tau;
+    uint32_t survivors, base, usable;
     int bin;
-    uint32_t survivors, choice;
     uint64_t before, found;
 };
 
@@ -67,8 +73,7 @@ __device__ __forceinline__ uint64_t order_key(float x, uint32_t index) { return 
 struct SampleRow {
     float top;
     double shift, rate, floor_t;  // w = 2^-t, t = shift - x * rate; floor_t: no weight beyond
-    double min_p;
-    uint64_t first;  // key of the first token: always kept
+    double min_p;  // at most 1: the first token is always kept
     const double* table;
     // 2^-t: t to the nearest 1/128 from the table, the rest (a = rest * ln 2 up to 0.0027) by the exponential series up to a^4 / 24; a^5 / 120 is 1.2e-15.
     __device__ __forceinline__ double weight(float x) const {
@@ -86,9 +91,9 @@ struct SampleRow {
     static __device__ __forceinline__ uint64_t units(double w) { return (uint64_t)(__double_as_longlong(w + 256.0) - __double_as_longlong(256.0)); }
     __device__ __forceinline__ uint64_t mass(float x) const { return units(weight(x)); }
     // of a value that the order keeps
-    __device__ __forceinline__ uint64_t kept_mass(float x, uint64_t key) const {
+    __device__ __forceinline__ uint64_t kept_mass(float x) const {
         const double w = weight(x);
-        return w >= min_p || key == first ? units(w) : 0;
+        return w >= min_p ? units(w) : 0;
     }
 };
 
@@ -129,65 +134,68 @@ __device__ __forceinline__ void add_mass(SampleShared& s, int bin, uint64_t w) {
     if (hi) atomicAdd(&s.high[bin], hi);
 }
 
-// For every one of n keys in s.all: how many are above it, and their mass.  Several threads share a key when there are few: `lanes` of them, and all get the
-// sums.  body(e, i, place, above): i = the key's number, n or more for none; e counts this thread's keys.
+// How many of the first n of `keys` are above keys[i], for each i: several threads share an i when there are few, and one of them calls body(i, count).
 template <class Body>
-__device__ __forceinline__ void for_each_above(SampleShared& s, int n, Body&& body) {
+__device__ __forceinline__ void places(const uint64_t* keys, int n, Body&& body) {
     int lanes = 16;
     while (lanes > 1 && FS_THREADS / lanes < n) lanes /= 2;
     const int q = threadIdx.x % lanes;
-#pragma unroll
-    for (int e = 0; e < FS_LIST / FS_THREADS; ++e) {
-        const int i = (int)threadIdx.x / lanes + e * (FS_THREADS / lanes);
-        if (e > 0 && FS_THREADS / lanes >= n) break;  // (the same for all threads)
-        const uint64_t key = i < n ? s.all[i] : ~0ull;
+    for (int i0 = 0; i0 < n; i0 += FS_THREADS / lanes) {  // (the same for all threads)
+        const int i = i0 + (int)threadIdx.x / lanes;
+        const uint64_t key = i < n ? keys[i] : ~0ull;
         uint32_t place = 0;
+#pragma unroll 8
+        for (int j = q; j < n; j += lanes) place += keys[j] > key;
+        for (int o = 1; o < lanes; o <<= 1) place += __shfl_xor_sync(0xffffffffu, place, o);
+        if (q == 0 && i < n) body(i, place);
+    }
+}
+// The same with the mass above: of keys[j], mass[j].
+template <class Body>
+__device__ __forceinline__ void masses_above(const uint64_t* keys, const uint64_t* mass, int n, Body&& body) {
+    int lanes = 16;
+    while (lanes > 1 && FS_THREADS / lanes < n) lanes /= 2;
+    const int q = threadIdx.x % lanes;
+    for (int i0 = 0; i0 < n; i0 += FS_THREADS / lanes) {
+        const int i = i0 + (int)threadIdx.x / lanes;
+        const uint64_t key = i < n ? keys[i] : ~0ull;
         uint64_t above = 0;
 #pragma unroll 4
-        for (int j = q; j < n; j += lanes) {
-            const bool yes = s.all[j] > key;
-            place += yes;
-            above += yes ? s.w[j] : 0;
-        }
-        for (int o = 1; o < lanes; o <<= 1) {
-            place += __shfl_xor_sync(0xffffffffu, place, o);
-            above += __shfl_xor_sync(0xffffffffu, above, o);
-        }
-        body(e, i, key, place, above, q == 0);
+        for (int j = q; j < n; j += lanes) above += keys[j] > key ? mass[j] : 0;
+        for (int o = 1; o < lanes; o <<= 1) above += __shfl_xor_sync(0xffffffffu, above, o);
+        if (q == 0 && i < n) body(i, above);
     }
 }
 
 template <typename T>
-__global__ void __launch_bounds__(FS_THREADS) filtered_sample_kernel(const __grid_constant__ SampleParams p) {
+__global__ void __launch_bounds__(FS_THREADS, 2) filtered_sample_kernel(const __grid_constant__ SampleParams p) {
     namespace cg = cooperative_groups;
     extern __shared__ __align__(16) float fs_x[];
     __shared__ SampleShared s;
     const cg::cluster_group cluster = cg::this_cluster();
     const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, rank = (int)blockIdx.x % p.cluster, row = (int)(blockIdx.x / p.cluster);
-    const int first = rank * p.slice, n = max(0, min(p.slice, p.vocab - first));
+    const int first = rank * p.slice, n = max(0, min(p.slice, p.vocab - first)), quads = (n + 3) / 4;
     if (tid < FS_TABLE) s.table[tid] = exp2(-(double)tid / FS_TABLE);
     for (int i = tid; i < FS_BINS; i += FS_THREADS) s.low[i] = s.high[i] = 0;
-    if (tid == 0) s.survivors = 0;
+    if (tid < 3) s.listed[tid] = 0;
+    if (tid == 0) {
+        s.survivors = s.usable = 0;
+        s.own_tau = -INFINITY;
+    }
+    cluster_arrive();  // (waited for before the first word goes to another block: that block has begun, and its counters are zero)
     pdl_wait();
     const float temperature = p.temperature ? p.temperature[row] : 1.f;
     const int k = p.top_k ? p.top_k[row] : 0;
-    const float top_p = p.top_p ? p.top_p[row] : 1.f, min_p = p.min_p && p.min_p[row] > 0.f ? p.min_p[row] : 0.f;
+    const float top_p = p.top_p ? p.top_p[row] : 1.f, min_p = p.min_p ? p.min_p[row] : 0.f;
     double u = p.uniform[row];
 
-    // the slice, its maximum (first of equals), its smallest finite value and how many values are choices at all
+    // the slice, its maximum and its smallest finite value; no numbers become -inf, which is no choice
     float mx = -INFINITY, mn = INFINITY;
-    uint32_t mi = 0xffffffffu, usable = 0;
-    auto take = [&](int i, float x) {
-        x = x > -INFINITY ? x + 0.f : -INFINITY;  // no number: no choice
-        fs_x[i] = x;
-        if (x > mx) {
-            mx = x;
-            mi = (uint32_t)(first + i);
-        }
-        if (x > -INFINITY) {
-            ++usable;
-            mn = fminf(mn, x);
-        }
+    auto take = [&](float x) {
+        x = fmaxf(x, -INFINITY);
+        mx = fmaxf(mx, x);
+        mn = fminf(mn, x > -INFINITY ? x : INFINITY);
+        return x;
     };
     const T* const src = (const T*)p.logits + row * p.stride + first;
     constexpr int V = 16 / sizeof(T);
@@ -197,96 +205,92 @@ __global__ void __launch_bounds__(FS_THREADS) filtered_sample_kernel(const __gri
         float x[V];
         get(src + i * V, x);
 #pragma unroll
-        for (int e = 0; e < V; ++e) take(i * V + e, x[e]);
+        for (int e = 0; e < V; ++e) x[e] = take(x[e]);
+#pragma unroll
+        for (int e = 0; e < V; e += 4) *reinterpret_cast<float4*>(fs_x + i * V + e) = make_float4(x[e], x[e + 1], x[e + 2], x[e + 3]);
     }
-#pragma unroll 4
-    for (int i = nv * V + tid; i < n; i += FS_THREADS) take(i, to_f32(src[i]));
+#pragma unroll 8
+    for (int i = nv * V + tid; i < n; i += FS_THREADS) fs_x[i] = take(to_f32(src[i]));
+    if (tid < quads * 4 - n) fs_x[n + tid] = -INFINITY;
     const float own_max = mx;
-    for (int o = 16; o > 0; o >>= 1) {
-        const float v = __shfl_xor_sync(0xffffffffu, mx, o);
-        const uint32_t i = __shfl_xor_sync(0xffffffffu, mi, o);
-        if (v > mx || (v == mx && i < mi)) {
-            mx = v;
-            mi = i;
+    mx = warp_max(mx);
+    mn = -warp_max(-mn);
+    // The block's share of the k-th place: the value at that place among its threads' maxima.  Only those count that are as large as the weakest warp's
+    // value at its own share of that place: there are enough of them.
+    const bool fast = k > 1 && k <= FS_FAST;
+    const int place = fast ? (k + p.cluster - 1) / p.cluster - 1 : 0;
+    float mine = mx;
+    if (fast) {
+        float left = own_max;
+        for (int j = place / FS_WARPS; j > 0; --j) {  // the warp's largest maxima one after the other
+            const unsigned with = __ballot_sync(0xffffffffu, left == mine);
+            if (lane == __ffs(with) - 1) left = -INFINITY;
+            mine = warp_max(left);
         }
-        mn = fminf(mn, __shfl_xor_sync(0xffffffffu, mn, o));
-        usable += __shfl_xor_sync(0xffffffffu, usable, o);
     }
     if (lane == 0) {
         s.wmax[warp] = mx;
-        s.widx[warp] = mi;
         s.wmin[warp] = mn;
-        s.wcnt[warp] = usable;
+        s.sums[warp] = __float_as_uint(mine);
     }
     __syncthreads();
     float weakest = INFINITY;
-    for (int w = 0; w < FS_WARPS; ++w) weakest = fminf(weakest, s.wmax[w]);
-    if (tid == 0) {
-        mx = -INFINITY;
-        mn = INFINITY;
-        mi = 0xffffffffu;
-        usable = 0;
-        for (int w = 0; w < FS_WARPS; ++w) {
-            if (s.wmax[w] > mx || (s.wmax[w] == mx && s.widx[w] < mi)) {
-                mx = s.wmax[w];
-                mi = s.widx[w];
-            }
-            mn = fminf(mn, s.wmin[w]);
-            usable += s.wcnt[w];
-        }
-        s.max = mx;
-        s.idx = mi;
-        s.min = mn;
-        s.usable = usable;
-        s.listed = 0;
-        s.tau = -INFINITY;
+    mx = -INFINITY;
+#pragma unroll
+    for (int w = 0; w < FS_WARPS; ++w) {
+        mx = fmaxf(mx, s.wmax[w]);
+        mn = fminf(mn, s.wmin[w]);
+        weakest = fminf(weakest, __uint_as_float((uint32_t)s.sums[w]));
     }
-    // The block's share of the k-th place: the value at that place among its threads' maxima (of up to 16: only those as large as the weakest warp's
-    // count, there are 16 of them at least).
-    const bool fast = k > 1 && k <= FS_FAST;
     if (fast) {
-        const int place = (k + p.cluster - 1) / p.cluster - 1;
-        const bool in = place >= FS_WARPS || own_max >= weakest;
+        const bool in = own_max >= weakest;
         const unsigned v = __ballot_sync(0xffffffffu, in);
         uint32_t at = 0;
-        if (lane == 0) at = atomicAdd(&s.survivors, __popc(v));
+        if (lane == 0 && v) at = atomicAdd(&s.survivors, __popc(v));
         at = __shfl_sync(0xffffffffu, at, 0) + __popc(v & ((1u << lane) - 1u));
         if (in) s.tmax[at] = own_max;
         __syncthreads();
         const int m = (int)s.survivors;
         if (tid < m) {
-            const float mine = s.tmax[tid];
+            const float t = s.tmax[tid];
             int above = 0;
 #pragma unroll 8
-            for (int j = 0; j < m; ++j) above += s.tmax[j] > mine || (s.tmax[j] == mine && j < tid);
-            if (above == place) s.tau = mine;
+            for (int j = 0; j < m; ++j) above += s.tmax[j] > t || (s.tmax[j] == t && j < tid);
+            if (above == place) s.own_tau = t;
         }
+        __syncthreads();
+    }
+    cluster_wait();
+    if (tid < p.cluster) {
+        SampleShared* const o = cluster.map_shared_rank(&s, tid);
+        o->max[rank] = mx;
+        o->min[rank] = mn;
+        o->tau[rank] = s.own_tau;
     }
     cluster.sync();
     float tau = INFINITY;
-    mx = -INFINITY;
-    mn = INFINITY;
-    mi = 0xffffffffu;
-    usable = 0;
     for (int b = 0; b < p.cluster; ++b) {
-        const SampleShared* o = cluster.map_shared_rank(&s, b);
-        const float v = o->max;
-        if (v > mx) {  // (the lower index first: blocks hold ascending ranges)
-            mx = v;
-            mi = o->idx;
-        }
-        mn = fminf(mn, o->min);
-        tau = fminf(tau, o->tau);
-        usable += o->usable;
+        mx = fmaxf(mx, s.max[b]);
+        mn = fminf(mn, s.min[b]);
+        tau = fminf(tau, s.tau[b]);
     }
-
-    const bool has_k = k > 0 && (uint32_t)k < usable, has_p = top_p < 1.f;
-    if (usable == 0 || !(temperature > 0.f) || k == 1 || top_p <= 0.f) {  // nothing to choose from, or to choose
-        if (rank == 0 && tid == 0) {
-            p.tokens[row] = usable ? (int)mi : -1;
-            if (p.probs) p.probs[row] = usable ? 1.f : 0.f;
+    const bool has_p = top_p < 1.f;
+    if (mx == -INFINITY || !(temperature > 0.f) || k == 1 || top_p <= 0.f) {  // nothing to choose from, or to choose: the first maximum
+        int b = 0;
+        while (s.max[b] < mx) ++b;
+        if (rank != b) return;
+        if (tid == 0) s.base = 0xffffffffu;
+        __syncthreads();
+        for (int i = tid; i < n; i += FS_THREADS)
+            if (fs_x[i] == mx) {
+                atomicMin(&s.base, (uint32_t)(first + i));
+                break;
+            }
+        __syncthreads();
+        if (tid == 0) {
+            p.tokens[row] = mx > -INFINITY ? (int)s.base : -1;
+            if (p.probs) p.probs[row] = mx > -INFINITY ? 1.f : 0.f;
         }
-        cluster.sync();  // (nobody leaves while its shared memory is read)
         return;
     }
     SampleRow r;
@@ -294,8 +298,7 @@ __global__ void __launch_bounds__(FS_THREADS) filtered_sample_kernel(const __gri
     r.rate = 1.4426950408889634 / (double)temperature;
     r.shift = (double)mx * r.rate;
     r.floor_t = 46.0;
-    r.min_p = (double)min_p;
-    r.first = order_key(mx, mi);
+    r.min_p = min_p > 0.f ? fmin((double)min_p, 1.0) : 0.0;
     r.table = s.table;
     u = u > 0.0 ? fmin(u, 1.0) : 0.0;
     // the last of the mass counts as not reached: u * whole rounds to at most whole, and the token is there where the sum exceeds it
@@ -305,49 +308,48 @@ __global__ void __launch_bounds__(FS_THREADS) filtered_sample_kernel(const __gri
     auto bin_of = [&](float x) { return min(FS_BINS - 1, (int)((mx - x) * per)); };
     uint64_t cut = 0;  // key of the last that is kept
 
-    // Values of one kind, listed by every block and brought together.  Returns how many there are (more than FS_LIST: no list).  everyone: for all
-    // blocks, else for block 0.
-    auto gather = [&](bool everyone, auto&& wanted) -> uint32_t {
-        if (tid == 0) s.listed = 0;
-        __syncthreads();
-        for (int i0 = 0; i0 < n; i0 += FS_THREADS) {
-            const int i = i0 + tid;
-            const bool yes = i < n && fs_x[i] > -INFINITY && wanted(fs_x[i], (uint32_t)(first + i));
-            const unsigned v = __ballot_sync(0xffffffffu, yes);
-            if (v) {
-                uint32_t at = 0;
-                if (lane == 0) at = atomicAdd(&s.listed, __popc(v));
-                at = __shfl_sync(0xffffffffu, at, 0) + __popc(v & ((1u << lane) - 1u));
-                if (yes && at < FS_LIST) s.list[at] = order_key(fs_x[i], (uint32_t)(first + i));
+    // Values between lo and hi that pass `wanted`, of all blocks, to the first block's list or to everyone's.  Returns how many there are; more than FS_LIST:
+    // no list.  One barrier of the cluster.
+    auto gather = [&](int which, bool everyone, float lo, float hi, auto&& wanted) -> uint32_t {
+        uint32_t mine = 0;
+        for (int i = tid; i < quads; i += FS_THREADS) {
+            const float4 x = *reinterpret_cast<const float4*>(fs_x + 4 * i);
+            const float xs[4] = {x.x, x.y, x.z, x.w};
+            if ((xs[0] >= lo && xs[0] <= hi) || (xs[1] >= lo && xs[1] <= hi) || (xs[2] >= lo && xs[2] <= hi) || (xs[3] >= lo && xs[3] <= hi)) {
+                for (int e = 0; e < 4; ++e) mine += xs[e] >= lo && xs[e] <= hi && wanted(xs[e], order_key(xs[e], (uint32_t)(first + 4 * i + e)));
             }
+        }
+        uint32_t at = (uint32_t)block_before(mine, s);
+        if (tid == FS_THREADS - 1) {
+            const uint32_t here = at + mine;
+            s.base = here && here <= FS_LIST ? atomicAdd(&cluster.map_shared_rank(&s, 0)->listed[which], here) : FS_LIST;
+            for (int b = 0; b < p.cluster; ++b) cluster.map_shared_rank(&s, b)->count[which][rank] = here;
+        }
+        __syncthreads();
+        at += s.base;
+        if (mine) {
+            for (int i = tid; i < quads; i += FS_THREADS)
+                for (int e = 0; e < 4; ++e) {
+                    const float x = fs_x[4 * i + e];
+                    const uint64_t key = order_key(x, (uint32_t)(first + 4 * i + e));
+                    if (x >= lo && x <= hi && wanted(x, key)) {
+                        if (at < FS_LIST)
+                            for (int b = 0; b < (everyone ? p.cluster : 1); ++b) cluster.map_shared_rank(&s, b)->all[at] = key;
+                        ++at;
+                    }
+                }
         }
         cluster.sync();
-        uint32_t all = 0, of[FS_CLUSTER];
-#pragma unroll
-        for (int b = 0; b < FS_CLUSTER; ++b) {
-            of[b] = b < p.cluster ? cluster.map_shared_rank(&s, b)->listed : 0;
-            all += of[b];
-        }
-        if (all <= FS_LIST && (everyone || rank == 0)) {
-            for (uint32_t i = tid; i < all; i += FS_THREADS) {
-                uint32_t b = 0, at = i;
-#pragma unroll
-                for (int c = 0; c < FS_CLUSTER - 1; ++c)
-                    if (b == (uint32_t)c && at >= of[c]) {
-                        at -= of[c];
-                        ++b;
-                    }
-                const uint64_t key = cluster.map_shared_rank(&s, b)->list[at];
-                s.all[i] = key;
-                s.w[i] = r.mass(from_ordered((uint32_t)(key >> 32)));
-            }
-            __syncthreads();
-        }
+        uint32_t all = 0;
+        for (int b = 0; b < p.cluster; ++b) all += min(s.count[which][b], (uint32_t)FS_LIST + 1);
         return all;
     };
+    // where the values of a bin lie, with room for the rounding of both ways to say it; -inf is in none
+    auto bin_low = [&](int b) { return b == FS_BINS - 1 ? -FLT_MAX : fmaxf(-FLT_MAX, mx - ((float)b + 1.02f) / per - fabsf(mx) * 0x1p-21f); };
+    auto bin_high = [&](int b) { return b == 0 ? INFINITY : mx - ((float)b - 0.02f) / per + fabsf(mx) * 0x1p-21f; };
     // The smallest key c with measure(keys above c) below `most`: what is kept is c and all above it.  A pass over the row per bit.
     auto bisect = [&](auto&& measure, double most) -> uint64_t {
-        uint64_t lo = (uint64_t)ordered_bits(mn) << 32, hi = r.first;  // holds at hi: nothing is above it
+        uint64_t lo = (uint64_t)ordered_bits(mn) << 32, hi = order_key(mx, 0);  // holds at hi: nothing is above it
         int turn = 0;
         while (lo < hi) {
             const uint64_t mid = lo + (hi - lo) / 2;
@@ -357,10 +359,10 @@ __global__ void __launch_bounds__(FS_THREADS) filtered_sample_kernel(const __gri
                 if (fs_x[i] > -INFINITY && key > mid) v += measure(fs_x[i], key);
             }
             v = block_total(v, s);
-            if (tid == 0) s.total[turn] = v;
+            if (tid < p.cluster) cluster.map_shared_rank(&s, tid)->total[turn][rank] = v;
             cluster.sync();
             uint64_t all = 0;
-            for (int b = 0; b < p.cluster; ++b) all += cluster.map_shared_rank(&s, b)->total[turn];
+            for (int b = 0; b < p.cluster; ++b) all += s.total[turn][b];
             turn ^= 1;  // (the other slot: a block may be a step ahead)
             if ((double)all < most) hi = mid;
             else lo = mid + 1;
@@ -369,19 +371,23 @@ __global__ void __launch_bounds__(FS_THREADS) filtered_sample_kernel(const __gri
         return lo;
     };
     // The bin at which the running measure (counts, or masses) reaches `most`, and the measure before it and with it; the last bin, which is not measured, has the rest.
-    auto reach = [&](double most) {
+    auto reach = [&](double most, bool masses) {
         uint64_t c[FS_BINS / FS_THREADS], sum = 0;
 #pragma unroll
-        for (int e = 0; e < FS_BINS / FS_THREADS; ++e) {
-            c[e] = 0;
-            const int bin = tid * (FS_BINS / FS_THREADS) + e;
-            for (int b = 0; b < p.cluster; ++b) {
-                const SampleShared* o = cluster.map_shared_rank(&s, b);
-                c[e] += (uint64_t)o->high[bin] << 32;
-                c[e] += o->low[bin];
+        for (int e = 0; e < FS_BINS / FS_THREADS; ++e) c[e] = 0;
+#pragma unroll 4
+        for (int b = 0; b < p.cluster; ++b) {
+            const SampleShared* o = cluster.map_shared_rank(&s, b);
+            const uint2 low = *reinterpret_cast<const uint2*>(&o->low[2 * tid]);
+            c[0] += low.x;
+            c[1] += low.y;
+            if (masses) {
+                const uint2 high = *reinterpret_cast<const uint2*>(&o->high[2 * tid]);
+                c[0] += (uint64_t)high.x << 32;
+                c[1] += (uint64_t)high.y << 32;
             }
-            sum += c[e];
         }
+        sum = c[0] + c[1];
         uint64_t before = block_before(sum, s);
         if (tid == FS_THREADS - 1) {
             s.bin = FS_BINS - 1;
@@ -400,70 +406,67 @@ __global__ void __launch_bounds__(FS_THREADS) filtered_sample_kernel(const __gri
         }
         __syncthreads();
     };
+    static_assert(FS_BINS == 2 * FS_THREADS && FS_FAST <= FS_THREADS, "two bins, or one kept value, to a thread");
 
-    if (has_k) {
+    if (k > 0 && k < p.vocab) {
         uint32_t m = FS_LIST + 1;
-        if (fast) m = gather(false, [&](float x, uint32_t) { return x >= tau; });
+        if (fast) m = gather(0, false, fmaxf(tau, -FLT_MAX), INFINITY, [](float, uint64_t) { return true; });
         if (m <= FS_LIST) {
             // everything that is kept is among these
-            if (rank == 0) {
-                constexpr int E = FS_LIST / FS_THREADS;
-                uint64_t above[E] = {}, key[E] = {}, w[E] = {}, mass_k = 0;
-                uint32_t place[E] = {};
-                bool mine[E] = {};  // (one of the threads that share a key)
-                for_each_above(s, (int)m, [&](int e, int i, uint64_t ke, uint32_t pl, uint64_t ab, bool one) {
-                    mine[e] = one && i < (int)m;
-                    key[e] = ke;
-                    place[e] = pl;
-                    above[e] = ab;
-                    w[e] = mine[e] && pl < (uint32_t)k ? s.w[i] : 0;
-                    mass_k += w[e];
-                });
-                const double most = (double)top_p * (double)block_total(mass_k, s);
-                uint64_t whole = 0;
-#pragma unroll
-                for (int e = 0; e < E; ++e) {
-                    const bool keep = mine[e] && place[e] < (uint32_t)k && (!has_p || (double)above[e] < most || key[e] == r.first);
-                    w[e] = keep ? r.kept_mass(from_ordered((uint32_t)(key[e] >> 32)), key[e]) : 0;
-                    whole += w[e];
-                }
-                whole = block_total(whole, s);  // (its barriers: everyone has read s.all and s.w)
-                // the kept ones again, ordered by index: keys with the index in front
-#pragma unroll
-                for (int e = 0; e < E; ++e)
-                    if (mine[e]) {
-                        s.all[place[e]] = w[e] ? (key[e] & 0xffffffffu) : 0;  // (higher for a lower index)
-                        s.w[place[e]] = w[e];
-                    }
-                __syncthreads();
-                const uint64_t most_u = border(whole);
-                for_each_above(s, (int)m, [&](int e, int i, uint64_t ke, uint32_t, uint64_t ab, bool one) {
-                    if (one && i < (int)m && ke && ab <= most_u && most_u < ab + s.w[i]) {  // (of one key only)
-                        p.tokens[row] = (int)(0xffffffffu - (uint32_t)ke);
-                        if (p.probs) p.probs[row] = (float)((double)s.w[i] / (double)whole);
-                    }
-                });
-            }
-            cluster.sync();
-            return;
-        }
-        for (int i = tid; i < n; i += FS_THREADS) {
-            const int b = fs_x[i] > -INFINITY ? bin_of(fs_x[i]) : FS_BINS - 1;
-            if (b < FS_BINS - 1) atomicAdd(&s.low[b], 1u);
-        }
-        cluster.sync();
-        reach((double)k);
-        const int bk = s.bin;
-        const uint32_t ahead = (uint32_t)s.before, upto = s.found != ~0ull ? (uint32_t)s.found : usable;
-        if (upto - ahead <= FS_LIST) {
-            m = gather(true, [&](float x, uint32_t) { return bin_of(x) == bk; });
-            for_each_above(s, (int)m, [&](int, int i, uint64_t key, uint32_t place, uint64_t, bool one) {
-                if (one && i < (int)m && ahead + place == (uint32_t)k - 1) s.found = key;
+            if (rank != 0) return;
+            const int most_k = min(k, (int)m);
+            places(s.all, (int)m, [&](int i, uint32_t at) {
+                if (at < (uint32_t)most_k) s.sorted[at] = s.all[i];
             });
             __syncthreads();
-            cut = s.found;
-        } else {
-            cut = bisect([](float, uint64_t) { return (uint64_t)1; }, (double)k);
+            // a kept value to a thread, in order
+            const uint64_t key = tid < most_k ? s.sorted[tid] : 0;
+            uint64_t w = tid < most_k ? r.mass(from_ordered((uint32_t)(key >> 32))) : 0;
+            if (has_p) {
+                const uint64_t above = block_before(w, s);
+                const double most = (double)top_p * (double)block_total(w, s);
+                if (!((double)above < most) && tid > 0) w = 0;
+            }
+            if (w) w = r.kept_mass(from_ordered((uint32_t)(key >> 32)));
+            if (tid < most_k) {
+                s.all[tid] = key & 0xffffffffu;  // by index: the lower, the higher
+                s.w[tid] = w;
+            }
+            const uint64_t whole = block_total(w, s), most_u = border(whole);  // (with barriers)
+            masses_above(s.all, s.w, most_k, [&](int i, uint64_t above) {
+                if (above <= most_u && most_u < above + s.w[i]) {  // (of one value only)
+                    p.tokens[row] = (int)(0xffffffffu - (uint32_t)s.all[i]);
+                    if (p.probs) p.probs[row] = (float)((double)s.w[i] / (double)whole);
+                }
+            });
+            return;
+        }
+        uint32_t usable = 0;
+        for (int i = tid; i < n; i += FS_THREADS) {
+            const float x = fs_x[i];
+            const int b = x > -INFINITY ? bin_of(x) : FS_BINS - 1;
+            usable += x > -INFINITY;
+            if (b < FS_BINS - 1) atomicAdd(&s.low[b], 1u);
+        }
+        usable = (uint32_t)block_total(usable, s);
+        if (tid < p.cluster) cluster.map_shared_rank(&s, tid)->total[2][rank] = usable;
+        cluster.sync();
+        usable = 0;
+        for (int b = 0; b < p.cluster; ++b) usable += (uint32_t)s.total[2][b];
+        if ((uint32_t)k < usable) {
+            reach((double)k, false);
+            const int bk = s.bin;
+            const uint32_t ahead = (uint32_t)s.before, upto = s.found != ~0ull ? (uint32_t)s.found : usable;
+            if (upto - ahead <= FS_LIST) {
+                m = gather(1, true, bin_low(bk), bin_high(bk), [&](float x, uint64_t) { return bin_of(x) == bk; });
+                places(s.all, (int)m, [&](int i, uint32_t at) {
+                    if (ahead + at == (uint32_t)k - 1) s.found = s.all[i];
+                });
+                __syncthreads();
+                cut = s.found;
+            } else {
+                cut = bisect([](float, uint64_t) { return (uint64_t)1; }, (double)k);
+            }
         }
         if (has_p) {
             cluster.sync();  // (all have read the counts)
@@ -476,7 +479,7 @@ __global__ void __launch_bounds__(FS_THREADS) filtered_sample_kernel(const __gri
         uint64_t sum = 0;
         for (int i = tid; i < n; i += FS_THREADS) {
             const float x = fs_x[i];
-            if (x > -INFINITY && order_key(x, (uint32_t)(first + i)) >= cut) {
+            if (x > -INFINITY && (cut == 0 || order_key(x, (uint32_t)(first + i)) >= cut)) {
                 const uint64_t w = r.mass(x);
                 const int b = bin_of(x);
                 sum += w;
@@ -484,20 +487,21 @@ __global__ void __launch_bounds__(FS_THREADS) filtered_sample_kernel(const __gri
             }
         }
         sum = block_total(sum, s);
-        if (tid == 0) s.total[0] = sum;
+        if (tid < p.cluster) cluster.map_shared_rank(&s, tid)->total[2][rank] = sum;
         cluster.sync();
         uint64_t whole = 0;
-        for (int b = 0; b < p.cluster; ++b) whole += cluster.map_shared_rank(&s, b)->total[0];
+        for (int b = 0; b < p.cluster; ++b) whole += s.total[2][b];
         const double most = (double)top_p * (double)whole;
-        reach(most);
+        reach(most, true);
         const int bp = s.bin;
         const uint64_t ahead = s.before;
-        const uint32_t m = gather(true, [&](float x, uint32_t index) { return bin_of(x) == bp && order_key(x, index) >= cut; });
+        const uint32_t m = gather(2, true, bin_low(bp), bin_high(bp), [&](float x, uint64_t key) { return bin_of(x) == bp && key >= cut; });
         if (m <= FS_LIST) {
-            if (tid == 0) s.found = r.first;  // (the first is always kept)
+            for (uint32_t i = tid; i < m; i += FS_THREADS) s.w[i] = r.mass(from_ordered((uint32_t)(s.all[i] >> 32)));
+            if (tid == 0) s.found = order_key(mx, 0);
             __syncthreads();
-            for_each_above(s, (int)m, [&](int, int i, uint64_t key, uint32_t, uint64_t above, bool one) {
-                if (one && i < (int)m && (double)(ahead + above) < most) atomicMin((unsigned long long*)&s.found, (unsigned long long)key);
+            masses_above(s.all, s.w, (int)m, [&](int i, uint64_t above) {  // (the first of a row has nothing before it, and it is less than most)
+                if ((double)(ahead + above) < most) atomicMin((unsigned long long*)&s.found, (unsigned long long)s.all[i]);
             });
             __syncthreads();
             cut = max(cut, s.found);
@@ -508,30 +512,51 @@ __global__ void __launch_bounds__(FS_THREADS) filtered_sample_kernel(const __gri
     }
 
     // the choice among all that is kept: masses per warp's stretch of the slice, then inside the stretch that holds it
-    if (min_p > 0.f) r.floor_t = fmin(r.floor_t, fmax(0.0, 1e-6 - log2((double)min_p)));  // (a little beyond min_p: the comparison is made on the weight)
-    const int stretch = (p.slice + FS_WARPS - 1) / FS_WARPS;
+    if (r.min_p > 0.0) r.floor_t = fmin(r.floor_t, fmax(1e-6, 1e-6 - log2(r.min_p)));  // (a little beyond min_p: the comparison is made on the weight)
+    const int stretch = ((p.slice + FS_WARPS - 1) / FS_WARPS + 31) / 32 * 32;
+    // no smaller value is kept: the cut's, or the one from which on weights vanish (or are below min_p), with room for rounding
+    const float low = fmaxf(fmaxf(from_ordered((uint32_t)(cut >> 32) | (cut ? 0u : 0x00800000u)), -FLT_MAX), mx - (float)(r.floor_t / r.rate) * 1.0001f - fabsf(mx) * 0x1p-21f);
     auto kept = [&](int i) -> uint64_t {
         const float x = fs_x[i];
-        if (!(x > -INFINITY)) return 0;
-        const uint64_t key = order_key(x, (uint32_t)(first + i));
-        return key >= cut ? r.kept_mass(x, key) : 0;
+        return x >= low && order_key(x, (uint32_t)(first + i)) >= cut ? r.kept_mass(x) : 0;
     };
     const int lo = min(n, warp * stretch), hi = min(n, lo + stretch);
     uint64_t sum = 0;
-    for (int i = lo + lane; i < hi; i += 32) sum += kept(i);
+    int queued = 0;
+    for (int i0 = lo; i0 < hi; i0 += 32) {
+        const int i = i0 + lane;
+        const float x = i < hi ? fs_x[i] : -INFINITY;
+        const bool in = x >= low && (x > low || order_key(x, (uint32_t)(first + i)) >= cut);
+        const unsigned v = __ballot_sync(0xffffffffu, in);
+        if (v == ~0u) {
+            sum += r.kept_mass(x);
+        } else if (v) {
+            if (in) s.queue[warp][queued + __popc(v & ((1u << lane) - 1u))] = x;
+            queued += __popc(v);
+            __syncwarp();
+            if (queued >= 32) {
+                sum += r.kept_mass(s.queue[warp][lane]);
+                queued -= 32;
+                const float over = lane < queued ? s.queue[warp][32 + lane] : 0.f;
+                __syncwarp();
+                if (lane < queued) s.queue[warp][lane] = over;
+                __syncwarp();
+            }
+        }
+    }
+    if (lane < queued) sum += r.kept_mass(s.queue[warp][lane]);
     sum = warp_sum64(sum);
     __syncthreads();
     if (lane == 0) s.sums[warp] = sum;
     __syncthreads();
     sum = 0;
     for (int w = 0; w < FS_WARPS; ++w) sum += s.sums[w];
-    if (tid == 0) s.total[1] = sum;
+    if (tid < p.cluster) cluster.map_shared_rank(&s, tid)->total[1][rank] = sum;
     cluster.sync();
     uint64_t whole = 0, ahead = 0;
     for (int b = 0; b < p.cluster; ++b) {
-        const uint64_t t = cluster.map_shared_rank(&s, b)->total[1];
-        whole += t;
-        ahead += b < rank ? t : 0;
+        whole += s.total[1][b];
+        ahead += b < rank ? s.total[1][b] : 0;
     }
     const uint64_t most_u = border(whole);
     if (ahead <= most_u && most_u < ahead + sum) {  // here (one block of the cluster, and all of its threads)
@@ -554,7 +579,6 @@ __global__ void __launch_bounds__(FS_THREADS) filtered_sample_kernel(const __gri
             }
         }
     }
-    cluster.sync();
 }
 
 }  // namespace l2b
