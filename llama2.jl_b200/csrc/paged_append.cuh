@@ -3,19 +3,23 @@
 // rotation of the pairs (a, b) = (y_2i, y_2i+1) or (y_i, y_i+size/2) by t = position * base^(-2i / size),
 //   (a, b) -> (a cos t - b sin t, a sin t + b cos t),
 // queries to the caller's buffer, keys and values into their pages, rounded once.  Everything is read once and written once, so memory bounds it.
-// A group of LANES threads holds one head: each thread one unit of U values, as two pieces that are each other's partners when the pairs lie half a
-// head apart.  So the norm is a few shuffles, the gains stay in registers, and all accesses are of 16 bytes (heads of 8, 24, 40 .. values: 8 bytes
-// for 16-bit types).  The angles of a token are shared by its heads: a block computes them once for its tokens, in 64 bits up to the fraction of a
+// A group of threads holds one head: each thread two pieces of P values, half a head apart, so that pairs that lie half a head apart are one thread's and
+// so are adjacent ones, and the norm is a few shuffles.  A warp works on the heads of one token.  Gains, cosines and sines of a thread's values are the
+// same for all of them and become four coefficients per pair once (a' = r (A a - B b), b' = r (C a + D b), r = 1 / sqrt(..)), in registers: norm and rotation
+// cost three operations a value.  (With gains and angles applied one after the other, and a kind looked up for each head, the instructions took twice the
+// memory's time.)  The angles of a token are shared by its heads: a block computes them once for its tokens, in 64 bits up to the fraction of a
 // turn (a far position times the fastest frequency would lose all of a turn in 32), and the first heads' values are on their way meanwhile.
 #pragma once
 #include <cuda_bf16.h>
+
+#include <type_traits>
 
 #include "common.cuh"
 #include "paged.h"
 
 namespace l2b {
 
-constexpr int PA_THREADS = 256, PA_MAX_SIZE = 128, PA_MAX_TOKENS = 8;
+constexpr int PA_THREADS = 256, PA_MAX_SIZE = 128, PA_MAX_TOKENS = 8, PA_WARPS = PA_THREADS / 32;
 
 struct AppendParams {
     PagedPool pool;
@@ -24,8 +28,8 @@ struct AppendParams {
     void* q_out;
     int64_t q_stride, k_stride, v_stride, q_out_stride;
     const float *q_gain, *k_gain;  // null: no norm
-    float eps;
-    int n_heads, rotate, neox, tokens;  // tokens of a block
+    float eps, inv_size;
+    int n_heads, rotate, tokens;  // tokens of a block
     double turns[PA_MAX_SIZE / 2];      // turns per position
 };
 
@@ -52,6 +56,17 @@ __device__ __forceinline__ void get(const T* p, float (&x)[N]) {
 #pragma unroll
     for (int i = 0; i < N; ++i) x[i] = to_f32(a.v[i]);
 }
+// N values as they were loaded, in words.
+template <typename T, int N>
+struct alignas(sizeof(T) * N < 16 ? sizeof(T) * N : 16) Words {
+    uint32_t w[sizeof(T) * N / 4];
+    __device__ __forceinline__ float value(int i) const {
+        if (sizeof(T) == 4) return __uint_as_float(w[i]);
+        const uint32_t p = w[i / 2];
+        if (std::is_same<T, __half>::value) return half_bits_to_float(i & 1 ? p >> 16 : p & 0xffffu);
+        return __uint_as_float(i & 1 ? p & 0xffff0000u : p << 16);
+    }
+};
 template <typename T, int N>
 __device__ __forceinline__ void put(T* p, const float (&x)[N]) {
     Pack<T, N> a;
@@ -60,20 +75,21 @@ __device__ __forceinline__ void put(T* p, const float (&x)[N]) {
     *reinterpret_cast<Pack<T, N>*>(p) = a;
 }
 
-// TI: type of the rows, TC: of the cache, U: values of a thread (16, or 8 for heads that are no multiple of 16)
-template <typename TI, typename TC, int U>
-__global__ void __launch_bounds__(PA_THREADS) paged_append_kernel(const __grid_constant__ AppendParams p) {
-    constexpr int P = U / 2;  // values of a piece
-    __shared__ float2 s_cs[PA_MAX_TOKENS][PA_MAX_SIZE / 2];
+// TI: type of the rows, TC: of the cache, P: values of a piece (8, or 4 for heads that are no multiple of 16),
+// NEOX: pairs half a head apart
+template <typename TI, typename TC, int P, bool NEOX>
+__global__ void __launch_bounds__(PA_THREADS, 3) paged_append_kernel(const __grid_constant__ AppendParams p) {
+    constexpr int AHEAD = 32 / (P * (int)sizeof(TI));  // groups of heads under way
+    __shared__ __align__(16) float2 s_cs[PA_MAX_TOKENS][PA_MAX_SIZE / 2];
     __shared__ int s_page[PA_MAX_TOKENS], s_slot[PA_MAX_TOKENS], s_new[PA_MAX_TOKENS];
-    const int hs = p.pool.hs, half = hs / 2, units = hs / U, tid = threadIdx.x;
+    const int hs = p.pool.hs, half = hs / 2, units = hs / (2 * P), tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
     int lanes = 1;
     while (lanes < units) lanes *= 2;
-    const int unit = tid % lanes, heads_at_once = PA_THREADS / lanes;
+    const int unit = lane % lanes, at_once = 32 / lanes;  // heads of a warp at once
     const bool active = unit < units;
     // where this thread's two pieces lie in a head
-    const int d0 = p.neox ? unit * P : unit * U, d1 = p.neox ? half + unit * P : d0 + P;
-    const int nq = p.q ? p.n_heads : 0, slots = nq + 2 * p.pool.n_kv;
+    const int d0 = unit * P, d1 = half + d0;
+    const int nq = p.q ? p.n_heads : 0, q_groups = (nq + at_once - 1) / at_once, kv_groups = (p.pool.n_kv + at_once - 1) / at_once;
     const int64_t rows = (int64_t)p.seqs.n_seq * p.seqs.n_query, row0 = (int64_t)blockIdx.x * p.tokens;
     const int here = (int)(rows - row0 < p.tokens ? rows - row0 : p.tokens);
     pdl_wait();
@@ -102,74 +118,88 @@ __global__ void __launch_bounds__(PA_THREADS) paged_append_kernel(const __grid_c
             s_cs[t][f] = make_float2(c, s);
         }
     }
-    float gq[2][P], gk[2][P];
-#pragma unroll
-    for (int i = 0; i < P; ++i) gq[0][i] = gq[1][i] = gk[0][i] = gk[1][i] = 1.f;
-    if (active && p.q_gain) get(p.q_gain + d0, gq[0]), get(p.q_gain + d1, gq[1]);
-    if (active && p.k_gain) get(p.k_gain + d0, gk[0]), get(p.k_gain + d1, gk[1]);
     __syncthreads();
 
-    const int total = here * slots;
-    for (int base = (int)blockIdx.y * heads_at_once; base < total; base += (int)gridDim.y * heads_at_once) {  // (the same for all threads of a warp)
-        const int it = base + tid / lanes;
-        const bool mine = it < total;
-        const int t = mine ? it / slots : 0, h = it - t * slots;
-        const int64_t row = row0 + t;
-        const bool is_q = h < nq, is_v = h >= nq + p.pool.n_kv, go = mine && active && s_new[t] && (is_q || s_page[t] >= 0);
-        float x[2][P];
-        if (go) {
-            const TI* src = is_q ? (const TI*)p.q + row * p.q_stride + (int64_t)h * hs
-                                 : is_v ? (const TI*)p.v + row * p.v_stride + (int64_t)(h - nq - p.pool.n_kv) * hs : (const TI*)p.k + row * p.k_stride + (int64_t)(h - nq) * hs;
-            get(src + d0, x[0]);
-            get(src + d1, x[1]);
-        }
-        const bool norm = is_q ? p.q_gain != nullptr : !is_v && p.k_gain != nullptr;
-        if (p.q_gain || p.k_gain) {
-            float ss = 0.f;
-            if (go && norm) {
+    const int per_token = PA_WARPS / p.tokens, t = warp / per_token;  // warps of a token; this warp's
+    if (t >= here || !s_new[t]) return;
+    const int64_t row = row0 + t;
+    const int page = s_page[t], stride = (int)gridDim.y * per_token, start = (int)blockIdx.y * per_token + warp % per_token, sub = lane / lanes;
+    // Groups of heads kind by kind, one to each warp of the token in turn.  `of`: groups of the kinds before.
+    auto heads = [&](auto kind, int n_heads, int n_groups, int of, const TI* src, auto* dst, int64_t dst_head, const float* gains) {
+        constexpr bool VALUES = decltype(kind)::value;
+        using TO = typename std::remove_pointer<decltype(dst)>::type;
+        int g = start - of % stride;
+        if (g < 0) g += stride;
+        if (g >= n_groups) return;
+        float ca[P], cb[P], cc[P], cd[P];  // of pairs (d0 + i, d1 + i), or of the adjacent ones of either piece
+        if constexpr (!VALUES) {
 #pragma unroll
-                for (int i = 0; i < P; ++i) ss = fmaf(x[0][i], x[0][i], fmaf(x[1][i], x[1][i], ss));
+            for (int i = 0; i < P; ++i) {
+                const int da = NEOX ? d0 + i : (i < P / 2 ? d0 + 2 * i : d1 + 2 * i - P), db = NEOX ? d1 + i : da + 1;
+                float2 cs = make_float2(1.f, 0.f);
+                float ga = 1.f, gb = 1.f;
+                if (active && p.rotate) cs = s_cs[t][NEOX ? da : da / 2];
+                if (active && gains) {
+                    ga = gains[da];
+                    gb = gains[db];
+                }
+                ca[i] = ga * cs.x;
+                cb[i] = gb * cs.y;
+                cc[i] = ga * cs.y;
+                cd[i] = gb * cs.x;
             }
-            for (int o = lanes / 2; o > 0; o >>= 1) ss += __shfl_xor_sync(0xffffffffu, ss, o);
-            if (norm) {
-                const float r = rsqrtf(ss / (float)hs + p.eps);
+        }
+        for (; g < n_groups; g += AHEAD * stride) {
+            Words<TI, P> raw[AHEAD][2];
+#pragma unroll
+            for (int n = 0; n < AHEAD; ++n) {
+                const int h = (g + n * stride) * at_once + sub;
+                if (active && h < n_heads) {
+                    const TI* const from = src + (int64_t)h * hs;
+                    raw[n][0] = *reinterpret_cast<const Words<TI, P>*>(from + d0);
+                    raw[n][1] = *reinterpret_cast<const Words<TI, P>*>(from + d1);
+                }
+            }
+#pragma unroll
+            for (int n = 0; n < AHEAD; ++n) {
+                const int h = (g + n * stride) * at_once + sub;
+                const bool go = active && h < n_heads;
+                float x[2][P], r = 1.f;
 #pragma unroll
                 for (int i = 0; i < P; ++i) {
-                    x[0][i] *= r * (is_q ? gq[0][i] : gk[0][i]);
-                    x[1][i] *= r * (is_q ? gq[1][i] : gk[1][i]);
+                    x[0][i] = go ? raw[n][0].value(i) : 0.f;
+                    x[1][i] = go ? raw[n][1].value(i) : 0.f;
+                }
+                if constexpr (!VALUES) {
+                    if (gains) {
+                        float ss = 0.f;
+#pragma unroll
+                        for (int i = 0; i < P; ++i) ss = fmaf(x[0][i], x[0][i], fmaf(x[1][i], x[1][i], ss));
+                        for (int o = lanes / 2; o > 0; o >>= 1) ss += __shfl_xor_sync(0xffffffffu, ss, o);
+                        r = rsqrtf(fmaf(ss, p.inv_size, p.eps));
+                    }
+#pragma unroll
+                    for (int i = 0; i < P; ++i) {
+                        float& xa = NEOX ? x[0][i] : x[2 * i / P][2 * i % P];
+                        float& xb = NEOX ? x[1][i] : x[2 * i / P][2 * i % P + 1];
+                        const float a = xa * r, b = xb * r;
+                        xa = a * ca[i] - b * cb[i];
+                        xb = a * cc[i] + b * cd[i];
+                    }
+                }
+                if (go) {
+                    TO* const to = dst + h * dst_head;
+                    put(to + d0, x[0]);
+                    put(to + d1, x[1]);
                 }
             }
         }
-        if (!go) continue;
-        if (p.rotate && !is_v) {
-            if (p.neox) {
-#pragma unroll
-                for (int i = 0; i < P; ++i) {
-                    const float2 cs = s_cs[t][d0 + i];
-                    const float a = x[0][i], b = x[1][i];
-                    x[0][i] = a * cs.x - b * cs.y;
-                    x[1][i] = a * cs.y + b * cs.x;
-                }
-            } else {
-#pragma unroll
-                for (int i = 0; i < U; i += 2) {
-                    const float2 cs = s_cs[t][(d0 + i) / 2];
-                    float &ra = i < P ? x[0][i % P] : x[1][i % P], &rb = i < P ? x[0][i % P + 1] : x[1][i % P + 1];
-                    const float a = ra, b = rb;
-                    ra = a * cs.x - b * cs.y;
-                    rb = a * cs.y + b * cs.x;
-                }
-            }
-        }
-        if (is_q) {
-            TI* dst = (TI*)p.q_out + row * p.q_out_stride + (int64_t)h * hs;
-            put(dst + d0, x[0]);
-            put(dst + d1, x[1]);
-        } else {
-            TC* dst = (TC*)(is_v ? p.pool.v : p.pool.k) + paged_offset(s_page[t], is_v ? h - nq - p.pool.n_kv : h - nq, s_slot[t], p.pool);
-            put(dst + d0, x[0]);
-            put(dst + d1, x[1]);
-        }
+    };
+    if (nq) heads(std::false_type(), nq, q_groups, 0, (const TI*)p.q + row * p.q_stride, (TI*)p.q_out + row * p.q_out_stride, hs, p.q_gain);
+    if (page >= 0) {
+        const int64_t at = paged_offset(page, 0, s_slot[t], p.pool), head = (int64_t)hs << p.pool.page_shift;
+        heads(std::false_type(), p.pool.n_kv, kv_groups, q_groups, (const TI*)p.k + row * p.k_stride, (TC*)p.pool.k + at, head, p.k_gain);
+        heads(std::true_type(), p.pool.n_kv, kv_groups, q_groups + kv_groups, (const TI*)p.v + row * p.v_stride, (TC*)p.pool.v + at, head, nullptr);
     }
 }
 

@@ -213,8 +213,8 @@ extern "C" int32_t l2b_paged_append_device(const l2b_paged_cache* cache, const l
     if (!(rows->rope_freq_base >= 0.f) || std::isinf(rows->rope_freq_base)) return fail(L2B_ERR_BAD_ARG, "rope_freq_base must be positive, or 0 for no rotation");
     p.q = rows->dev_q; p.k = rows->dev_k; p.v = rows->dev_v; p.q_out = rows->dev_q_out;
     p.q_stride = rows->q_stride; p.k_stride = rows->k_stride; p.v_stride = rows->v_stride; p.q_out_stride = rows->q_out_stride;
-    p.q_gain = rows->dev_q_gain; p.k_gain = rows->dev_k_gain; p.eps = rows->eps;
-    p.n_heads = rows->n_heads; p.neox = rows->rope_is_neox != 0; p.rotate = rows->rope_freq_base > 0.f;
+    p.q_gain = rows->dev_q_gain; p.k_gain = rows->dev_k_gain; p.eps = rows->eps; p.inv_size = 1.f / (float)hs;
+    p.n_heads = rows->n_heads; p.rotate = rows->rope_freq_base > 0.f;
     if (p.rotate) {
         const long double step = powl((long double)rows->rope_freq_base, -2.0L / hs);
         long double f = 0.15915494309189533576888376337251436L;  // turns per radian
@@ -224,24 +224,31 @@ extern "C" int32_t l2b_paged_append_device(const l2b_paged_cache* cache, const l
     L2B_TRY(on.enter(cache->dev_k, "dev_k"));
     const int64_t n = (int64_t)p.seqs.n_seq * p.seqs.n_query;
     if (n == 0) return L2B_OK;
-    // Tokens of a block: their angles are worked out together, 256 at a time, so several tokens once there are blocks for every SM twice over;
-    // before that one token, and its heads over several blocks while that leaves SMs idle.
+    // Tokens of a block: their angles are worked out together, so as many tokens as the block has warps once there are blocks enough for every SM three
+    // times over; before that fewer, and their heads over several warps, at last over several blocks.
     int sms = 0;
     L2B_TRY(sm_count(on.device, &sms));
-    p.tokens = n >= (int64_t)16 * sms ? 8 : n >= (int64_t)8 * sms ? 4 : 1;
-    const int unit = hs % 16 ? 8 : 16, units = hs / unit;
+    p.tokens = PA_WARPS;
+    while (p.tokens > 1 && n < (int64_t)3 * sms * p.tokens) p.tokens /= 2;
+    const int piece = hs % 16 ? 4 : 8;
     int lanes = 1;
-    while (lanes < units) lanes *= 2;
-    const int64_t slots = ((p.q ? p.n_heads : 0) + 2 * p.pool.n_kv) * p.tokens, passes = (slots + PA_THREADS / lanes - 1) / (PA_THREADS / lanes), blocks = (n + p.tokens - 1) / p.tokens;
-    int64_t y = 1;
-    while (y < passes && y < 64 && blocks * y < 2 * sms) ++y;
+    while (lanes < hs / (2 * piece)) lanes *= 2;
+    const int at_once = 32 / lanes, groups = ((p.q ? p.n_heads : 0) + at_once - 1) / at_once + 2 * ((p.pool.n_kv + at_once - 1) / at_once);
+    const int64_t blocks = (n + p.tokens - 1) / p.tokens;
+    int y = 1;
+    while (y * (PA_WARPS / p.tokens) < groups && y < 64 && blocks * y < 2 * sms) ++y;
     const dim3 grid((unsigned)blocks, (unsigned)y);
     return by_types(cache->type, rows->type, [&](auto t, auto io) -> int32_t {
         using T = decltype(t);
         using TIO = decltype(io);
         cudaStream_t st = (cudaStream_t)stream;
-        if (unit == 16) CU(launch_kernel(paged_append_kernel<TIO, T, 16>, grid, dim3(PA_THREADS), 0, st, true, p));
-        else CU(launch_kernel(paged_append_kernel<TIO, T, 8>, grid, dim3(PA_THREADS), 0, st, true, p));
+        auto go = [&](auto kernel) -> int32_t {
+            CU(launch_kernel(kernel, grid, dim3(PA_THREADS), 0, st, true, p));
+            return L2B_OK;
+        };
+        const bool neox = rows->rope_is_neox != 0;
+        if (piece == 8) L2B_TRY(neox ? go(paged_append_kernel<TIO, T, 8, true>) : go(paged_append_kernel<TIO, T, 8, false>));
+        else L2B_TRY(neox ? go(paged_append_kernel<TIO, T, 4, true>) : go(paged_append_kernel<TIO, T, 4, false>));
         return L2B_OK;
     });
 }
