@@ -72,7 +72,7 @@ struct PrefixCut {
     int tiles, row_tiles, streams_share;
 };
 
-constexpr int PT_KEYS = 16, PT_ROWS = 16;  // a tile of the own parts' kernel
+constexpr int PT_KEYS = 16;  // of a tile of the own parts' kernel
 
 // Rows of a group are the query heads of one key/value head, of all the group's rows one after the other.  Groups: the prefix first where it is one
 // (thin_prefix), then the sequences.
@@ -81,6 +81,7 @@ struct PagedWork {
     PagedSeqs seqs;
     int group;  // query heads of a key/value head
     int thin_prefix;
+    int tile_rows;  // 8 or 16
 };
 struct GroupShape {
     int keys, tiles, row_tiles;
@@ -89,7 +90,7 @@ L2B_HD GroupShape group_shape(const PagedWork& p, int g, int length) {  // lengt
     GroupShape s;
     const bool pre = p.thin_prefix && g == 0;
     s.keys = pre ? p.seqs.prefix_len : paged_keys(length, p.seqs.width, p.pool.page_shift);
-    s.row_tiles = (int)(((int64_t)(pre ? p.seqs.n_seq : 1) * p.seqs.n_query * p.group + PT_ROWS - 1) / PT_ROWS);
+    s.row_tiles = (int)(((int64_t)(pre ? p.seqs.n_seq : 1) * p.seqs.n_query * p.group + p.tile_rows - 1) / p.tile_rows);
     s.tiles = (int)(((int64_t)s.keys + PT_KEYS - 1) / PT_KEYS);
     return s;
 }

@@ -123,7 +123,7 @@ int32_t by_types(int cache_type, int type, F&& f) {
 
 // What an attention call needs of its workspace, all in floats, and how it is cut.
 struct AttnPlan {
-    int blocks, smem, thin_prefix, slot_rows;
+    int blocks, smem, thin_prefix, tile_rows, slot_rows;
     PrefixCut cut;              // the prefix's own kernel, a block per SM
     int cut_blocks, stages, cut_smem;
     int64_t starts, slots, whole, cut_slots, pre, total;  // floats of the slots, of whole items, of the prefix's slots and whole items, of everything
@@ -136,12 +136,14 @@ AttnPlan attention_plan(const PagedPool& pool, const PagedSeqs& s, const l2b_pag
     memset(&a, 0, sizeof(a));
     const int ks = (pool.hs + 31) / 32 * 2, n_heads = q.n_heads, group = n_heads / pool.n_kv;
     const int64_t n_tok = (int64_t)s.n_seq * s.n_query, rows = n_tok * group;
-    const bool tiled = s.prefix_len > 0 && rows > PT_ROWS && q.scale >= 0.f && (int64_t)pool.n_pages * pool.n_kv < 0x7fffffff;
+    const bool tiled = s.prefix_len > 0 && rows > 16 && q.scale >= 0.f && (int64_t)pool.n_pages * pool.n_kv < 0x7fffffff;
     a.thin_prefix = s.prefix_len > 0 && !tiled;
     const int64_t most = (int64_t)s.n_query * group * (a.thin_prefix ? s.n_seq : 1);
-    a.slot_rows = (int)(most < PT_ROWS ? most : PT_ROWS);
-    a.smem = PT_WARPS * PT_STAGES * 2 * PT_KEYS * (ks * 32 + 16);
-    a.blocks = sms * 2;
+    a.tile_rows = most <= 8 ? 8 : 16;
+    a.slot_rows = (int)(most < a.tile_rows ? most : a.tile_rows);
+    const int stages = a.tile_rows == 8 ? 2 : 3;  // (ThinTraits)
+    a.smem = PT_WARPS * stages * 2 * PT_KEYS * (ks * 32 + 16);
+    a.blocks = sms * (a.tile_rows == 8 ? 3 : 2);
     const int64_t row = pool.hs + 4;  // sums, then maximum and total, on 16-byte boundaries
     a.slots = (int64_t)2 * a.blocks * PT_WARPS * a.slot_rows * row;
     a.whole = a.pre = s.prefix_len ? n_tok * n_heads * row : 0;
@@ -294,6 +296,7 @@ extern "C" int32_t l2b_paged_attention_device(const l2b_paged_cache* cache, cons
     p.cut = plan.cut;
     p.workers = plan.blocks * PT_WARPS;
     p.slot_rows = plan.slot_rows;
+    p.tile_rows = plan.tile_rows;
     p.starts = (int64_t*)dev_workspace;
     float* const w = (float*)dev_workspace + plan.starts;
     const int64_t n_rows = (int64_t)p.seqs.n_seq * p.seqs.n_query * p.n_heads;
@@ -340,18 +343,21 @@ extern "C" int32_t l2b_paged_attention_device(const l2b_paged_cache* cache, cons
                 L2B_TRY(tiled(std::integral_constant<int, 1>()));
             }
         }
-        auto go = [&](auto ks) -> int32_t {
-            constexpr int KS = decltype(ks)::value;
-            L2B_TRY((allow_smem<paged_attention_kernel<T, TIO, KS>>(on.device)));
-            CU(launch_kernel(paged_attention_kernel<T, TIO, KS>, dim3((unsigned)plan.blocks), dim3(PT_WARPS * 32), (size_t)plan.smem, st, true, p));
+        auto go = [&](auto ks, auto nt) -> int32_t {
+            constexpr int KS = decltype(ks)::value, NT = decltype(nt)::value;
+            L2B_TRY((allow_smem<paged_attention_kernel<T, TIO, KS, NT>>(on.device)));
+            CU(launch_kernel(paged_attention_kernel<T, TIO, KS, NT>, dim3((unsigned)plan.blocks), dim3(PT_WARPS * 32), (size_t)plan.smem, st, true, p));
             return L2B_OK;
         };
-        switch ((hs + 31) / 32) {
-            case 1: L2B_TRY(go(std::integral_constant<int, 2>())); break;
-            case 2: L2B_TRY(go(std::integral_constant<int, 4>())); break;
-            case 3: L2B_TRY(go(std::integral_constant<int, 6>())); break;
-            default: L2B_TRY(go(std::integral_constant<int, 8>())); break;
-        }
+        auto size = [&](auto nt) -> int32_t {
+            switch ((hs + 31) / 32) {
+                case 1: return go(std::integral_constant<int, 2>(), nt);
+                case 2: return go(std::integral_constant<int, 4>(), nt);
+                case 3: return go(std::integral_constant<int, 6>(), nt);
+                default: return go(std::integral_constant<int, 8>(), nt);
+            }
+        };
+        L2B_TRY(plan.tile_rows == 8 ? size(std::integral_constant<int, 1>()) : size(std::integral_constant<int, 2>()));
         JoinParams j;
         j.a = p;
         j.heads = n_rows >= 4096 ? 8 : n_rows >= 1024 ? 2 : 1;

@@ -94,12 +94,13 @@ SIMULATE = r"""
 using namespace l2b;
 // Walks every worker's share as the kernel does.  out: blocks that did each unit of (group, item, tile), in that order; returns the number of units, or a
 // negative number where a slot is used twice or a part is missing.
-extern "C" long long walk(const int* lengths, int n_seq, int n_query, int width, int page_shift, int prefix_len, int thin_prefix, int n_kv, int group, int blocks, int least, int* out, long long room) {
+extern "C" long long walk(const int* lengths, int n_seq, int n_query, int width, int page_shift, int prefix_len, int thin_prefix, int n_kv, int group, int blocks, int least, int tile_rows, int* out, long long room) {
     PagedWork w;
     w.pool = {nullptr, nullptr, 1, page_shift, n_kv, 64};
     w.seqs = {lengths, nullptr, nullptr, nullptr, n_seq, n_query, width, prefix_len};
     w.group = group;
     w.thin_prefix = thin_prefix;
+    w.tile_rows = tile_rows;
     const int groups = n_seq + thin_prefix;
     std::vector<long long> first(groups + 1, 0);
     for (int g = 0; g < groups; ++g) first[g + 1] = first[g] + group_units(w, group_shape(w, g));
@@ -166,9 +167,10 @@ def test_every_tile_belongs_to_one_share(sim, blocks):
         prefix = int(rng.choice([0, 1, 63, 64, 65, 1000]))
         thin = int(prefix > 0)
         out, least = np.zeros(1 << 22, np.int32), int(rng.choice([1, 2, 4]))
-        units = sim.walk(lengths.ctypes.data_as(C.c_void_p), n_seq, n_query, width, shift, prefix, thin, n_kv, group, blocks, least, out.ctypes.data_as(C.c_void_p), out.size)
+        tile = int(rng.choice([8, 16]))
+        units = sim.walk(lengths.ctypes.data_as(C.c_void_p), n_seq, n_query, width, shift, prefix, thin, n_kv, group, blocks, least, tile, out.ctypes.data_as(C.c_void_p), out.size)
         up = lambda a, b: -(-a // b)  # noqa: E731
-        want = sum(up(min(max(int(n), 0), width << shift), 16) for n in lengths) * up(n_query * group, 16) * n_kv + thin * up(prefix, 16) * up(n_seq * n_query * group, 16) * n_kv
+        want = sum(up(min(max(int(n), 0), width << shift), 16) for n in lengths) * up(n_query * group, tile) * n_kv + thin * up(prefix, 16) * up(n_seq * n_query * group, tile) * n_kv
         assert units == want
         assert (out[:units] == 1).all() and (out[units:] == 0).all()
 
