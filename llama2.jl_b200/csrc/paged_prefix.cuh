@@ -6,8 +6,10 @@
 //   TILES = 2: the streams are two row tiles that share the tiles of keys (128 each);
 //   TILES = 1: one row tile, the streams take the tiles of keys in turn and leave a partial result each: for few rows, and for f32 rows, whose three (f16: two)
 //              terms of Q take the place of a second tile (64 keys a tile).
+// A thread takes its row of scores to registers at once and hands P over in two halves, so that P V begins beside the second half's exponentials.  (Measured and not kept: two buffers of 64 keys per stream, Q K^T a step ahead; a product of 64 columns
+// takes as long as one of 128.)
 //   warps 0-3, 4-7  the streams' softmax; before it they bring the block's rows of Q into shared memory, after it the sums to the workspace
-//   warp 8          issues the products; those of a stream follow one another: P V of a tile, then Q K^T of its next, which overwrites that P
+//   warp 8          issues the products: P V of a tile, then Q K^T of the stream's next, which overwrites that P
 //   warp 9          TMA copies of keys and values straight from the pages: 8 rows or more at a time, V's rows behind the prefix's end through a map
 //                   that ends there, so that they are zeros; pages that are none lie outside the map and are zeros, too
 // Rows are rescaled only when a maximum has grown by more than 2^8.  The work, items (key/value head, row tile) of the prefix' key tiles, is cut
@@ -34,7 +36,7 @@ template <typename T, typename TIO, int TILES>
 struct PrefixTraits {
     static constexpr bool WIDE = sizeof(TIO) == 4, F16 = std::is_same<T, __half>::value;
     static constexpr int QT = !WIDE ? 1 : F16 ? 2 : 3, PT = QT;
-    static constexpr int KEYS = WIDE ? 64 : 128;
+    static constexpr int KEYS = WIDE ? 64 : 128, HALVES = KEYS / 64;
     static constexpr int SUB_Q = PX_ROWS * 128, SUB_K = KEYS * 128;  // bytes of 64 values of a tile's rows
     // bytes of Q's place: its terms, or 4 KB for each of the eight warps that take the sums out
     __host__ __device__ static constexpr int queries(int nd) { return QT * TILES * nd * SUB_Q > 8 * 4096 ? QT * TILES * nd * SUB_Q : 8 * 4096; }
@@ -44,7 +46,7 @@ struct PrefixTraits {
     }
 };
 // 64 consecutive columns of this thread's tensor-memory lane, and a store of 32
-__device__ __forceinline__ void tmem_ld64f(uint32_t taddr, float (&v)[64]) {
+__device__ __forceinline__ void tmem_load(uint32_t taddr, float (&v)[64]) {
     asm volatile(
         "tcgen05.ld.sync.aligned.32x32b.x64.b32 {"
         "%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15,%16,%17,%18,%19,%20,%21,%22,%23,%24,%25,%26,%27,%28,%29,%30,%31,"
@@ -131,7 +133,7 @@ __global__ void __launch_bounds__(PX_THREADS, 1) paged_prefix_kernel(const __gri
     using TR = PrefixTraits<T, TIO, TILES>;
     constexpr int KEYS = TR::KEYS;
     extern __shared__ __align__(1024) uint8_t px_raw[];
-    __shared__ __align__(8) uint64_t s_kfull[PX_MAX_STAGES], s_kfree[PX_MAX_STAGES], s_vfull[PX_MAX_STAGES], s_vfree[PX_MAX_STAGES], s_mask[PX_RING], s_q, s_seg, s_s[2], s_p[2];
+    __shared__ __align__(8) uint64_t s_kfull[PX_MAX_STAGES], s_kfree[PX_MAX_STAGES], s_vfull[PX_MAX_STAGES], s_vfree[PX_MAX_STAGES], s_mask[PX_RING], s_q, s_seg, s_s[2], s_p[2][2];  // s_p: of each half
     __shared__ uint32_t s_tmem, s_valid[PX_RING][4];
     __shared__ int s_exp[TILES * PX_ROWS];
     uint8_t* const smem = px_raw + ((1024u - (smem_u32(px_raw) & 1023u)) & 1023u);
@@ -151,7 +153,8 @@ __global__ void __launch_bounds__(PX_THREADS, 1) paged_prefix_kernel(const __gri
         mbar_init(&s_seg, 1);
         for (int i = 0; i < 2; ++i) {
             mbar_init(s_s + i, 1);
-            mbar_init(s_p + i, 4);
+            mbar_init(&s_p[i][0], 4);
+            mbar_init(&s_p[i][1], 4);
         }
         fence_barrier_init();
         fence_proxy_async();
@@ -160,7 +163,7 @@ __global__ void __launch_bounds__(PX_THREADS, 1) paged_prefix_kernel(const __gri
     tc_fence_before();
     __syncthreads();
     tc_fence_after();
-    const uint32_t tmem = s_tmem;
+    const uint32_t tmem = __shfl_sync(0xffffffffu, s_tmem, 0);
     pdl_wait();
     pdl_launch_dependents();  // (behind the wait: what follows reads the lengths before it waits itself)
 
@@ -170,112 +173,157 @@ __global__ void __launch_bounds__(PX_THREADS, 1) paged_prefix_kernel(const __gri
         bool ok = true;
         const int shift = min(p.pool.page_shift, KEYS == 128 ? 7 : 6), chunks = KEYS >> shift;  // a chunk: the map's box
         const int outside = p.pool.n_pages * p.pool.n_kv, last_page = (p.seqs.prefix_len - 1) >> p.pool.page_shift;
-        int g = 0;  // tiles so far
-        for (int64_t u = begin; u < end && ok; ++u, ++g) {
-            const int item = (int)(u / p.cut.tiles), tile = (int)(u - (int64_t)item * p.cut.tiles), kv = item / p.cut.row_tiles;
+        // Keys run a tile ahead of the values: the products of a tile's scores come before those of the tile before with its values, and with two stages a
+        // tile of values that waits for its place must not hold up the keys behind it.
+        const int n = (int)(end - begin);
+        int z_before = 0, y_before = 0;
+        bool end_before = false;
+        for (int g = 0; g <= n && ok; ++g) {
             const int stage = g % p.stages, use = g / p.stages;
-            // which keys are there: four to a lane (of one page)
-            const int key = tile * KEYS + lane * 4;
-            uint32_t nibble = 0;
-            if (lane * 4 < KEYS && key < p.seqs.prefix_len) {
-                const int page = p.seqs.prefix_pages[key >> p.pool.page_shift];
-                if (page >= 0 && page < p.pool.n_pages) nibble = p.seqs.prefix_len - key >= 4 ? 15u : (1u << (p.seqs.prefix_len - key)) - 1u;
+            int z = outside, y = 0;
+            bool at_end = false;
+            if (g < n) {
+                const int64_t u = begin + g;
+                const int item = (int)(u / p.cut.tiles), tile = (int)(u - (int64_t)item * p.cut.tiles), kv = item / p.cut.row_tiles;
+                // which keys are there: four to a lane (of one page)
+                const int key = tile * KEYS + lane * 4;
+                uint32_t nibble = 0;
+                if (lane * 4 < KEYS && key < p.seqs.prefix_len) {
+                    const int page = p.seqs.prefix_pages[key >> p.pool.page_shift];
+                    if (page >= 0 && page < p.pool.n_pages) nibble = p.seqs.prefix_len - key >= 4 ? 15u : (1u << (p.seqs.prefix_len - key)) - 1u;
+                }
+                uint32_t word = nibble << (4 * (lane & 7));
+                for (int o = 1; o < 8; o <<= 1) word |= __shfl_xor_sync(0xffffffffu, word, o);
+                // a chunk of rows of one page to a lane
+                const int first = tile * KEYS + (lane << shift), index = first >> p.pool.page_shift;
+                int page = -1;
+                if (lane < chunks && first < p.seqs.prefix_len) page = p.seqs.prefix_pages[index];
+                if (page >= 0 && page < p.pool.n_pages) z = page * p.pool.n_kv + kv;
+                y = first & ((1 << p.pool.page_shift) - 1);
+                at_end = index == last_page;
+                if (use > 0 && !mbar_wait_warp(s_kfree + stage, (uint32_t)((use - 1) & 1))) {
+                    ok = false;
+                    break;
+                }
+                if ((lane & 7) == 0) s_valid[g % PX_RING][lane >> 3] = word;
+                __syncwarp();
+                if (lane == 0) {
+                    mbar_arrive(s_mask + g % PX_RING);
+                    mbar_arrive_expect_tx(s_kfull + stage, (uint32_t)(nd * TR::SUB_K));
+                }
+                __syncwarp();
+                if (lane < chunks)
+                    for (int d = 0; d < nd; ++d) tma_load_3d(sk + (stage * nd + d) * TR::SUB_K + (lane << shift) * 128, &map_k, 64 * d, y, z, s_kfull + stage);
             }
-            uint32_t word = nibble << (4 * (lane & 7));
-            for (int o = 1; o < 8; o <<= 1) word |= __shfl_xor_sync(0xffffffffu, word, o);
-            // a chunk of rows of one page to a lane
-            const int first = tile * KEYS + (lane << shift), index = first >> p.pool.page_shift;
-            int page = -1;
-            if (lane < chunks && first < p.seqs.prefix_len) page = p.seqs.prefix_pages[index];
-            const bool there = page >= 0 && page < p.pool.n_pages;
-            const int z = there ? page * p.pool.n_kv + kv : outside, y = first & ((1 << p.pool.page_shift) - 1);
-            if (use > 0 && !mbar_wait_warp(s_kfree + stage, (uint32_t)((use - 1) & 1))) {
-                ok = false;
-                break;
+            if (g > 0) {
+                const int vs = (g - 1) % p.stages, vu = (g - 1) / p.stages;
+                if (vu > 0 && !mbar_wait_warp(s_vfree + vs, (uint32_t)((vu - 1) & 1))) {
+                    ok = false;
+                    break;
+                }
+                if (lane == 0) mbar_arrive_expect_tx(s_vfull + vs, (uint32_t)(nd * TR::SUB_K));
+                __syncwarp();
+                if (lane < chunks)
+                    for (int d = 0; d < nd; ++d)
+                        tma_load_3d(sv + (vs * nd + d) * TR::SUB_K + (lane << shift) * 128, end_before ? &map_end : &map_v, 64 * d, y_before, z_before, s_vfull + vs);
             }
-            if ((lane & 7) == 0) s_valid[g % PX_RING][lane >> 3] = word;
-            __syncwarp();
-            if (lane == 0) {
-                mbar_arrive(s_mask + g % PX_RING);
-                mbar_arrive_expect_tx(s_kfull + stage, (uint32_t)(nd * TR::SUB_K));
-            }
-            __syncwarp();
-            if (lane < chunks)
-                for (int d = 0; d < nd; ++d) tma_load_3d(sk + (stage * nd + d) * TR::SUB_K + (lane << shift) * 128, &map_k, 64 * d, y, z, s_kfull + stage);
-            if (use > 0 && !mbar_wait_warp(s_vfree + stage, (uint32_t)((use - 1) & 1))) {
-                ok = false;
-                break;
-            }
-            if (lane == 0) mbar_arrive_expect_tx(s_vfull + stage, (uint32_t)(nd * TR::SUB_K));
-            __syncwarp();
-            if (lane < chunks)
-                for (int d = 0; d < nd; ++d) tma_load_3d(sv + (stage * nd + d) * TR::SUB_K + (lane << shift) * 128, index == last_page ? &map_end : &map_v, 64 * d, y, z, s_vfull + stage);
+            z_before = z;
+            y_before = y;
+            end_before = at_end;
         }
         if (!ok)
             for (int i = 0; i < 2000; ++i) __nanosleep(1000);  // copies in flight land within microseconds
     } else if (warp == 8) {
         // ---- products
-        if (lane == 0) {
-            const uint32_t idesc_s = TR::idesc(KEYS, 0), idesc_o = TR::idesc(vn, 1);
-            bool ok = true;
-            int g = 0, segment = 0, np[2] = {0, 0};
-            auto qk = [&](int i, int gt) {  // scores of tile gt for stream i
-                const int stage = gt % p.stages, qtile = TILES == 2 ? i : 0;
-                bool more = false;
-#pragma unroll 1
-                for (int t = TR::QT - 1; t >= 0; --t)  // (small terms first)
-                    for (int kk = 0; 16 * kk < hs; ++kk) {
-                        umma_f16(tmem + (uint32_t)(i * 128), umma_desc_sw128(sq + ((t * TILES + qtile) * nd + (kk >> 2)) * TR::SUB_Q, (kk & 3) * 32),
-                                 umma_desc_sw128(sk + (stage * nd + (kk >> 2)) * TR::SUB_K, (kk & 3) * 32), idesc_s, more ? 1u : 0u);
-                        more = true;
-                    }
-                umma_commit(s_s + i);
-            };
-            auto pv = [&](int i, int gt, bool more) {
-                const int stage = gt % p.stages;
-#pragma unroll 1
-                for (int t = TR::PT - 1; t >= 0; --t)
-                    for (int kk = 0; kk < KEYS / 16; ++kk) {
-                        umma_f16_at(tmem + 256 + (uint32_t)(i * 128), tmem + (uint32_t)(i * 128 + t * (KEYS / 2) + kk * 8), umma_desc_sw128_mn(sv + stage * nd * TR::SUB_K, kk * 2048, TR::SUB_K), idesc_o,
-                                    more ? 1u : 0u);
-                        more = true;
-                    }
-            };
-            for (int64_t u = begin; u < end && ok; ++segment) {
-                const int item = (int)(u / p.cut.tiles), n = (int)min((int64_t)p.cut.tiles - (u - (int64_t)item * p.cut.tiles), end - u);
-                if (!mbar_wait_bounded(&s_q, (uint32_t)(segment & 1))) {
-                    ok = false;
-                    break;
+        // The warp goes through its loop together and one thread of it issues: what differs between the streams is known to the compiler, descriptors are uniform,
+        // stages and phases are counted, not divided for.  (By a thread that had the loop for itself a product took 110 cycles to issue, twice its length.)
+        const bool leader = elect_one();
+        const uint32_t idesc_s = TR::idesc(KEYS, 0), idesc_o = TR::idesc(vn, 1), stage_step = (uint32_t)(nd * TR::SUB_K) >> 4;
+        const uint64_t desc_q = umma_desc_sw128(sq, 0), desc_k = umma_desc_sw128(sk, 0), desc_v = umma_desc_sw128_mn(sv, 0, TR::SUB_K);
+        bool ok = true;
+        int g = 0, segment = 0;
+        struct Place {  // of a stream in a ring
+            int stage;
+            uint32_t phase;
+        } k0, k1, v0, v1;
+        uint32_t p0 = 0, p1 = 0;  // phases of the streams' P
+        auto advance = [&](Place& at) {
+#pragma unroll
+            for (int j = 0; j < (TILES == 2 ? 1 : 2); ++j)
+                if (++at.stage == p.stages) {
+                    at.stage = 0;
+                    at.phase ^= 1u;
                 }
-                const int lag = TILES == 2 ? 1 : 2;  // a stream's next tile
-                for (int s = 0; s < n + lag && ok; ++s)
-                    for (int i = TILES == 2 ? 0 : s & 1; i <= (TILES == 2 ? 1 : s & 1); ++i) {
-                        if (s >= lag) {
-                            const int gt = g + s - lag;
-                            if (!mbar_wait_bounded(s_p + i, (uint32_t)(np[i] & 1)) || !mbar_wait_bounded(s_vfull + gt % p.stages, (uint32_t)(gt / p.stages & 1))) {
-                                ok = false;
-                                break;
-                            }
-                            ++np[i];
-                            tc_fence_after();
-                            pv(i, gt, s >= 2 * lag);
-                            if (TILES == 1 || i == 1) umma_commit(s_vfree + gt % p.stages);
-                        }
-                        if (s < n) {
-                            const int gt = g + s;
-                            if (!mbar_wait_bounded(s_kfull + gt % p.stages, (uint32_t)(gt / p.stages & 1))) {
-                                ok = false;
-                                break;
-                            }
-                            tc_fence_after();
-                            qk(i, gt);
-                            if (TILES == 1 || i == 1) umma_commit(s_kfree + gt % p.stages);
-                        }
+        };
+        auto qk = [&](auto which) {  // scores of a stream's next tile
+            constexpr int i = decltype(which)::value;
+            Place& at = i ? k1 : k0;
+            ok = __all_sync(0xffffffffu, mbar_wait_bounded(s_kfull + at.stage, at.phase));
+            if (!ok) return;
+            tc_fence_after();
+            const uint32_t d = tmem + (uint32_t)(i * 128);
+            const uint64_t kd = desc_k + (uint32_t)at.stage * stage_step;
+#pragma unroll
+            for (int t = TR::QT - 1; t >= 0; --t) {  // (small terms first)
+                const uint64_t qd = desc_q + (uint32_t)((t * TILES + (TILES == 2 ? i : 0)) * nd) * (uint32_t)(TR::SUB_Q >> 4);
+#pragma unroll
+                for (int sub = 0; sub < 2; ++sub)
+                    if (sub < nd && leader) {  // (values behind a head's end are zeros)
+#pragma unroll
+                        for (int kk = 0; kk < 4; ++kk)
+                            umma_f16(d, qd + (uint32_t)(sub * (TR::SUB_Q >> 4) + kk * 2), kd + (uint32_t)(sub * (TR::SUB_K >> 4) + kk * 2), idesc_s, t == TR::QT - 1 && sub == 0 && kk == 0 ? 0u : 1u);
                     }
-                if (ok) umma_commit(&s_seg);
-                g += n;
-                u += n;
             }
+            if (leader) {
+                umma_commit(s_s + i);
+                if (TILES == 1 || i == 1) umma_commit(s_kfree + at.stage);
+            }
+            advance(at);
+        };
+        auto pv = [&](auto which, bool first) {
+            constexpr int i = decltype(which)::value;
+            Place& at = i ? v1 : v0;
+            uint32_t& phase = i ? p1 : p0;
+            const uint32_t a = tmem + (uint32_t)(i * 128), d = tmem + 256 + (uint32_t)(i * 128);
+            const uint64_t vd = desc_v + (uint32_t)at.stage * stage_step;
+            ok = __all_sync(0xffffffffu, mbar_wait_bounded(s_vfull + at.stage, at.phase));
+#pragma unroll
+            for (int half = 0; half < TR::HALVES; ++half) {
+                if (ok) ok = __all_sync(0xffffffffu, mbar_wait_bounded(&s_p[i][half], phase));
+                if (!ok) return;
+                tc_fence_after();
+                if (leader) {
+#pragma unroll
+                    for (int t = TR::PT - 1; t >= 0; --t)
+#pragma unroll
+                        for (int kk = 0; kk < 4; ++kk)
+                            umma_f16_at(d, a + (uint32_t)(t * 32 + half * 32 + kk * 8), vd + (uint32_t)((half * 4 + kk) * (2048 >> 4)), idesc_o,
+                                        half > 0 || t < TR::PT - 1 || kk > 0 ? 1u : first ? 0u : 1u);
+                }
+            }
+            phase ^= 1u;
+            if (leader && (TILES == 1 || i == 1)) umma_commit(s_vfree + at.stage);
+            advance(at);
+        };
+        for (int64_t u = begin; u < end && ok; ++segment) {
+            const int item = (int)(u / p.cut.tiles), tiles = (int)min((int64_t)p.cut.tiles - (u - (int64_t)item * p.cut.tiles), end - u);
+            const int n0 = TILES == 2 ? tiles : (tiles + 1) / 2, n1 = TILES == 2 ? tiles : tiles / 2;  // tiles of the streams
+            k0 = v0 = {g % p.stages, (uint32_t)(g / p.stages & 1)};
+            const int g1 = TILES == 2 ? g : g + 1;
+            k1 = v1 = {g1 % p.stages, (uint32_t)(g1 / p.stages & 1)};
+            ok = __all_sync(0xffffffffu, mbar_wait_bounded(&s_q, (uint32_t)(segment & 1)));
+            using First = std::integral_constant<int, 0>;
+            using Second = std::integral_constant<int, 1>;
+#pragma unroll 1
+            for (int n = -1; n < n0 && ok; ++n) {
+                if (n >= 0) pv(First(), n == 0);
+                if (ok && n + 1 < n0) qk(First());
+                if (ok && n >= 0 && n < n1) pv(Second(), n == 0);
+                if (ok && n + 1 < n1) qk(Second());
+            }
+            if (ok && leader) umma_commit(&s_seg);
+            g += tiles;
+            u += tiles;
         }
     } else {
         // ---- softmax: a thread per row of its stream
@@ -300,22 +348,25 @@ __global__ void __launch_bounds__(PX_THREADS, 1) paged_prefix_kernel(const __gri
             for (int t = TILES == 2 ? 0 : i; t < n; t += TILES == 2 ? 1 : 2) {
                 const int gt = g + t;
                 if (ok) ok = __all_sync(0xffffffffu, mbar_wait_bounded(s_mask + gt % PX_RING, (uint32_t)(gt / PX_RING & 1)));
-                if (ok) ok = __all_sync(0xffffffffu, mbar_wait_bounded(s_s + i, (uint32_t)(ns & 1)));
+                if (ok) ok = __all_sync(0xffffffffu, mbar_wait_bounded(s_s + i, (uint32_t)(ns & 1)));  // (P V of the tile before is done then, too)
                 ++ns;
                 tc_fence_after();
-                float m4[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
-#pragma unroll 1
-                for (int c = 0; c < KEYS; c += 64) {
-                    float x[64];
-                    tmem_ld64f(ts + (uint32_t)c, x);
-                    const uint32_t v0 = s_valid[gt % PX_RING][c >> 5], v1 = s_valid[gt % PX_RING][(c >> 5) + 1];
-                    if ((v0 & v1) != ~0u) {
+                float x[KEYS];
 #pragma unroll
-                        for (int k = 0; k < 64; ++k) x[k] = (k < 32 ? v0 : v1) >> (k & 31) & 1 ? x[k] : -INFINITY;
-                    }
+                for (int c = 0; c < KEYS; c += 64) tmem_load(ts + (uint32_t)c, *reinterpret_cast<float(*)[64]>(x + c));
+                uint32_t there[KEYS / 32], all = ~0u;
 #pragma unroll
-                    for (int k = 0; k < 64; k += 2) m4[k >> 1 & 3] = fmaxf(fmaxf(x[k], x[k + 1]), m4[k >> 1 & 3]);
+                for (int c = 0; c < KEYS / 32; ++c) {
+                    there[c] = s_valid[gt % PX_RING][c];
+                    all &= there[c];
                 }
+                if (all != ~0u) {
+#pragma unroll
+                    for (int k = 0; k < KEYS; ++k) x[k] = there[k >> 5] >> (k & 31) & 1 ? x[k] : -INFINITY;
+                }
+                float m4[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
+#pragma unroll
+                for (int k = 0; k < KEYS; k += 2) m4[k >> 1 & 3] = fmaxf(fmaxf(x[k], x[k + 1]), m4[k >> 1 & 3]);
                 const float mx = fmaxf(fmaxf(m4[0], m4[1]), fmaxf(m4[2], m4[3])) * sc;
                 if (!some) {
                     m = mx;
@@ -324,43 +375,38 @@ __global__ void __launch_bounds__(PX_THREADS, 1) paged_prefix_kernel(const __gri
                     l *= corr;
                     m = mn;
 #pragma unroll 1
-                    for (int c = 0; c < vn; c += 32) {
-                        float o[32];
-                        tmem_ld32f(to + (uint32_t)c, o);
+                    for (int c = 0; c < vn; c += 16) {
+                        float o[16];
+                        tmem_ld16f(to + (uint32_t)c, o);
 #pragma unroll
-                        for (int e = 0; e < 32; ++e) o[e] *= corr;
-                        tmem_st32f(to + (uint32_t)c, o);
+                        for (int e = 0; e < 16; ++e) o[e] *= corr;
+                        tmem_st16f(to + (uint32_t)c, o);
                     }
                 }
                 some = true;
                 const float use = m == -INFINITY ? 0.f : m;
                 float l4[4] = {0.f, 0.f, 0.f, 0.f};
-#pragma unroll 1
-                for (int c = 0; c < KEYS; c += 64) {
-                    float x[64];
-                    tmem_ld64f(ts + (uint32_t)c, x);
-                    const uint32_t v0 = s_valid[gt % PX_RING][c >> 5], v1 = s_valid[gt % PX_RING][(c >> 5) + 1];
 #pragma unroll
-                    for (int k = 0; k < 64; ++k) x[k] = exp2_approx(fmaf(x[k], sc, -use));
-                    if ((v0 & v1) != ~0u) {
+                for (int half = 0; half < TR::HALVES; ++half) {
 #pragma unroll
-                        for (int k = 0; k < 64; ++k) x[k] = (k < 32 ? v0 : v1) >> (k & 31) & 1 ? x[k] : 0.f;
+                    for (int k = half * 64; k < half * 64 + 64; ++k) {
+                        x[k] = exp2_approx(fmaf(x[k], sc, -use));
+                        l4[k & 3] += x[k];
                     }
-#pragma unroll
-                    for (int k = 0; k < 64; ++k) l4[k & 3] += x[k];
 #pragma unroll
                     for (int t2 = 0; t2 < TR::PT; ++t2) {
                         uint32_t w[32];
 #pragma unroll
-                        for (int k = 0; k < 32; ++k) w[k] = TR::PT == 1 ? pair_of<T>(x[2 * k], x[2 * k + 1]) : split_pair<T>(x[2 * k], x[2 * k + 1]);
-                        tmem_st32u(ts + (uint32_t)(t2 * 32 + c / 2), w);  // (columns of scores that have been read)
+                        for (int k = 0; k < 32; ++k)
+                            w[k] = TR::PT == 1 ? pair_of<T>(x[half * 64 + 2 * k], x[half * 64 + 2 * k + 1]) : split_pair<T>(x[half * 64 + 2 * k], x[half * 64 + 2 * k + 1]);
+                        tmem_st32u(ts + (uint32_t)((t2 + half) * 32), w);  // (in the place of the scores, which have been read)
                     }
+                    tmem_wait_st();
+                    tc_fence_before();
+                    __syncwarp();
+                    if (lane == 0) mbar_arrive(&s_p[i][half]);
                 }
                 l += (l4[0] + l4[1]) + (l4[2] + l4[3]);
-                tmem_wait_st();
-                tc_fence_before();
-                __syncwarp();
-                if (lane == 0) mbar_arrive(s_p + i);
             }
             // the segment's products are all done: this row's sums to the workspace
             if (ok) ok = __all_sync(0xffffffffu, mbar_wait_bounded(&s_seg, (uint32_t)(segment & 1)));
