@@ -9,7 +9,7 @@
 // A thread takes its row of scores to registers at once and hands P over in two halves, so that P V begins beside the second half's exponentials.  (Measured and not kept: two buffers of 64 keys per stream, Q K^T a step ahead; a product of 64 columns
 // takes as long as one of 128.)
 //   warps 0-3, 4-7  the streams' softmax; before it they bring the block's rows of Q into shared memory, after it the sums to the workspace
-//   warp 8          issues the products: P V of a tile, then Q K^T of the stream's next, which overwrites that P
+//   warps 8, 10     issue a stream's products each: P V of a tile, then Q K^T of the stream's next, which overwrites that P
 //   warp 9          TMA copies of keys and values straight from the pages: 8 rows or more at a time, V's rows behind the prefix's end through a map
 //                   that ends there, so that they are zeros; pages that are none lie outside the map and are zeros, too
 // Rows are rescaled only when a maximum has grown by more than 2^8.  The work, items (key/value head, row tile) of the prefix' key tiles, is cut
@@ -20,7 +20,7 @@
 
 namespace l2b {
 
-constexpr int PX_ROWS = 128, PX_THREADS = 320, PX_MAX_STAGES = 8, PX_RING = 16;  // PX_RING: masks under way, more than stages
+constexpr int PX_ROWS = 128, PX_THREADS = 352, PX_MAX_STAGES = 8, PX_RING = 16;  // PX_RING: masks under way, more than stages
 
 struct PrefixParams : PagedWork {
     const void* q;
@@ -144,13 +144,13 @@ __global__ void __launch_bounds__(PX_THREADS, 1) paged_prefix_kernel(const __gri
     if (threadIdx.x == 0) {
         for (int i = 0; i < p.stages; ++i) {
             mbar_init(s_kfull + i, 1);
-            mbar_init(s_kfree + i, 1);
+            mbar_init(s_kfree + i, TILES);  // (the streams that read it)
             mbar_init(s_vfull + i, 1);
-            mbar_init(s_vfree + i, 1);
+            mbar_init(s_vfree + i, TILES);
         }
         for (int i = 0; i < PX_RING; ++i) mbar_init(s_mask + i, 1);
         mbar_init(&s_q, 8);
-        mbar_init(&s_seg, 1);
+        mbar_init(&s_seg, 2);
         for (int i = 0; i < 2; ++i) {
             mbar_init(s_s + i, 1);
             mbar_init(&s_p[i][0], 4);
@@ -233,20 +233,22 @@ __global__ void __launch_bounds__(PX_THREADS, 1) paged_prefix_kernel(const __gri
         }
         if (!ok)
             for (int i = 0; i < 2000; ++i) __nanosleep(1000);  // copies in flight land within microseconds
-    } else if (warp == 8) {
-        // ---- products
-        // The warp goes through its loop together and one thread of it issues: what differs between the streams is known to the compiler, descriptors are uniform,
-        // stages and phases are counted, not divided for.  (By a thread that had the loop for itself a product took 110 cycles to issue, twice its length.)
+    } else if (warp >= 8) {
+        // ---- products of a stream
+        // The warp goes through its loop together and one thread of it issues: descriptors are uniform, stages and phases are counted, not divided for.  (By a thread
+        // that had the loop for itself a product took 110 cycles to issue, twice its length.)
+        const int i = warp == 8 ? 0 : 1;
         const bool leader = elect_one();
         const uint32_t idesc_s = TR::idesc(KEYS, 0), idesc_o = TR::idesc(vn, 1), stage_step = (uint32_t)(nd * TR::SUB_K) >> 4;
-        const uint64_t desc_q = umma_desc_sw128(sq, 0), desc_k = umma_desc_sw128(sk, 0), desc_v = umma_desc_sw128_mn(sv, 0, TR::SUB_K);
+        const uint64_t desc_q = umma_desc_sw128(sq + (TILES == 2 ? i : 0) * nd * TR::SUB_Q, 0), desc_k = umma_desc_sw128(sk, 0), desc_v = umma_desc_sw128_mn(sv, 0, TR::SUB_K);
+        const uint32_t ds = tmem + (uint32_t)(i * 128), dout = tmem + 256 + (uint32_t)(i * 128);
         bool ok = true;
         int g = 0, segment = 0;
-        struct Place {  // of a stream in a ring
+        struct Place {  // in a ring
             int stage;
             uint32_t phase;
-        } k0, k1, v0, v1;
-        uint32_t p0 = 0, p1 = 0;  // phases of the streams' P
+        } k = {0, 0}, v = {0, 0};
+        uint32_t p_phase = 0;
         auto advance = [&](Place& at) {
 #pragma unroll
             for (int j = 0; j < (TILES == 2 ? 1 : 2); ++j)
@@ -255,41 +257,34 @@ __global__ void __launch_bounds__(PX_THREADS, 1) paged_prefix_kernel(const __gri
                     at.phase ^= 1u;
                 }
         };
-        auto qk = [&](auto which) {  // scores of a stream's next tile
-            constexpr int i = decltype(which)::value;
-            Place& at = i ? k1 : k0;
-            ok = __all_sync(0xffffffffu, mbar_wait_bounded(s_kfull + at.stage, at.phase));
+        auto qk = [&]() {  // scores of the next tile
+            ok = __all_sync(0xffffffffu, mbar_wait_bounded(s_kfull + k.stage, k.phase));
             if (!ok) return;
             tc_fence_after();
-            const uint32_t d = tmem + (uint32_t)(i * 128);
-            const uint64_t kd = desc_k + (uint32_t)at.stage * stage_step;
+            const uint64_t kd = desc_k + (uint32_t)k.stage * stage_step;
 #pragma unroll
             for (int t = TR::QT - 1; t >= 0; --t) {  // (small terms first)
-                const uint64_t qd = desc_q + (uint32_t)((t * TILES + (TILES == 2 ? i : 0)) * nd) * (uint32_t)(TR::SUB_Q >> 4);
+                const uint64_t qd = desc_q + (uint32_t)(t * TILES * nd) * (uint32_t)(TR::SUB_Q >> 4);
 #pragma unroll
                 for (int sub = 0; sub < 2; ++sub)
                     if (sub < nd && leader) {  // (values behind a head's end are zeros)
 #pragma unroll
                         for (int kk = 0; kk < 4; ++kk)
-                            umma_f16(d, qd + (uint32_t)(sub * (TR::SUB_Q >> 4) + kk * 2), kd + (uint32_t)(sub * (TR::SUB_K >> 4) + kk * 2), idesc_s, t == TR::QT - 1 && sub == 0 && kk == 0 ? 0u : 1u);
+                            umma_f16(ds, qd + (uint32_t)(sub * (TR::SUB_Q >> 4) + kk * 2), kd + (uint32_t)(sub * (TR::SUB_K >> 4) + kk * 2), idesc_s, t == TR::QT - 1 && sub == 0 && kk == 0 ? 0u : 1u);
                     }
             }
             if (leader) {
                 umma_commit(s_s + i);
-                if (TILES == 1 || i == 1) umma_commit(s_kfree + at.stage);
+                umma_commit(s_kfree + k.stage);
             }
-            advance(at);
+            advance(k);
         };
-        auto pv = [&](auto which, bool first) {
-            constexpr int i = decltype(which)::value;
-            Place& at = i ? v1 : v0;
-            uint32_t& phase = i ? p1 : p0;
-            const uint32_t a = tmem + (uint32_t)(i * 128), d = tmem + 256 + (uint32_t)(i * 128);
-            const uint64_t vd = desc_v + (uint32_t)at.stage * stage_step;
-            ok = __all_sync(0xffffffffu, mbar_wait_bounded(s_vfull + at.stage, at.phase));
+        auto pv = [&](bool first) {
+            const uint64_t vd = desc_v + (uint32_t)v.stage * stage_step;
+            ok = __all_sync(0xffffffffu, mbar_wait_bounded(s_vfull + v.stage, v.phase));
 #pragma unroll
             for (int half = 0; half < TR::HALVES; ++half) {
-                if (ok) ok = __all_sync(0xffffffffu, mbar_wait_bounded(&s_p[i][half], phase));
+                if (ok) ok = __all_sync(0xffffffffu, mbar_wait_bounded(&s_p[i][half], p_phase));
                 if (!ok) return;
                 tc_fence_after();
                 if (leader) {
@@ -297,29 +292,25 @@ __global__ void __launch_bounds__(PX_THREADS, 1) paged_prefix_kernel(const __gri
                     for (int t = TR::PT - 1; t >= 0; --t)
 #pragma unroll
                         for (int kk = 0; kk < 4; ++kk)
-                            umma_f16_at(d, a + (uint32_t)(t * 32 + half * 32 + kk * 8), vd + (uint32_t)((half * 4 + kk) * (2048 >> 4)), idesc_o,
+                            umma_f16_at(dout, ds + (uint32_t)(t * 32 + half * 32 + kk * 8), vd + (uint32_t)((half * 4 + kk) * (2048 >> 4)), idesc_o,
                                         half > 0 || t < TR::PT - 1 || kk > 0 ? 1u : first ? 0u : 1u);
                 }
             }
-            phase ^= 1u;
-            if (leader && (TILES == 1 || i == 1)) umma_commit(s_vfree + at.stage);
-            advance(at);
+            p_phase ^= 1u;
+            if (leader) umma_commit(s_vfree + v.stage);
+            advance(v);
         };
         for (int64_t u = begin; u < end && ok; ++segment) {
             const int item = (int)(u / p.cut.tiles), tiles = (int)min((int64_t)p.cut.tiles - (u - (int64_t)item * p.cut.tiles), end - u);
-            const int n0 = TILES == 2 ? tiles : (tiles + 1) / 2, n1 = TILES == 2 ? tiles : tiles / 2;  // tiles of the streams
-            k0 = v0 = {g % p.stages, (uint32_t)(g / p.stages & 1)};
-            const int g1 = TILES == 2 ? g : g + 1;
-            k1 = v1 = {g1 % p.stages, (uint32_t)(g1 / p.stages & 1)};
+            const int n = TILES == 2 ? tiles : (tiles + 1 - i) / 2;  // of this stream
+            const int first = TILES == 2 ? g : g + i;
+            k = v = {first % p.stages, (uint32_t)(first / p.stages & 1)};
             ok = __all_sync(0xffffffffu, mbar_wait_bounded(&s_q, (uint32_t)(segment & 1)));
-            using First = std::integral_constant<int, 0>;
-            using Second = std::integral_constant<int, 1>;
+            if (ok && n > 0) qk();
 #pragma unroll 1
-            for (int n = -1; n < n0 && ok; ++n) {
-                if (n >= 0) pv(First(), n == 0);
-                if (ok && n + 1 < n0) qk(First());
-                if (ok && n >= 0 && n < n1) pv(Second(), n == 0);
-                if (ok && n + 1 < n1) qk(Second());
+            for (int t = 0; t < n && ok; ++t) {
+                pv(t == 0);
+                if (ok && t + 1 < n) qk();
             }
             if (ok && leader) umma_commit(&s_seg);
             g += tiles;
