@@ -50,7 +50,7 @@ struct SampleShared {
     double table[FS_TABLE];    // 2^(-i / FS_TABLE)
     uint64_t sums[FS_WARPS];
     float wmax[FS_WARPS], wmin[FS_WARPS], tmax[FS_THREADS];
-    float queue[FS_WARPS][64];
+    float queue[FS_WARPS][160];
     // of each block of the cluster, written by it
     float max[FS_CLUSTER], min[FS_CLUSTER], tau[FS_CLUSTER];
     uint32_t count[3][FS_CLUSTER];  // listed for a top-k, for the bin with the k-th value, for the nucleus' bin
@@ -72,23 +72,27 @@ __device__ __forceinline__ uint64_t order_key(float x, uint32_t index) { return 
 
 struct SampleRow {
     float top;
-    double shift, rate, floor_t;  // w = 2^-t, t = shift - x * rate; floor_t: no weight beyond
-    double min_p;  // at most 1: the first token is always kept
+    double dtop, rate;  // w = 2^-t, t = (top - x) * rate
+    double min_p;       // at most 1: the first token is always kept
     const double* table;
-    // 2^-t: t to the nearest 1/128 from the table, the rest (a = rest * ln 2 up to 0.0027) by the exponential series up to a^4 / 24; a^5 / 120 is 1.2e-15.
+    bool infinite;      // top
+    // 2^-t: t to the nearest 1/128 from the table, the rest by the exponential series up to its fourth power (|rest * ln 2| <= 0.0027, whose fifth over 120 is
+    // 1.2e-15).  No branch: beyond 100 (of -inf, too) t is 100, and the mass 0.
     __device__ __forceinline__ double weight(float x) const {
-        if (x == top) return 1.0;
-        const double t = fma(-(double)x, rate, shift);
-        if (!(t < floor_t)) return 0.0;  // (also: infinite minus infinite)
-        constexpr double magic = 6755399441055744.0 / FS_TABLE;  // 1.5 * 2^52 / 128: the sum's last bit is 1/128
+        if (infinite) return x == top ? 1.0 : 0.0;
+        double t = (dtop - (double)x) * rate;
+        t = t < 100.0 ? t : 100.0;
+        constexpr double magic = 6755399441055744.0 / FS_TABLE, l = 0.6931471805599453;  // 1.5 * 2^52 / 128: the sum's last bit is 1/128
         const double u = t + magic;
-        const int k = max(0, (int)(__double_as_longlong(u) & 0xffffffff));
-        const double a = (t - (u - magic)) * -0.6931471805599453;
-        const double q = fma(a, fma(a, fma(a, fma(a, 1.0 / 24, 1.0 / 6), 0.5), 1.0), 1.0) * table[k & (FS_TABLE - 1)];
-        return __longlong_as_double(__double_as_longlong(q) - ((long long)(k / FS_TABLE) << 52));  // (2^-46 at least)
+        const int k = __double2loint(u);
+        const double rest = t - (u - magic), q = fma(rest, fma(rest, fma(rest, fma(rest, l * l * l * l / 24, -l * l * l / 6), l * l / 2), -l), 1.0) * table[k & (FS_TABLE - 1)];
+        return __hiloint2double(__double2hiint(q) - (k / FS_TABLE << 20), __double2loint(q));
     }
     // In units of 2^-44, to the nearest: the last bits of w + 2^8.
-    static __device__ __forceinline__ uint64_t units(double w) { return (uint64_t)(__double_as_longlong(w + 256.0) - __double_as_longlong(256.0)); }
+    static __device__ __forceinline__ uint64_t units(double w) {
+        const double v = w + 256.0;
+        return (uint64_t)(uint32_t)(__double2hiint(v) - 0x40700000) << 32 | (uint32_t)__double2loint(v);
+    }
     __device__ __forceinline__ uint64_t mass(float x) const { return units(weight(x)); }
     // of a value that the order keeps
     __device__ __forceinline__ uint64_t kept_mass(float x) const {
@@ -295,9 +299,9 @@ __global__ void __launch_bounds__(FS_THREADS, 2) filtered_sample_kernel(const __
     }
     SampleRow r;
     r.top = mx;
+    r.infinite = mx == INFINITY;
+    r.dtop = (double)mx;
     r.rate = 1.4426950408889634 / (double)temperature;
-    r.shift = (double)mx * r.rate;
-    r.floor_t = 46.0;
     r.min_p = min_p > 0.f ? fmin((double)min_p, 1.0) : 0.0;
     r.table = s.table;
     u = u > 0.0 ? fmin(u, 1.0) : 0.0;
@@ -328,7 +332,9 @@ __global__ void __launch_bounds__(FS_THREADS, 2) filtered_sample_kernel(const __
         __syncthreads();
         at += s.base;
         if (mine) {
-            for (int i = tid; i < quads; i += FS_THREADS)
+            for (int i = tid; i < quads; i += FS_THREADS) {
+                const float4 q = *reinterpret_cast<const float4*>(fs_x + 4 * i);
+                if (!((q.x >= lo && q.x <= hi) || (q.y >= lo && q.y <= hi) || (q.z >= lo && q.z <= hi) || (q.w >= lo && q.w <= hi))) continue;
                 for (int e = 0; e < 4; ++e) {
                     const float x = fs_x[4 * i + e];
                     const uint64_t key = order_key(x, (uint32_t)(first + 4 * i + e));
@@ -338,6 +344,7 @@ __global__ void __launch_bounds__(FS_THREADS, 2) filtered_sample_kernel(const __
                         ++at;
                     }
                 }
+            }
         }
         cluster.sync();
         uint32_t all = 0;
@@ -477,13 +484,22 @@ __global__ void __launch_bounds__(FS_THREADS, 2) filtered_sample_kernel(const __
 
     if (has_p) {
         uint64_t sum = 0;
-        for (int i = tid; i < n; i += FS_THREADS) {
-            const float x = fs_x[i];
-            if (x > -INFINITY && (cut == 0 || order_key(x, (uint32_t)(first + i)) >= cut)) {
-                const uint64_t w = r.mass(x);
-                const int b = bin_of(x);
-                sum += w;
-                if (w && b < FS_BINS - 1) add_mass(s, b, w);
+#pragma unroll 1
+        for (int i = tid; i < quads; i += FS_THREADS) {
+            const float4 x4 = *reinterpret_cast<const float4*>(fs_x + 4 * i);
+            const float x[4] = {x4.x, x4.y, x4.z, x4.w};
+            uint64_t w[4];
+#pragma unroll
+            for (int e = 0; e < 4; ++e) w[e] = r.mass(x[e]);  // (of -inf: 0)
+            if (cut != 0) {
+#pragma unroll
+                for (int e = 0; e < 4; ++e) w[e] = order_key(x[e], (uint32_t)(first + 4 * i + e)) >= cut ? w[e] : 0;
+            }
+#pragma unroll
+            for (int e = 0; e < 4; ++e) {
+                sum += w[e];
+                const int b = bin_of(x[e]);
+                if (w[e] && b < FS_BINS - 1) add_mass(s, b, w[e]);
             }
         }
         sum = block_total(sum, s);
@@ -512,10 +528,10 @@ __global__ void __launch_bounds__(FS_THREADS, 2) filtered_sample_kernel(const __
     }
 
     // the choice among all that is kept: masses per warp's stretch of the slice, then inside the stretch that holds it
-    if (r.min_p > 0.0) r.floor_t = fmin(r.floor_t, fmax(1e-6, 1e-6 - log2(r.min_p)));  // (a little beyond min_p: the comparison is made on the weight)
-    const int stretch = ((p.slice + FS_WARPS - 1) / FS_WARPS + 31) / 32 * 32;
+    const double floor_t = r.min_p > 0.0 ? fmin(46.0, fmax(1e-6, 1e-6 - log2(r.min_p))) : 46.0;  // (a little beyond min_p: the comparison is made on the weight)
+    const int stretch = ((p.slice + FS_WARPS - 1) / FS_WARPS + 127) / 128 * 128;
     // no smaller value is kept: the cut's, or the one from which on weights vanish (or are below min_p), with room for rounding
-    const float low = fmaxf(fmaxf(from_ordered((uint32_t)(cut >> 32) | (cut ? 0u : 0x00800000u)), -FLT_MAX), mx - (float)(r.floor_t / r.rate) * 1.0001f - fabsf(mx) * 0x1p-21f);
+    const float low = fmaxf(fmaxf(from_ordered((uint32_t)(cut >> 32) | (cut ? 0u : 0x00800000u)), -FLT_MAX), mx - (float)(floor_t / r.rate) * 1.0001f - fabsf(mx) * 0x1p-21f);
     auto kept = [&](int i) -> uint64_t {
         const float x = fs_x[i];
         return x >= low && order_key(x, (uint32_t)(first + i)) >= cut ? r.kept_mass(x) : 0;
@@ -523,26 +539,41 @@ __global__ void __launch_bounds__(FS_THREADS, 2) filtered_sample_kernel(const __
     const int lo = min(n, warp * stretch), hi = min(n, lo + stretch);
     uint64_t sum = 0;
     int queued = 0;
-    for (int i0 = lo; i0 < hi; i0 += 32) {
-        const int i = i0 + lane;
-        const float x = i < hi ? fs_x[i] : -INFINITY;
-        const bool in = x >= low && (x > low || order_key(x, (uint32_t)(first + i)) >= cut);
-        const unsigned v = __ballot_sync(0xffffffffu, in);
-        if (v == ~0u) {
-            sum += r.kept_mass(x);
-        } else if (v) {
-            if (in) s.queue[warp][queued + __popc(v & ((1u << lane) - 1u))] = x;
-            queued += __popc(v);
-            __syncwarp();
-            if (queued >= 32) {
-                sum += r.kept_mass(s.queue[warp][lane]);
-                queued -= 32;
-                const float over = lane < queued ? s.queue[warp][32 + lane] : 0.f;
-                __syncwarp();
-                if (lane < queued) s.queue[warp][lane] = over;
-                __syncwarp();
-            }
+    for (int i0 = lo; i0 < hi; i0 += 128) {
+        const int i = i0 + 4 * lane;  // (what lies behind the slice's end up to a multiple of 4 is -inf)
+        float4 q = make_float4(-INFINITY, -INFINITY, -INFINITY, -INFINITY);
+        if (i < hi) q = *reinterpret_cast<const float4*>(fs_x + i);
+        const float x[4] = {q.x, q.y, q.z, q.w};
+        bool in[4];
+        int mine = 0;
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+            in[e] = x[e] >= low && (x[e] > low || order_key(x[e], (uint32_t)(first + i + e)) >= cut);
+            mine += in[e];
         }
+        if (__all_sync(0xffffffffu, mine >= 2)) {  // (most of them: as they lie)
+#pragma unroll
+            for (int e = 0; e < 4; ++e) sum += in[e] ? r.kept_mass(x[e]) : 0;
+            continue;
+        }
+        int at = mine;
+#pragma unroll
+        for (int o = 1; o < 32; o <<= 1) {
+            const int v = __shfl_up_sync(0xffffffffu, at, o);
+            if (lane >= o) at += v;
+        }
+        const int all = __shfl_sync(0xffffffffu, at, 31);
+        at += queued - mine;
+#pragma unroll
+        for (int e = 0; e < 4; ++e)
+            if (in[e]) s.queue[warp][at++] = x[e];
+        queued += all;
+        __syncwarp();
+        while (queued >= 32) {  // the last ones
+            queued -= 32;
+            sum += r.kept_mass(s.queue[warp][queued + lane]);
+        }
+        __syncwarp();
     }
     if (lane < queued) sum += r.kept_mass(s.queue[warp][lane]);
     sum = warp_sum64(sum);
