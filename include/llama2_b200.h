@@ -197,6 +197,10 @@ int32_t l2b_generate(l2b_session* session, const int32_t* host_prompt, int32_t n
 
 /* Copy the logits of the most recent position to the host (state.logits). */
 int32_t l2b_session_logits(l2b_session* session, float* host_logits);
+/* A token from those logits (of the most recent l2b_forward, l2b_decode_next or l2b_prefill call) by temperature and the cuts of l2b_sample_device
+ * (top_k 0, top_p 1 and min_p 0: none); temperature 0: argmax.  l2b_forward(session, token, pos, NULL) and this call are one iteration of the loop in
+ * `sample` (src/inference.jl:349-385) with cuts. */
+int32_t l2b_session_sample(l2b_session* session, float temperature, int32_t top_k, float top_p, float min_p, double uniform, int32_t* next_token);
 /* Copy an activation buffer of the most recent forward for stage-wise checks:
  * which: 0 = x (residual stream after the last layer, before the final norm is applied in place),
  *        2 = q (after RoPE, last layer), 5 = hb (SwiGLU output, last layer).  Returns element count in *n. */
@@ -370,7 +374,7 @@ int32_t l2b_paged_attention_device(const l2b_paged_cache* cache, const l2b_paged
  * tokens in order (larger logits first, of equal ones the lower index first):
  *   top_k in 1 .. vocab keeps the first top_k; other values: no cut;
  *   top_p < 1 keeps those of them before which less than top_p of their whole mass lies; 1 and more: no cut;
- *   min_p > 0 keeps those with w_i >= min_p;
+ *   min_p > 0 keeps those with w_i >= min_p (more than 1 counts as 1);
  *   the first one is always kept.
  * The token is the first, by index, at which the kept tokens' cumulated mass exceeds uniform times their whole (computed so that the result hangs on the
  * row alone).  T <= 0: argmax, first of equals.  Logits that are -inf or no numbers are never chosen; a row without any other gets token -1 and

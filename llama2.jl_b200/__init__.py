@@ -5,7 +5,8 @@ from .load_gguf import load_gguf_model  # noqa: F401
 from .load_karpathy import load_karpathy_model  # noqa: F401
 from .load_stack import load_model, load_stack_model  # noqa: F401
 from .model import (BatchRunState, LanguageModel, ModelConfig, QuantMatrix, RunState, StackConfig, StackWeights,  # noqa: F401
-                    TransformerLayerWeights, TransformerWeights, dequantize, extend, generate, matmul_, prefill, sample, transformer_)
+                    TransformerLayerWeights, TransformerWeights, dequantize, extend, generate, matmul_, prefill, sample, sample_next,
+                    transformer_)
 from .tokenizer import BPETokenizer, CharTokenizer, encode  # noqa: F401
 
 __all__ = ["ModelConfig", "CharTokenizer", "LanguageModel", "load_gguf_model", "load_karpathy_model", "encode", "sample"]

@@ -85,6 +85,7 @@ _SIGNATURES = {
     "l2b_decode_next": ([_P, C.c_int32, C.c_int32, C.c_float, C.c_double, C.POINTER(C.c_int32)], C.c_int32),
     "l2b_generate": ([_P, _P, C.c_int32, C.c_int32, C.c_float, C.c_uint64, _P, C.POINTER(C.c_float)], C.c_int32),
     "l2b_session_logits": ([_P, _P], C.c_int32),
+    "l2b_session_sample": ([_P, C.c_float, C.c_int32, C.c_float, C.c_float, C.c_double, C.POINTER(C.c_int32)], C.c_int32),
     "l2b_session_read": ([_P, C.c_int32, _P, C.c_int64, C.POINTER(C.c_int64)], C.c_int32),
     "l2b_session_last_device_ms": ([_P, C.POINTER(C.c_float)], C.c_int32),
     "l2b_session_last_phase_ms": ([_P, C.POINTER(C.c_float), C.POINTER(C.c_float)], C.c_int32),

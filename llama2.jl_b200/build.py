@@ -13,7 +13,7 @@ HEADERS = ["csrc/common.cuh", "csrc/kquants.cuh", "csrc/fused_matvec.cuh", "csrc
            "csrc/tcgen05.cuh", "csrc/json.h", "csrc/safetensors.h", "csrc/stack_config.h", "csrc/stack.h", "csrc/dense_ops.cuh",
            "csrc/dense_matvec.cuh", "csrc/dense_gemm.cuh", "csrc/stack_rows.cuh", "csrc/cache_scan.cuh", "csrc/latent_attention.cuh",
            "csrc/head_attention.cuh", "csrc/head_prefill.cuh", "csrc/mlstm.cuh", "csrc/mlstm_prefill.cuh", "csrc/latent_prefill.cuh",
-           "csrc/paged.h", "csrc/paged_append.cuh", "csrc/paged_attention.cuh", "csrc/paged_prefix.cuh", "csrc/filtered_sampling.cuh",
+           "csrc/paged.h", "csrc/paged_append.cuh", "csrc/paged_attention.cuh", "csrc/paged_prefix.cuh", "csrc/filtered_sampling.cuh", "csrc/serving.h",
            "../include/llama2_b200.h"]
 OUTPUT = os.path.join(_HERE, "libllama2_b200.so")
 SYNTH_OUTPUT = os.path.join(_HERE, "libl2b_synth.so")  # test support: seeded synthetic data, plain C++

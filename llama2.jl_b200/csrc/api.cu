@@ -14,6 +14,7 @@
 #include "gguf_reader.h"
 #include "host_common.h"
 #include "safetensors.h"
+#include "serving.h"
 #include "stack.h"
 #include "attention.cuh"
 #include "fused_matvec.cuh"
@@ -2412,6 +2413,21 @@ extern "C" int32_t l2b_session_logits(l2b_session* s, float* host_logits) {
     CU(cudaSetDevice(s->model->device));
     CU(cudaStreamSynchronize(s->stream));
     CU(cudaMemcpy(host_logits, s->logits, (size_t)s->model->cfg.vocab_size * 4, cudaMemcpyDeviceToHost));
+    return L2B_OK;
+}
+
+extern "C" int32_t l2b_session_sample(l2b_session* s, float temperature, int32_t top_k, float top_p, float min_p, double uniform, int32_t* next) {
+    if (!s || !next) return fail(L2B_ERR_BAD_ARG, "null argument");
+    if (!(temperature >= 0.f)) return fail(L2B_ERR_BAD_ARG, "temperature must be >= 0");
+    if (!(uniform >= 0.0 && uniform < 1.0)) return fail(L2B_ERR_BAD_ARG, "uniform must lie in [0,1)");
+    const int vocab = s->model->cfg.vocab_size;
+    if (vocab > SAMPLE_MAX_VOCAB) return fail(L2B_ERR_BAD_ARG, "a vocabulary of more than 393216");
+    CU(cudaSetDevice(s->model->device));
+    L2B_TRY(enqueue_filtered_sample(s->logits, vocab, temperature, top_k, top_p, min_p, uniform, s->next_token, s->model->device, s->stream));
+    CU(cudaMemcpyAsync(&s->h_small[0], s->next_token, 4, cudaMemcpyDeviceToHost, s->stream));
+    CU(cudaStreamSynchronize(s->stream));
+    if (s->h_small[0] < 0 || s->h_small[0] >= vocab) return fail(L2B_ERR_CUDA, "no valid token could be chosen (the logits are not finite)");
+    *next = s->h_small[0];
     return L2B_OK;
 }
 

@@ -31,9 +31,12 @@ struct SampleParams {
     const void* logits;
     int64_t stride;
     int vocab, slice, cluster;
-    const float *temperature, *top_p, *min_p;  // null: 1, no cut, no cut
-    const int* top_k;                          // null: no cut
+    const float *temperature, *top_p, *min_p;  // of each row; null: the same for all, as below
+    const int* top_k;
     const double* uniform;
+    float same_temperature, same_top_p, same_min_p;
+    int same_top_k;
+    double same_uniform;
     int* tokens;
     float* probs;  // may be null
 };
@@ -188,10 +191,10 @@ __global__ void __launch_bounds__(FS_THREADS, 2) filtered_sample_kernel(const __
     }
     cluster_arrive();  // (waited for before the first word goes to another block: that block has begun, and its counters are zero)
     pdl_wait();
-    const float temperature = p.temperature ? p.temperature[row] : 1.f;
-    const int k = p.top_k ? p.top_k[row] : 0;
-    const float top_p = p.top_p ? p.top_p[row] : 1.f, min_p = p.min_p ? p.min_p[row] : 0.f;
-    double u = p.uniform[row];
+    const float temperature = p.temperature ? p.temperature[row] : p.same_temperature;
+    const int k = p.top_k ? p.top_k[row] : p.same_top_k;
+    const float top_p = p.top_p ? p.top_p[row] : p.same_top_p, min_p = p.min_p ? p.min_p[row] : p.same_min_p;
+    double u = p.uniform ? p.uniform[row] : p.same_uniform;
 
     // the slice, its maximum and its smallest finite value; no numbers become -inf, which is no choice
     float mx = -INFINITY, mn = INFINITY;

@@ -6,12 +6,14 @@
 #include "host_common.h"
 #include "paged_attention.cuh"
 #include "paged_prefix.cuh"
+#include "serving.h"
 
 using namespace l2b;
 
 namespace {
 
 constexpr int MAX_DEVICES = 64;
+static_assert(SAMPLE_MAX_VOCAB == FS_CLUSTER * FS_SLICE, "what a cluster's shared memory holds");
 
 // The device that a pointer's memory is on is the current one while this lives.
 struct OnDeviceOf {
@@ -368,32 +370,45 @@ extern "C" int32_t l2b_paged_attention_device(const l2b_paged_cache* cache, cons
     return L2B_OK;
 }
 
+// Blocks of a row: as many as keep a slice at 16384 logits (two blocks to an SM), more while SMs would be idle and a slice has work for the block.
+template <typename T>
+static int32_t launch_sample(SampleParams& p, int n_rows, int device, cudaStream_t st) {
+    int sms = 0;
+    L2B_TRY(sm_count(device, &sms));
+    int cluster = 1;
+    while (cluster < FS_CLUSTER && ((p.vocab + cluster - 1) / cluster > 16384 || ((int64_t)n_rows * cluster * 2 <= 2 * sms && p.vocab / cluster >= 4096))) cluster *= 2;
+    p.cluster = cluster;
+    p.slice = ((p.vocab + cluster - 1) / cluster + 7) / 8 * 8;
+    L2B_TRY(allow_smem<filtered_sample_kernel<T>>(device));
+    CU(launch_kernel(filtered_sample_kernel<T>, dim3((unsigned)(n_rows * cluster)), dim3(FS_THREADS), (size_t)p.slice * 4, st, true, p, cluster));
+    return L2B_OK;
+}
+
 extern "C" int32_t l2b_sample_device(const l2b_sampling* a, void* stream) {
     if (!a || !a->dev_logits || !a->dev_tokens || !a->dev_uniform) return fail(L2B_ERR_BAD_ARG, "null argument");
     if (a->type != L2B_TYPE_F32 && a->type != L2B_TYPE_F16 && a->type != L2B_TYPE_BF16) return fail(L2B_ERR_UNSUPPORTED_TYPE, "logits are f32, f16 or bf16");
-    if (a->n_rows < 0 || a->vocab < 1 || a->vocab > FS_CLUSTER * FS_SLICE) return fail(L2B_ERR_BAD_ARG, "bad number of rows, or a vocabulary of more than 393216");
+    if (a->n_rows < 0 || a->vocab < 1 || a->vocab > SAMPLE_MAX_VOCAB) return fail(L2B_ERR_BAD_ARG, "bad number of rows, or a vocabulary of more than 393216");
     if (a->n_rows > 0x7fffffff / FS_CLUSTER) return fail(L2B_ERR_BAD_ARG, "too many rows");
     if (a->stride < a->vocab) return fail(L2B_ERR_BAD_ARG, "rows overlap");
     if (!aligned(a->dev_logits, type_bytes(a->type)) || !aligned(a->dev_tokens, 4) || !aligned(a->dev_uniform, 8)) return fail(L2B_ERR_BAD_ARG, "misaligned pointer");
     OnDeviceOf on;
     L2B_TRY(on.enter(a->dev_logits, "dev_logits"));
     if (a->n_rows == 0) return L2B_OK;
-    int sms = 0;
-    L2B_TRY(sm_count(on.device, &sms));
     SampleParams p;
+    memset(&p, 0, sizeof(p));
     p.logits = a->dev_logits; p.stride = a->stride; p.vocab = a->vocab;
     p.temperature = a->dev_temperature; p.top_p = a->dev_top_p; p.min_p = a->dev_min_p; p.top_k = a->dev_top_k;
+    p.same_temperature = p.same_top_p = 1.f;
     p.uniform = a->dev_uniform; p.tokens = a->dev_tokens; p.probs = a->dev_probs;
-    // Blocks of a row: as many as keep a slice at 16384 logits (two blocks to an SM), more while SMs would be idle and a slice has work for the block.
-    int cluster = 1;
-    while (cluster < FS_CLUSTER && ((a->vocab + cluster - 1) / cluster > 16384 || ((int64_t)a->n_rows * cluster * 2 <= 2 * sms && a->vocab / cluster >= 4096))) cluster *= 2;
-    p.cluster = cluster;
-    p.slice = ((a->vocab + cluster - 1) / cluster + 7) / 8 * 8;
-    auto go = [&](auto t) -> int32_t {
-        using T = decltype(t);
-        L2B_TRY(allow_smem<filtered_sample_kernel<T>>(on.device));
-        CU(launch_kernel(filtered_sample_kernel<T>, dim3((unsigned)(a->n_rows * cluster)), dim3(FS_THREADS), (size_t)p.slice * 4, (cudaStream_t)stream, true, p, cluster));
-        return L2B_OK;
-    };
-    return a->type == L2B_TYPE_F32 ? go(float()) : a->type == L2B_TYPE_F16 ? go(__half()) : go(__nv_bfloat16());
+    cudaStream_t st = (cudaStream_t)stream;
+    return a->type == L2B_TYPE_F32 ? launch_sample<float>(p, a->n_rows, on.device, st)
+                                   : a->type == L2B_TYPE_F16 ? launch_sample<__half>(p, a->n_rows, on.device, st) : launch_sample<__nv_bfloat16>(p, a->n_rows, on.device, st);
+}
+
+int32_t enqueue_filtered_sample(const float* logits, int vocab, float temperature, int top_k, float top_p, float min_p, double uniform, int* token, int device, cudaStream_t st) {
+    SampleParams p;
+    memset(&p, 0, sizeof(p));
+    p.logits = logits; p.stride = vocab; p.vocab = vocab; p.tokens = token;
+    p.same_temperature = temperature; p.same_top_k = top_k; p.same_top_p = top_p; p.same_min_p = min_p; p.same_uniform = uniform;
+    return launch_sample<float>(p, 1, device, st);
 }

@@ -160,6 +160,14 @@ function decode_next(s::B200RunState, token::Int, pos::Int, temperature::Float32
     return Int(next[]) + 1
 end
 
+# A token from the logits the state holds, among those that top_k, top_p and min_p leave (0, 1, 0: no cut).
+function sample_next(s::B200RunState, temperature::Float32, top_k::Int, top_p::Float32, min_p::Float32)
+    next = Ref{Int32}(0)
+    check(ccall((:l2b_session_sample, LIB), Int32, (Ptr{Cvoid}, Float32, Int32, Float32, Float32, Float64, Ref{Int32}),
+                s.session, temperature, top_k, top_p, min_p, temperature == 0f0 ? 0.0 : rand(), next))
+    return Int(next[]) + 1
+end
+
 # The iterations of that loop whose next token is a prompt token (src/inference.jl:349-356), as one call: tokens at
 # positions 1..length(tokens) (the library streams the weights once for two positions where it can).
 function prefill!(s::B200RunState, tokens::Vector{Int})
@@ -172,6 +180,7 @@ end
 # ---- sample ------------------------------------------------------------------------------------------------
 # src/inference.jl:317-395, statement for statement where the device does not change it: same keywords, same printing, same
 # stop rule (a BOS or EOS as the next token ends the loop, prompt tokens included, :371-373), same tok/s line (:391-392).
+# top_k, top_p and min_p, which the package does not have, restrict what is sampled from.
 function sample(
         model::B200LanguageModel,
         prompt::String = "";
@@ -179,6 +188,9 @@ function sample(
         stop_on_special_token = true,
         max_seq_len = typemax(Int),
         bos_token = true,
+        top_k::Int = 0,
+        top_p::Float32 = 1f0,
+        min_p::Float32 = 0f0,
     )
     if !bos_token && isempty(prompt)
         error("Prompt cannot be empty if bos_token = false")
@@ -210,7 +222,12 @@ function sample(
         first_pos = n_forced + 1
     end
     for pos in first_pos:limit
-        next = decode_next(state, token, pos, temperature)
+        if temperature != 0f0 && (top_k > 0 || top_p < 1f0 || min_p > 0f0)
+            transformer!(token, pos, config, state, model.weights)
+            next = sample_next(state, temperature, top_k, top_p, min_p)
+        else
+            next = decode_next(state, token, pos, temperature)
+        end
         generated_seq_len += 1
         if pos + 1 <= length(prompt_tokens)
             next = prompt_tokens[pos + 1]

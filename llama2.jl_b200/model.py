@@ -409,6 +409,15 @@ def prefill(s: RunState, tokens, pos0: int = 0) -> int:
     return nxt.value
 
 
+def sample_next(s: RunState, temperature: float = 1.0, top_k: int = 0, top_p: float = 1.0, min_p: float = 0.0, uniform: float = 0.5) -> int:
+    """A token from the logits the state holds (after transformer_ or prefill), by temperature and among those that three cuts leave: the top_k first
+    (0: all), those before which less than top_p of the mass lies (1: all), those at least min_p times as likely as the likeliest (0: all).  uniform in
+    [0, 1) is the random number."""
+    nxt = C.c_int32()
+    L.check(L.lib().l2b_session_sample(s.session, float(temperature), int(top_k), float(top_p), float(min_p), float(uniform), C.byref(nxt)))
+    return nxt.value
+
+
 def extend(s: RunState, tokens, pos0: int, want=()) -> np.ndarray:
     """A portion of a sequence on top of what the state holds: tokens at positions pos0.., logits [len(want), vocab] at the places
     `want` (ascending, counted within the portion)."""
@@ -435,8 +444,11 @@ def _text(tok) -> str:
 
 
 def sample(model: LanguageModel, prompt: str = "", *, temperature: float = 0.9, stop_on_special_token: bool = True,
-           max_seq_len: int = sys.maxsize, bos_token: bool = True, rng: Optional[random.Random] = None, out=None) -> None:
+           max_seq_len: int = sys.maxsize, bos_token: bool = True, rng: Optional[random.Random] = None, out=None, top_k: int = 0, top_p: float = 1.0,
+           min_p: float = 0.0) -> None:
     """sample(model, prompt; temperature, stop_on_special_token, max_seq_len, bos_token) (src/inference.jl:317-395).
+
+    top_k, top_p and min_p, which the reference does not have, restrict what is sampled from (sample_next).
 
     Prints the text and the achieved tok/s like the reference and returns None.  The prompt positions whose next token is
     a prompt token go through one l2b_prefill call (unless the stop condition could fire among them); every other position
@@ -458,6 +470,7 @@ def sample(model: LanguageModel, prompt: str = "", *, temperature: float = 0.9, 
     generated_seq_len = 0
     lib = L.lib()
     nxt = C.c_int32()
+    cuts = temperature != 0 and (top_k > 0 or top_p < 1 or min_p > 0)
     limit = min(config.seq_len, max_seq_len)
     first = 0
     n_forced = len(prompt_tokens) - 1  # positions 0 .. n_forced-1 are followed by a prompt token
@@ -471,8 +484,12 @@ def sample(model: LanguageModel, prompt: str = "", *, temperature: float = 0.9, 
         token = prompt_tokens[n_forced]
         first = n_forced
     for pos in range(first, limit):
-        L.check(lib.l2b_decode_next(state.session, int(token), pos, float(temperature), rng.random() if temperature != 0 else 0.0,
-                                    C.byref(nxt)))
+        uniform = rng.random() if temperature != 0 else 0.0
+        if cuts:
+            L.check(lib.l2b_forward(state.session, int(token), pos, None))
+            L.check(lib.l2b_session_sample(state.session, float(temperature), int(top_k), float(top_p), float(min_p), uniform, C.byref(nxt)))
+        else:
+            L.check(lib.l2b_decode_next(state.session, int(token), pos, float(temperature), uniform, C.byref(nxt)))
         generated_seq_len += 1
         next_token = prompt_tokens[pos + 1] if pos + 1 < len(prompt_tokens) else nxt.value
         if stop_on_special_token and next_token in (tokenizer.bos_token_id, tokenizer.eos_token_id):
