@@ -331,10 +331,66 @@ def test_f32_queries_over_f16_keys_of_any_size(L, scale):
     check_attention(b, queries(b, 2, "f32", scale=scale), 2, scale=0.3 / scale)
 
 
+@pytest.mark.parametrize("heads", [2, 40, 300])
 @pytest.mark.parametrize("scale", [0.05, -0.2])
-def test_scales(L, scale):
-    b = Batch(L, [70, 3], kv=1, hs=64, page=16, prefix=9)
-    check_attention(b, queries(b, 2, "bf16"), 2, scale=scale)
+def test_scales(L, scale, heads):
+    b = Batch(L, [70, 3], kv=1, hs=64, page=16, prefix=209)
+    check_attention(b, queries(b, heads, "bf16"), heads, scale=scale)
+
+
+@pytest.mark.parametrize("io,cache", TYPES)
+@pytest.mark.parametrize("page", [8, 16, 32, 64, 128, 256, 512, 1024])
+def test_prefixes_in_pages_of_every_size(L, page, io, cache):
+    """Many rows on one prefix: pages smaller and larger than a tile of keys, the prefix's end anywhere in the last one, a hole in the middle."""
+    for prefix, heads in ((page, 20), (2 * page + 1, 130), (3 * page - 1, 300), (1500, 64)):
+        b = Batch(L, [5, 0], kv=2, hs=72, page=page, prefix=prefix, cache=cache, seed=prefix)
+        if prefix == 3 * page - 1:
+            b.prefix_pages[1] = -1
+        check_attention(b, queries(b, heads, io), heads)
+
+
+def test_sequences_that_share_pages_of_their_own(L):
+    """The same pages in several rows of the table."""
+    b = Batch(L, [40, 40, 33], kv=2, hs=64, page=16, prefix=20)
+    b.table[1:] = b.table[0]
+    check_attention(b, queries(b, 4, "bf16"), 4)
+
+
+def test_first_calls_in_a_capture(pkg):
+    """A process whose first calls are captured ones."""
+    import os
+    import subprocess
+    import sys
+    here = os.path.dirname(os.path.abspath(__file__))
+    code = """
+import sys
+sys.path[:0] = [%r, %r]
+import __graft_entry__ as g
+g.load_package()
+from llama2_jl_b200 import _lib as L
+import ctypes as C, torch, test_gpu_paged as T
+b = T.Batch(L, [60, 200, 1, 90], kv=2, hs=128, page=16, prefix=200)
+q = T.queries(b, 32, "bf16")
+out, plan = torch.zeros_like(q), None
+plan = b.plan(q, out, 32)
+x, u, tokens = torch.zeros((3, 5000), device="cuda"), torch.full((3,), 0.5, dtype=torch.float64, device="cuda"), torch.full((3,), -7, dtype=torch.int32, device="cuda")
+a = L.Sampling(type=0, n_rows=3, vocab=5000, dev_logits=T.at(x), stride=5000, dev_uniform=T.at(u), dev_tokens=T.at(tokens))
+rows = torch.ones((4, 256), device="cuda").bfloat16()
+torch.cuda.synchronize()
+graph = torch.cuda.CUDAGraph()
+with torch.cuda.graph(graph):
+    b.append(L.PagedRows(type=30, dev_k=T.at(rows), dev_v=T.at(rows), k_stride=256, v_stride=256, rope_freq_base=1e4))
+    b.attend(plan)
+    L.check(L.lib().l2b_sample_device(C.byref(a), T.stream()))
+graph.replay()
+torch.cuda.synchronize()
+for r, (o, tol) in T.attention_reference(b, q, 32).items():
+    assert ((out[r].double().view(32, 128) - o).abs() <= tol).all()
+assert tokens.tolist() == [2500] * 3
+print("done")
+""" % (here, os.path.dirname(here))
+    r = subprocess.run([sys.executable, "-c", code], capture_output=True, text=True, timeout=300)
+    assert r.returncode == 0 and "done" in r.stdout, r.stdout + r.stderr
 
 
 @pytest.mark.parametrize("n_seq,prefix,most,heads,kv,hs", [(1, 0, 5000, 8, 2, 128), (1, 3000, 1, 8, 2, 128), (70, 900, 90, 8, 2, 64), (40, 0, 2000, 4, 4, 96), (3, 2500, 1500, 32, 1, 64)])
