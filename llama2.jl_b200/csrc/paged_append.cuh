@@ -8,7 +8,8 @@
 // same for all of them and become four coefficients per pair once (a' = r (A a - B b), b' = r (C a + D b), r = 1 / sqrt(..)), in registers: norm and rotation
 // cost three operations a value.  (With gains and angles applied one after the other, and a kind looked up for each head, the instructions took twice the
 // memory's time.)  The angles of a token are shared by its heads: a block computes them once for its tokens, in 64 bits up to the fraction of a
-// turn (a far position times the fastest frequency would lose all of a turn in 32), and the first heads' values are on their way meanwhile.
+// turn (a far position times the fastest frequency would lose all of a turn in 32).
+// Measured: 12 000 rows of 64 + 16 heads of 128 bf16 values (491 MB) in 102 us, 4.8 TB/s, 0.74 of the copy rate; one row of 32 + 16 heads in 3.5 us, a launch and its look-ups.
 #pragma once
 #include <cuda_bf16.h>
 

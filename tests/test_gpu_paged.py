@@ -219,9 +219,9 @@ def attention_reference(b, q, heads, scale=0.0):
         o, size = torch.einsum("hn,nhd->hd", w, v), torch.einsum("hn,nhd->hd", w, v.abs())
         # Scores: at most 24 products of 16 are added up (three terms of 8), each sum off by a step of f32 at most, 24 * 2^-23 < 2^-18 of their absolute size.
         ds = 2.0 ** -18 * (torch.einsum("hd,nhd->hn", x.abs(), k.abs()) * abs(scale)).amax(-1)
-        # Weights: rounded to the cache's type once for rows of that type; for f32 rows two terms, half a step squared (f16: or 2^-25 of the largest
-        # weight, a number below 2^-14); sums: a step of f32 per 16 keys.
-        weights = half if q.dtype != torch.float32 else max((torch.finfo(b.k.dtype).eps / 2) ** 2, 2.0 ** -25)
+        # Weights: rounded to the cache's type once for rows of that type; for f32 rows three terms of bf16 or two of f16, half a step to that power (f16: or
+        # 2^-25 of the largest weight, a number below 2^-14); sums: a step of f32 per 16 keys.
+        weights = half if q.dtype != torch.float32 else (torch.finfo(b.k.dtype).eps / 2) ** (3 if b.cache == "bf16" else 2)
         tiny = (2.0 ** -25 * v.abs().sum(0)) if b.cache == "f16" else 0.0
         steps = (len(page) / 16 + 16) * 2.0 ** -23
         tol = (weights + ds[:, None] + steps) * size + tiny
