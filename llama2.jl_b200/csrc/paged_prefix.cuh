@@ -6,14 +6,16 @@
 //   TILES = 2: the streams are two row tiles that share the tiles of keys (128 each);
 //   TILES = 1: one row tile, the streams take the tiles of keys in turn and leave a partial result each: for few rows, and for f32 rows, whose three (f16: two)
 //              terms of Q take the place of a second tile (64 keys a tile).
-// A thread takes its row of scores to registers at once and hands P over in two halves, so that P V begins beside the second half's exponentials.  (Measured and not kept: two buffers of 64 keys per stream, Q K^T a step ahead; a product of 64 columns
-// takes as long as one of 128.)
+// The scores come in steps of 64 keys.  16-bit rows have two buffers of them, so that the next step's Q K^T is done before this step's exponentials are: with one
+// buffer of 128 keys a stream waited 2000 of 3900 cycles per tile for its products, and attention behind 16 000 positions took 128 us instead of 116.
 //   warps 0-3, 4-7  the streams' softmax; before it they bring the block's rows of Q into shared memory, after it the sums to the workspace
-//   warps 8, 10     issue a stream's products each: P V of a tile, then Q K^T of the stream's next, which overwrites that P
+//   warps 8, 10     issue a stream's products each: P V of a step, then Q K^T of the step that gets its buffer
 //   warp 9          TMA copies of keys and values straight from the pages: 8 rows or more at a time, V's rows behind the prefix's end through a map
 //                   that ends there, so that they are zeros; pages that are none lie outside the map and are zeros, too
 // Rows are rescaled only when a maximum has grown by more than 2^8.  The work, items (key/value head, row tile) of the prefix' key tiles, is cut
 // into equal shares of a block per SM (paged.h).  Every wait is bounded; a block whose wait ran out leaves NaN.
+// Measured: 128 rows of 64 heads over 8 x 16 000 keys of 128 values (65.5 GFLOP) in about 72 us of the 116, 0.9 PFLOP/s; bound by the chain scores - maximum - exponentials of
+// a stream and the exponentials' rate.
 #pragma once
 #include "paged_attention.cuh"
 #include "tcgen05.cuh"
@@ -36,7 +38,7 @@ template <typename T, typename TIO, int TILES>
 struct PrefixTraits {
     static constexpr bool WIDE = sizeof(TIO) == 4, F16 = std::is_same<T, __half>::value;
     static constexpr int QT = !WIDE ? 1 : F16 ? 2 : 3, PT = QT;
-    static constexpr int KEYS = WIDE ? 64 : 128, HALVES = KEYS / 64;
+    static constexpr int KEYS = WIDE ? 64 : 128, STEPS = KEYS / 64, BUFFERS = STEPS;  // steps of 64 keys of a tile, buffers of a stream's scores
     static constexpr int SUB_Q = PX_ROWS * 128, SUB_K = KEYS * 128;  // bytes of 64 values of a tile's rows
     // bytes of Q's place: its terms, or 4 KB for each of the eight warps that take the sums out
     __host__ __device__ static constexpr int queries(int nd) { return QT * TILES * nd * SUB_Q > 8 * 4096 ? QT * TILES * nd * SUB_Q : 8 * 4096; }
@@ -133,7 +135,7 @@ __global__ void __launch_bounds__(PX_THREADS, 1) paged_prefix_kernel(const __gri
     using TR = PrefixTraits<T, TIO, TILES>;
     constexpr int KEYS = TR::KEYS;
     extern __shared__ __align__(1024) uint8_t px_raw[];
-    __shared__ __align__(8) uint64_t s_kfull[PX_MAX_STAGES], s_kfree[PX_MAX_STAGES], s_vfull[PX_MAX_STAGES], s_vfree[PX_MAX_STAGES], s_mask[PX_RING], s_q, s_seg, s_s[2], s_p[2][2];  // s_p: of each half
+    __shared__ __align__(8) uint64_t s_kfull[PX_MAX_STAGES], s_kfree[PX_MAX_STAGES], s_vfull[PX_MAX_STAGES], s_vfree[PX_MAX_STAGES], s_mask[PX_RING], s_q, s_seg, s_s[2][2], s_p[2][2], s_o[2];  // s_s, s_p: of each buffer (a stream's softmax may be two steps ahead of its P V)
     __shared__ uint32_t s_tmem, s_valid[PX_RING][4];
     __shared__ int s_exp[TILES * PX_ROWS];
     uint8_t* const smem = px_raw + ((1024u - (smem_u32(px_raw) & 1023u)) & 1023u);
@@ -152,7 +154,9 @@ __global__ void __launch_bounds__(PX_THREADS, 1) paged_prefix_kernel(const __gri
         mbar_init(&s_q, 8);
         mbar_init(&s_seg, 2);
         for (int i = 0; i < 2; ++i) {
-            mbar_init(s_s + i, 1);
+            mbar_init(&s_s[i][0], 1);
+            mbar_init(&s_s[i][1], 1);
+            mbar_init(s_o + i, 1);
             mbar_init(&s_p[i][0], 4);
             mbar_init(&s_p[i][1], 4);
         }
@@ -239,7 +243,7 @@ __global__ void __launch_bounds__(PX_THREADS, 1) paged_prefix_kernel(const __gri
         // that had the loop for itself a product took 110 cycles to issue, twice its length.)
         const int i = warp == 8 ? 0 : 1;
         const bool leader = elect_one();
-        const uint32_t idesc_s = TR::idesc(KEYS, 0), idesc_o = TR::idesc(vn, 1), stage_step = (uint32_t)(nd * TR::SUB_K) >> 4;
+        const uint32_t idesc_s = TR::idesc(64, 0), idesc_o = TR::idesc(vn, 1), stage_step = (uint32_t)(nd * TR::SUB_K) >> 4;
         const uint64_t desc_q = umma_desc_sw128(sq + (TILES == 2 ? i : 0) * nd * TR::SUB_Q, 0), desc_k = umma_desc_sw128(sk, 0), desc_v = umma_desc_sw128_mn(sv, 0, TR::SUB_K);
         const uint32_t ds = tmem + (uint32_t)(i * 128), dout = tmem + 256 + (uint32_t)(i * 128);
         bool ok = true;
@@ -248,7 +252,7 @@ __global__ void __launch_bounds__(PX_THREADS, 1) paged_prefix_kernel(const __gri
             int stage;
             uint32_t phase;
         } k = {0, 0}, v = {0, 0};
-        uint32_t p_phase = 0;
+        uint32_t before = 0;  // steps of the segments before
         auto advance = [&](Place& at) {
 #pragma unroll
             for (int j = 0; j < (TILES == 2 ? 1 : 2); ++j)
@@ -257,11 +261,13 @@ __global__ void __launch_bounds__(PX_THREADS, 1) paged_prefix_kernel(const __gri
                     at.phase ^= 1u;
                 }
         };
-        auto qk = [&]() {  // scores of the next tile
-            ok = __all_sync(0xffffffffu, mbar_wait_bounded(s_kfull + k.stage, k.phase));
+        auto qk = [&](uint32_t n) {  // scores of step n
+            const uint32_t buffer = (before + n) % TR::BUFFERS, half = n % TR::STEPS;
+            if (half == 0) ok = __all_sync(0xffffffffu, mbar_wait_bounded(s_kfull + k.stage, k.phase));
             if (!ok) return;
             tc_fence_after();
-            const uint64_t kd = desc_k + (uint32_t)k.stage * stage_step;
+            const uint64_t kd = desc_k + (uint32_t)k.stage * stage_step + half * (64 * 128 >> 4);
+            const uint32_t d = ds + buffer * 64;
 #pragma unroll
             for (int t = TR::QT - 1; t >= 0; --t) {  // (small terms first)
                 const uint64_t qd = desc_q + (uint32_t)(t * TILES * nd) * (uint32_t)(TR::SUB_Q >> 4);
@@ -270,48 +276,48 @@ __global__ void __launch_bounds__(PX_THREADS, 1) paged_prefix_kernel(const __gri
                     if (sub < nd && leader) {  // (values behind a head's end are zeros)
 #pragma unroll
                         for (int kk = 0; kk < 4; ++kk)
-                            umma_f16(ds, qd + (uint32_t)(sub * (TR::SUB_Q >> 4) + kk * 2), kd + (uint32_t)(sub * (TR::SUB_K >> 4) + kk * 2), idesc_s, t == TR::QT - 1 && sub == 0 && kk == 0 ? 0u : 1u);
+                            umma_f16(d, qd + (uint32_t)(sub * (TR::SUB_Q >> 4) + kk * 2), kd + (uint32_t)(sub * (TR::SUB_K >> 4) + kk * 2), idesc_s, t == TR::QT - 1 && sub == 0 && kk == 0 ? 0u : 1u);
                     }
             }
-            if (leader) {
-                umma_commit(s_s + i);
-                umma_commit(s_kfree + k.stage);
+            if (leader) umma_commit(&s_s[i][buffer]);
+            if (half == TR::STEPS - 1) {
+                if (leader) umma_commit(s_kfree + k.stage);
+                advance(k);
             }
-            advance(k);
         };
-        auto pv = [&](bool first) {
-            const uint64_t vd = desc_v + (uint32_t)v.stage * stage_step;
-            ok = __all_sync(0xffffffffu, mbar_wait_bounded(s_vfull + v.stage, v.phase));
+        auto pv = [&](uint32_t n) {
+            const uint32_t c = before + n, buffer = c % TR::BUFFERS, half = n % TR::STEPS;
+            const uint64_t vd = desc_v + (uint32_t)v.stage * stage_step + half * (64 * 128 >> 4);
+            const uint32_t a = ds + buffer * 64;
+            if (half == 0) ok = __all_sync(0xffffffffu, mbar_wait_bounded(s_vfull + v.stage, v.phase));
+            if (ok) ok = __all_sync(0xffffffffu, mbar_wait_bounded(&s_p[i][buffer], c / TR::BUFFERS & 1u));
+            if (!ok) return;
+            tc_fence_after();
+            if (leader) {
 #pragma unroll
-            for (int half = 0; half < TR::HALVES; ++half) {
-                if (ok) ok = __all_sync(0xffffffffu, mbar_wait_bounded(&s_p[i][half], p_phase));
-                if (!ok) return;
-                tc_fence_after();
-                if (leader) {
+                for (int t = TR::PT - 1; t >= 0; --t)
 #pragma unroll
-                    for (int t = TR::PT - 1; t >= 0; --t)
-#pragma unroll
-                        for (int kk = 0; kk < 4; ++kk)
-                            umma_f16_at(dout, ds + (uint32_t)(t * 32 + half * 32 + kk * 8), vd + (uint32_t)((half * 4 + kk) * (2048 >> 4)), idesc_o,
-                                        half > 0 || t < TR::PT - 1 || kk > 0 ? 1u : first ? 0u : 1u);
-                }
+                    for (int kk = 0; kk < 4; ++kk)
+                        umma_f16_at(dout, a + (uint32_t)(t * 32 + kk * 8), vd + (uint32_t)(kk * (2048 >> 4)), idesc_o, t < TR::PT - 1 || kk > 0 ? 1u : n > 0 ? 1u : 0u);
+                umma_commit(s_o + i);
             }
-            p_phase ^= 1u;
-            if (leader) umma_commit(s_vfree + v.stage);
-            advance(v);
+            if (half == TR::STEPS - 1) {
+                if (leader) umma_commit(s_vfree + v.stage);
+                advance(v);
+            }
         };
         for (int64_t u = begin; u < end && ok; ++segment) {
             const int item = (int)(u / p.cut.tiles), tiles = (int)min((int64_t)p.cut.tiles - (u - (int64_t)item * p.cut.tiles), end - u);
-            const int n = TILES == 2 ? tiles : (tiles + 1 - i) / 2;  // of this stream
+            const uint32_t n = (uint32_t)(TR::STEPS * (TILES == 2 ? tiles : (tiles + 1 - i) / 2));  // steps of this stream
             const int first = TILES == 2 ? g : g + i;
             k = v = {first % p.stages, (uint32_t)(first / p.stages & 1)};
             ok = __all_sync(0xffffffffu, mbar_wait_bounded(&s_q, (uint32_t)(segment & 1)));
-            if (ok && n > 0) qk();
 #pragma unroll 1
-            for (int t = 0; t < n && ok; ++t) {
-                pv(t == 0);
-                if (ok && t + 1 < n) qk();
+            for (uint32_t t = 0; t < n + TR::BUFFERS && ok; ++t) {  // P V of a step, then Q K^T of the one that gets its buffer
+                if (t >= TR::BUFFERS) pv(t - TR::BUFFERS);
+                if (ok && t < n) qk(t);
             }
+            before += n;
             if (ok && leader) umma_commit(&s_seg);
             g += tiles;
             u += tiles;
@@ -339,48 +345,45 @@ __global__ void __launch_bounds__(PX_THREADS, 1) paged_prefix_kernel(const __gri
             for (int t = TILES == 2 ? 0 : i; t < n; t += TILES == 2 ? 1 : 2) {
                 const int gt = g + t;
                 if (ok) ok = __all_sync(0xffffffffu, mbar_wait_bounded(s_mask + gt % PX_RING, (uint32_t)(gt / PX_RING & 1)));
-                if (ok) ok = __all_sync(0xffffffffu, mbar_wait_bounded(s_s + i, (uint32_t)(ns & 1)));  // (P V of the tile before is done then, too)
-                ++ns;
-                tc_fence_after();
-                float x[KEYS];
-#pragma unroll
-                for (int c = 0; c < KEYS; c += 64) tmem_load(ts + (uint32_t)c, *reinterpret_cast<float(*)[64]>(x + c));
-                uint32_t there[KEYS / 32], all = ~0u;
-#pragma unroll
-                for (int c = 0; c < KEYS / 32; ++c) {
-                    there[c] = s_valid[gt % PX_RING][c];
-                    all &= there[c];
-                }
-                if (all != ~0u) {
-#pragma unroll
-                    for (int k = 0; k < KEYS; ++k) x[k] = there[k >> 5] >> (k & 31) & 1 ? x[k] : -INFINITY;
-                }
-                float m4[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
-#pragma unroll
-                for (int k = 0; k < KEYS; k += 2) m4[k >> 1 & 3] = fmaxf(fmaxf(x[k], x[k + 1]), m4[k >> 1 & 3]);
-                const float mx = fmaxf(fmaxf(m4[0], m4[1]), fmaxf(m4[2], m4[3])) * sc;
-                if (!some) {
-                    m = mx;
-                } else if (__any_sync(0xffffffffu, mx > m + 8.f)) {
-                    const float mn = mx > m + 8.f ? mx : m, corr = m == -INFINITY ? 0.f : exp2_approx(m - mn);  // (a row that has seen nothing has sums of zero)
-                    l *= corr;
-                    m = mn;
 #pragma unroll 1
-                    for (int c = 0; c < vn; c += 16) {
-                        float o[16];
-                        tmem_ld16f(to + (uint32_t)c, o);
+                for (int step = 0; step < TR::STEPS; ++step, ++ns) {
+                    const int buffer = ns % TR::BUFFERS;
+                    const uint32_t tb = ts + (uint32_t)(buffer * 64);
+                    if (ok) ok = __all_sync(0xffffffffu, mbar_wait_bounded(&s_s[i][buffer], (uint32_t)(ns / TR::BUFFERS & 1)));
+                    tc_fence_after();
+                    float x[64];
+                    tmem_load(tb, x);
+                    const uint32_t v0 = s_valid[gt % PX_RING][2 * step], v1 = s_valid[gt % PX_RING][2 * step + 1];
+                    if ((v0 & v1) != ~0u) {
 #pragma unroll
-                        for (int e = 0; e < 16; ++e) o[e] *= corr;
-                        tmem_st16f(to + (uint32_t)c, o);
+                        for (int k = 0; k < 64; ++k) x[k] = (k < 32 ? v0 : v1) >> (k & 31) & 1 ? x[k] : -INFINITY;
                     }
-                }
-                some = true;
-                const float use = m == -INFINITY ? 0.f : m;
-                float l4[4] = {0.f, 0.f, 0.f, 0.f};
+                    float m4[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
 #pragma unroll
-                for (int half = 0; half < TR::HALVES; ++half) {
+                    for (int k = 0; k < 64; k += 2) m4[k >> 1 & 3] = fmaxf(fmaxf(x[k], x[k + 1]), m4[k >> 1 & 3]);
+                    const float mx = fmaxf(fmaxf(m4[0], m4[1]), fmaxf(m4[2], m4[3])) * sc;
+                    if (!some) {
+                        m = mx;
+                    } else if (__any_sync(0xffffffffu, mx > m + 8.f)) {
+                        const float mn = mx > m + 8.f ? mx : m, corr = m == -INFINITY ? 0.f : exp2_approx(m - mn);  // (a row that has seen nothing has sums of zero)
+                        l *= corr;
+                        m = mn;
+                        if (ok) ok = __all_sync(0xffffffffu, mbar_wait_bounded(s_o + i, (uint32_t)((ns - 1) & 1)));  // the sums of the step before are there
+                        tc_fence_after();
+#pragma unroll 1
+                        for (int c = 0; c < vn; c += 16) {
+                            float o[16];
+                            tmem_ld16f(to + (uint32_t)c, o);
 #pragma unroll
-                    for (int k = half * 64; k < half * 64 + 64; ++k) {
+                            for (int e = 0; e < 16; ++e) o[e] *= corr;
+                            tmem_st16f(to + (uint32_t)c, o);
+                        }
+                    }
+                    some = true;
+                    const float use = m == -INFINITY ? 0.f : m;
+                    float l4[4] = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+                    for (int k = 0; k < 64; ++k) {
                         x[k] = exp2_approx(fmaf(x[k], sc, -use));
                         l4[k & 3] += x[k];
                     }
@@ -388,16 +391,15 @@ __global__ void __launch_bounds__(PX_THREADS, 1) paged_prefix_kernel(const __gri
                     for (int t2 = 0; t2 < TR::PT; ++t2) {
                         uint32_t w[32];
 #pragma unroll
-                        for (int k = 0; k < 32; ++k)
-                            w[k] = TR::PT == 1 ? pair_of<T>(x[half * 64 + 2 * k], x[half * 64 + 2 * k + 1]) : split_pair<T>(x[half * 64 + 2 * k], x[half * 64 + 2 * k + 1]);
-                        tmem_st32u(ts + (uint32_t)((t2 + half) * 32), w);  // (in the place of the scores, which have been read)
+                        for (int k = 0; k < 32; ++k) w[k] = TR::PT == 1 ? pair_of<T>(x[2 * k], x[2 * k + 1]) : split_pair<T>(x[2 * k], x[2 * k + 1]);
+                        tmem_st32u(tb + (uint32_t)(t2 * 32), w);  // (in the place of the scores, which have been read)
                     }
+                    l += (l4[0] + l4[1]) + (l4[2] + l4[3]);
                     tmem_wait_st();
                     tc_fence_before();
                     __syncwarp();
-                    if (lane == 0) mbar_arrive(&s_p[i][half]);
+                    if (lane == 0) mbar_arrive(&s_p[i][buffer]);
                 }
-                l += (l4[0] + l4[1]) + (l4[2] + l4[3]);
             }
             // the segment's products are all done: this row's sums to the workspace
             if (ok) ok = __all_sync(0xffffffffu, mbar_wait_bounded(&s_seg, (uint32_t)(segment & 1)));
