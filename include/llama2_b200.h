@@ -299,7 +299,7 @@ int32_t l2b_sample_temperature(const float* host_logits, int64_t n, float temper
  * For callers that keep their sequences' keys and values themselves, in pages, and may let all of them begin with the same positions (a system
  * prompt, a document) that are stored once.  All buffers are device memory of the caller's and all of one device, which need not be the current one; the
  * calls allocate nothing, are asynchronous on `stream` (cudaStream_t; NULL = default) and may be captured into a graph.  The descriptors are read
- * during the call only; what their pointers point to is read when the kernels run, so a captured call serves other lengths and pages later.
+ * during the call only; what their pointers point to is read while the kernels run, so it must not change then, and a captured call serves other lengths and pages later.
  *
  * Pages: dev_k, dev_v [n_pages][n_kv_heads][page_size][head_size]. */
 typedef struct l2b_paged_cache {

@@ -62,7 +62,7 @@ struct SampleShared {
     uint32_t listed[3];             // of the first block: where the next keys go
     // found by one thread, used by all
     float own_tau;
-    uint32_t survivors, base, usable;
+    uint32_t survivors, base;
     int bin;
     uint64_t before, found;
 };
@@ -187,7 +187,7 @@ __global__ void __launch_bounds__(FS_THREADS, 2) filtered_sample_kernel(const __
     for (int i = tid; i < FS_BINS; i += FS_THREADS) s.low[i] = s.high[i] = 0;
     if (tid < 3) s.listed[tid] = 0;
     if (tid == 0) {
-        s.survivors = s.usable = 0;
+        s.survivors = 0;
         s.own_tau = -INFINITY;
     }
     cluster_arrive();  // (waited for before the first word goes to another block: that block has begun, and its counters are zero)

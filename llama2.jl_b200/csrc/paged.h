@@ -81,7 +81,7 @@ struct PagedWork {
     PagedSeqs seqs;
     int group;  // query heads of a key/value head
     int thin_prefix;
-    int tile_rows;  // 8 or 16
+    int tile_shift;  // a tile has 8 rows or 16
 };
 struct GroupShape {
     int keys, tiles, row_tiles;
@@ -90,8 +90,8 @@ L2B_HD GroupShape group_shape(const PagedWork& p, int g, int length) {  // lengt
     GroupShape s;
     const bool pre = p.thin_prefix && g == 0;
     s.keys = pre ? p.seqs.prefix_len : paged_keys(length, p.seqs.width, p.pool.page_shift);
-    s.row_tiles = (int)(((int64_t)(pre ? p.seqs.n_seq : 1) * p.seqs.n_query * p.group + p.tile_rows - 1) / p.tile_rows);
-    s.tiles = (int)(((int64_t)s.keys + PT_KEYS - 1) / PT_KEYS);
+    s.row_tiles = (int)(((int64_t)(pre ? p.seqs.n_seq : 1) * p.seqs.n_query * p.group + (1 << p.tile_shift) - 1) >> p.tile_shift);
+    s.tiles = s.keys / PT_KEYS + (s.keys % PT_KEYS != 0);
     return s;
 }
 L2B_HD int group_length(const PagedWork& p, int g) { return p.thin_prefix && g == 0 ? 0 : p.seqs.lengths[g - p.thin_prefix]; }
@@ -108,8 +108,13 @@ L2B_HD Cursor cursor_at(const PagedWork& p, int g, const GroupShape& s, int64_t 
     Cursor c;
     c.g = g;
     c.s = s;
-    c.item = (int)(unit_of_group / s.tiles);
-    c.tile = (int)(unit_of_group % s.tiles);
+    if (unit_of_group <= 0xffffffffll) {  // (as above: no 64-bit division where none is needed)
+        c.item = (int)((uint32_t)unit_of_group / (uint32_t)s.tiles);
+        c.tile = (int)((uint32_t)unit_of_group - (uint32_t)c.item * (uint32_t)s.tiles);
+    } else {
+        c.item = (int)(unit_of_group / s.tiles);
+        c.tile = (int)(unit_of_group % s.tiles);
+    }
     c.left = left;
     return c;
 }

@@ -33,7 +33,7 @@ struct PagedAttnParams : PagedWork {
     float scale2;          // scale * log2(e)
     int64_t* starts;            // [groups + 1]: first unit of each group, left by the own parts' kernel for the joining one
     int workers;                // warps of the own parts' kernel
-    int slot_rows;              // rows of a slot: tile_rows, or fewer when no tile has as many
+    int slot_rows;              // rows of a slot: a tile's, or fewer when no tile has as many
     float *slot_acc, *slot_ml;  // [2 * workers][slot_rows][hs], [..][2]
     float *own_acc, *own_ml;    // items that one warp did: [rows * n_heads][hs], [..][2]; null where nothing else is to be joined
     float *pre_acc, *pre_ml;    // the same of the prefix
@@ -444,7 +444,7 @@ __global__ void __launch_bounds__(PT_WARPS * 32, (ThinTraits<T, TIO, KS, NT>::BL
 // lie along the head's values and add the parts up, so that the loads of many parts are under way at once.  Several warps share a row where there are few.
 struct JoinParams {
     PagedAttnParams a;
-    int heads;  // of a block
+    int heads;  // of a block: PJ_WARPS, or 1
 };
 constexpr int PJ_WARPS = 8;
 
@@ -455,7 +455,7 @@ __global__ void __launch_bounds__(PJ_WARPS * 32) paged_join_kernel(const __grid_
     const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, hs = p.pool.hs;
     const uint32_t tok = blockIdx.x, seq = tok / (uint32_t)p.seqs.n_query, j = tok - seq * (uint32_t)p.seqs.n_query, group = seq + p.thin_prefix;
     const int length = p.seqs.lengths[seq], count = paged_count(length, p.seqs.counts ? p.seqs.counts[seq] : p.seqs.n_query, p.seqs.n_query);
-    const int per_row_shift = jp.heads == 8 ? 0 : jp.heads == 2 ? 2 : 3, per_row = 1 << per_row_shift, head = blockIdx.y * jp.heads + (warp >> per_row_shift), sub = warp & (per_row - 1);
+    const int per_row_shift = jp.heads == PJ_WARPS ? 0 : 3, per_row = 1 << per_row_shift, head = blockIdx.y * jp.heads + (warp >> per_row_shift), sub = warp & (per_row - 1);
     const bool real = head < p.n_heads;
     const uint32_t kv = (uint32_t)head / (uint32_t)p.group;
     const int g = head - (int)kv * p.group, d = lane * 4;
@@ -463,7 +463,7 @@ __global__ void __launch_bounds__(PJ_WARPS * 32) paged_join_kernel(const __grid_
 
     // the parts of this row: of the prefix's kernel, of the prefix as a group of the own parts' kernel, of the own positions
     const GroupShape own = group_shape(p, group, length), pre = group_shape(p, 0, length);
-    const uint32_t own_row = j * p.group + g, pre_row = tok * p.group + g, tile_shift = p.tile_rows == 8 ? 3 : 4, tile_mask = p.tile_rows - 1;
+    const uint32_t own_row = j * p.group + g, pre_row = tok * p.group + g, tile_shift = p.tile_shift, tile_mask = (1u << p.tile_shift) - 1u;
     const int item_shift = p.cut.streams_share == 2 ? 8 : 7, stream_shift = p.cut.streams_share == 2 ? 0 : 1;
     PagedParts of[3] = {};
     int n_parts[3] = {};

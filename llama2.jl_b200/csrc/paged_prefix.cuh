@@ -14,7 +14,7 @@
 //                   that ends there, so that they are zeros; pages that are none lie outside the map and are zeros, too
 // Rows are rescaled only when a maximum has grown by more than 2^8.  The work, items (key/value head, row tile) of the prefix' key tiles, is cut
 // into equal shares of a block per SM (paged.h).  Every wait is bounded; a block whose wait ran out leaves NaN.
-// Measured: 128 rows of 64 heads over 8 x 16 000 keys of 128 values (65.5 GFLOP) in about 72 us of the 116, 0.9 PFLOP/s; bound by the chain scores - maximum - exponentials of
+// Measured: 128 rows of 64 heads over 8 x 16 000 keys of 128 values (65.5 GFLOP) in 77 us of the 116, 0.86 PFLOP/s; bound by the chain scores - maximum - exponentials of
 // a stream and the exponentials' rate.
 #pragma once
 #include "paged_attention.cuh"

@@ -298,7 +298,7 @@ extern "C" int32_t l2b_paged_attention_device(const l2b_paged_cache* cache, cons
     p.cut = plan.cut;
     p.workers = plan.blocks * PT_WARPS;
     p.slot_rows = plan.slot_rows;
-    p.tile_rows = plan.tile_rows;
+    p.tile_shift = plan.tile_rows == 8 ? 3 : 4;
     p.starts = (int64_t*)dev_workspace;
     float* const w = (float*)dev_workspace + plan.starts;
     const int64_t n_rows = (int64_t)p.seqs.n_seq * p.seqs.n_query * p.n_heads;
@@ -362,7 +362,9 @@ extern "C" int32_t l2b_paged_attention_device(const l2b_paged_cache* cache, cons
         L2B_TRY(plan.tile_rows == 8 ? size(std::integral_constant<int, 1>()) : size(std::integral_constant<int, 2>()));
         JoinParams j;
         j.a = p;
-        j.heads = n_rows >= 4096 ? 8 : n_rows >= 1024 ? 2 : 1;
+        // A warp per row once there are rows for a few warps on every SM, else the block's eight share one.  (2 048 rows: 58 us of a call with a warp each, 59 with four;
+        // 8 192 rows: 116 with one, 134 with four; one row's 16 parts want them.)
+        j.heads = n_rows >= 1024 ? PJ_WARPS : 1;
         const dim3 grid((unsigned)(p.seqs.n_seq * p.seqs.n_query), (unsigned)((p.n_heads + j.heads - 1) / j.heads));
         CU(launch_kernel(paged_join_kernel<TIO>, grid, dim3(PJ_WARPS * 32), 0, st, true, j));
         return L2B_OK;

@@ -100,7 +100,7 @@ extern "C" long long walk(const int* lengths, int n_seq, int n_query, int width,
     w.seqs = {lengths, nullptr, nullptr, nullptr, n_seq, n_query, width, prefix_len};
     w.group = group;
     w.thin_prefix = thin_prefix;
-    w.tile_rows = tile_rows;
+    w.tile_shift = tile_rows == 8 ? 3 : 4;
     const int groups = n_seq + thin_prefix;
     std::vector<long long> first(groups + 1, 0);
     for (int g = 0; g < groups; ++g) first[g + 1] = first[g] + group_units(w, group_shape(w, g));
