@@ -14,8 +14,9 @@
 // positions: 7.6 us and 3.8 for the join, chains of look-ups.
 //
 // f32 rows over a 16-bit cache: a query and a weight are split into terms of the cache's type (three of bf16, two of f16, the query's behind a power of two
-// per row), which keeps the products' error at 2^-22 or less.  For 16-bit rows the weights are rounded once to the cache's type (at most
-// half a step of 2^-8 or 2^-11 relative, as the result itself is); scores, maxima, totals and sums are f32.
+// per row), which keeps the products' error at 2^-22 or less.  For 16-bit rows a weight is two terms (bf16: off by 2^-15 at most, f16: by 2^-22): rounded once
+// to the cache's type, weights put the results 0.0022 from the definition's (2-norms, bf16) where the rounding of a result itself is 0.0016.  Scores, maxima, totals and
+// sums are f32.
 #pragma once
 #include <type_traits>
 
@@ -78,11 +79,6 @@ __device__ __forceinline__ uint32_t transposed(uint32_t v) {
 }
 // Two values as a pair of T, and what that leaves of them.
 template <typename T>
-__device__ __forceinline__ uint32_t pair_of(float a, float b) {
-    const Pack<T, 2> v = {{from_f32<T>(a), from_f32<T>(b)}};
-    return *reinterpret_cast<const uint32_t*>(&v);
-}
-template <typename T>
 __device__ __forceinline__ uint32_t split_pair(float& a, float& b) {
     const T x = from_f32<T>(a), y = from_f32<T>(b);
     const Pack<T, 2> v = {{x, y}};
@@ -95,7 +91,7 @@ __device__ __forceinline__ uint32_t split_pair(float& a, float& b) {
 template <typename T, typename TIO, int KS, int NT>
 struct ThinTraits {
     static constexpr bool WIDE = sizeof(TIO) == 4;
-    static constexpr int QT = !WIDE ? 1 : std::is_same<T, __half>::value ? 2 : 3, PT = QT;
+    static constexpr int QT = !WIDE ? 1 : std::is_same<T, __half>::value ? 2 : 3, PT = WIDE ? QT : 2;  // terms of queries and of weights
     static constexpr int STAGES = NT == 1 ? 2 : 3, BLOCKS = NT == 1 ? 3 : 2;  // 12 warps of 168 registers on an SM, or 8 of 255
     static constexpr int PITCH = KS * 32 + 16;               // bytes of a row in shared memory
     static constexpr int HALF_STAGE = PT_KEYS * PITCH;       // keys of a stage, or values

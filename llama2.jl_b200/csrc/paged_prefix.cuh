@@ -37,7 +37,7 @@ struct PrefixParams : PagedWork {
 template <typename T, typename TIO, int TILES>
 struct PrefixTraits {
     static constexpr bool WIDE = sizeof(TIO) == 4, F16 = std::is_same<T, __half>::value;
-    static constexpr int QT = !WIDE ? 1 : F16 ? 2 : 3, PT = QT;
+    static constexpr int QT = !WIDE ? 1 : F16 ? 2 : 3, PT = WIDE ? QT : 2;  // terms of Q and of P
     static constexpr int KEYS = WIDE ? 64 : 128, STEPS = KEYS / 64, BUFFERS = STEPS;  // steps of 64 keys of a tile, buffers of a stream's scores
     static constexpr int SUB_Q = PX_ROWS * 128, SUB_K = KEYS * 128;  // bytes of 64 values of a tile's rows
     // bytes of Q's place: its terms, or 4 KB for each of the eight warps that take the sums out
@@ -47,7 +47,7 @@ struct PrefixTraits {
         return (1u << 4) | (F16 ? 0u : (1u << 7) | (1u << 10)) | ((uint32_t)b_mn << 16) | ((uint32_t)(n >> 3) << 17) | ((uint32_t)(PX_ROWS >> 4) << 24);
     }
 };
-// 64 consecutive columns of this thread's tensor-memory lane, and a store of 32
+// 64 consecutive columns of this thread's tensor-memory lane
 __device__ __forceinline__ void tmem_load(uint32_t taddr, float (&v)[64]) {
     asm volatile(
         "tcgen05.ld.sync.aligned.32x32b.x64.b32 {"
@@ -63,15 +63,20 @@ __device__ __forceinline__ void tmem_load(uint32_t taddr, float (&v)[64]) {
         : "r"(taddr)
         : "memory");
 }
-__device__ __forceinline__ void tmem_st32u(uint32_t taddr, const uint32_t (&v)[32]) {
-    asm volatile(
-        "tcgen05.st.sync.aligned.32x32b.x32.b32 [%0], {"
-        "%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15,%16,%17,%18,%19,%20,%21,%22,%23,%24,%25,%26,%27,%28,%29,%30,%31,%32"
-        "};" ::"r"(taddr),
-        "r"(v[0]), "r"(v[1]), "r"(v[2]), "r"(v[3]), "r"(v[4]), "r"(v[5]), "r"(v[6]), "r"(v[7]), "r"(v[8]), "r"(v[9]), "r"(v[10]), "r"(v[11]),
-        "r"(v[12]), "r"(v[13]), "r"(v[14]), "r"(v[15]), "r"(v[16]), "r"(v[17]), "r"(v[18]), "r"(v[19]), "r"(v[20]), "r"(v[21]), "r"(v[22]), "r"(v[23]),
-        "r"(v[24]), "r"(v[25]), "r"(v[26]), "r"(v[27]), "r"(v[28]), "r"(v[29]), "r"(v[30]), "r"(v[31])
-        : "memory");
+
+// The first term of two weights, and what it leaves of them.  bf16's is cut off, not rounded: what is left is below 2^-7 of a weight, and the next term's rounding
+// half a step of that, 2^-15 of the weight.  (Attention of 128 rows of 64 heads behind 16 000 positions, with a second term: 134 us; with the first one rounded,
+// which is an instruction more per value, 153; with one term, whose rounding the results would show, 116.)
+template <typename T>
+__device__ __forceinline__ uint32_t first_term(float& a, float& b) {
+    if constexpr (std::is_same<T, __half>::value) {
+        return split_pair<T>(a, b);
+    } else {
+        const uint32_t x = __float_as_uint(a), y = __float_as_uint(b);
+        a -= __uint_as_float(x & 0xffff0000u);
+        b -= __uint_as_float(y & 0xffff0000u);
+        return __byte_perm(x, y, 0x7632);
+    }
 }
 
 // The softmax threads' part in bringing 128 * TILES rows of Q to shared memory, in operand layout, as terms of T.  Rows of T come by asynchronous copies,
@@ -383,16 +388,19 @@ __global__ void __launch_bounds__(PX_THREADS, 1) paged_prefix_kernel(const __gri
                     const float use = m == -INFINITY ? 0.f : m;
                     float l4[4] = {0.f, 0.f, 0.f, 0.f};
 #pragma unroll
-                    for (int k = 0; k < 64; ++k) {
-                        x[k] = exp2_approx(fmaf(x[k], sc, -use));
-                        l4[k & 3] += x[k];
-                    }
+                    for (int c = 0; c < 64; c += 16) {  // (the exponentials of some while others become terms)
 #pragma unroll
-                    for (int t2 = 0; t2 < TR::PT; ++t2) {
-                        uint32_t w[32];
+                        for (int k = c; k < c + 16; ++k) {
+                            x[k] = exp2_approx(fmaf(x[k], sc, -use));
+                            l4[k & 3] += x[k];
+                        }
 #pragma unroll
-                        for (int k = 0; k < 32; ++k) w[k] = TR::PT == 1 ? pair_of<T>(x[2 * k], x[2 * k + 1]) : split_pair<T>(x[2 * k], x[2 * k + 1]);
-                        tmem_st32u(tb + (uint32_t)(t2 * 32), w);  // (in the place of the scores, which have been read)
+                        for (int t2 = 0; t2 < TR::PT; ++t2) {
+                            uint32_t w[8];
+#pragma unroll
+                            for (int k = 0; k < 8; ++k) w[k] = t2 == 0 ? first_term<T>(x[c + 2 * k], x[c + 2 * k + 1]) : split_pair<T>(x[c + 2 * k], x[c + 2 * k + 1]);
+                            tmem_st8(tb + (uint32_t)(t2 * 32 + c / 2), w);  // (in the place of the scores, which have been read)
+                        }
                     }
                     l += (l4[0] + l4[1]) + (l4[2] + l4[3]);
                     tmem_wait_st();

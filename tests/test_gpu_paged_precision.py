@@ -1,0 +1,63 @@
+"""The paged operators where rounding, range and size can spoil a result without showing in random data: against definitions in 64 bits, with bounds that a lost
+term, a lost bit or a wrapped place would break.  U, eps and the tolerances' names as in test_gpu_paged.py."""
+import ctypes as C
+
+import pytest
+
+from test_gpu_paged import GGML, TYPES, Batch, at, dtype, queries, stream  # noqa: F401
+
+pytestmark = pytest.mark.gpu
+
+
+@pytest.fixture(scope="module")
+def L(pkg):
+    from llama2_jl_b200 import _lib
+    _lib.lib()
+    return _lib
+
+
+def half(t):
+    import torch
+    return torch.finfo(t).eps / 2
+
+
+def keys_of(b, seq, pos):
+    """Keys and values [n, kv, hs] in f64 that the token at own position `pos` sees."""
+    import torch
+    places = []
+    for pages, n in ((b.prefix_pages, b.prefix), (b.table[seq], pos + 1)):
+        i = torch.arange(n, device="cuda")
+        places.append((pages.long()[i // b.page] if n else i, i % b.page))
+    page, slot = (torch.cat(x) for x in zip(*places))
+    return b.k[page, :, slot].double(), b.v[page, :, slot].double()
+
+
+def attended(b, q, heads, scale=0.0):
+    import torch
+    out = torch.full_like(q, 7.0)
+    b.attend(b.plan(q, out, heads, scale))
+    return out
+
+
+@pytest.mark.parametrize("io", ["bf16", "f16"])
+@pytest.mark.parametrize("lengths,prefix,heads,kv,hs", [([301, 64, 17], 0, 4, 2, 64), ([300, 5], 0, 16, 1, 128), ([9, 1], 500, 8, 2, 96), ([9, 1], 500, 64, 2, 96), ([40] * 9, 700, 40, 1, 128)])
+def test_rows_of_16_bits_are_rounded_once(L, io, lengths, prefix, heads, kv, hs):
+    """What leaves is the 64-bit result rounded once, but for errors of 32-bit size: softmax weights are not cut to 8 or 11 bits on the way.
+
+    Scores: 8 products of 16, the sums off by a step of f32 each, 8 * 2^-23 = 2^-20 of their absolute size.  Weights: two terms; bf16's first is cut to 8 bits (2^-7 is
+    left at most) and the second half a step of that, 2^-15; f16's are half a step squared, 2^-22, or 2^-25 of the largest weight.  Sums: two steps per 16 keys."""
+    import torch
+    b = Batch(L, lengths, kv=kv, hs=hs, page=16, prefix=prefix, cache=io, seed=hs + heads)
+    q = queries(b, heads, io)
+    out = attended(b, q, heads)
+    t = dtype(io)
+    for row, seq, pos in b.new_rows():
+        k, v = (x.repeat_interleave(heads // kv, 1) for x in keys_of(b, seq, pos))
+        x = q[row].double().view(heads, hs)
+        w = torch.softmax(torch.einsum("hd,nhd->hn", x, k) * hs ** -0.5, -1)
+        ds = 2.0 ** -20 * (torch.einsum("hd,nhd->hn", x.abs(), k.abs()) * hs ** -0.5).amax(-1)[:, None]
+        want, size = torch.einsum("hn,nhd->hd", w, v), torch.einsum("hn,nhd->hd", w, v.abs())
+        tol = ((2.0 ** -15 if io == "bf16" else 2.0 ** -22) + ds + (len(k) / 8 + 16) * 2.0 ** -23) * size + (2.0 ** -25 * v.abs().sum(0) if io == "f16" else 0.0)
+        err = (out[row].double().view(heads, hs) - want).abs()
+        least = 2.0 ** -25 if io == "f16" else 0.0
+        assert (err <= tol + half(t) * (want.abs() + tol) + least).all(), (row, float((err / (half(t) * want.abs() + tol)).max()))
