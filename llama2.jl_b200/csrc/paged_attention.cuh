@@ -87,12 +87,19 @@ __device__ __forceinline__ uint32_t split_pair(float& a, float& b) {
     return *reinterpret_cast<const uint32_t*>(&v);
 }
 
+// What the exponents of weights are counted from: the maximum, less `up`.  bf16 has f32's range, but f16's terms stop at steps of 2^-24: behind a maximum of 1, weights of
+// 2^-20 would keep four bits, and many such keys may be all there is in a result whose largest weight has a value near zero.  With weights up to 2^15 the steps end at
+// 2^-39 of the largest here; behind a prefix, whose reference may lag by 2^6, at 2^-33 (a lag of 2^4 would make it 2^-35 and 128 rows behind 16 000 positions 135 us
+// instead of 128, one of 2 149).  Totals and sums carry the factor; a row's partial results say what they are counted from.  (Beyond 2^23 the difference would not be exact.)
+__device__ __forceinline__ float weight_reference(float mx, float up) { return fabsf(mx) < 8388608.f ? mx - up : mx; }
+
 // KS: steps of 16 values of a head, NT: tiles of 8 rows
 template <typename T, typename TIO, int KS, int NT>
 struct ThinTraits {
     static constexpr bool WIDE = sizeof(TIO) == 4;
     static constexpr int QT = !WIDE ? 1 : std::is_same<T, __half>::value ? 2 : 3, PT = WIDE ? QT : 2;  // terms of queries and of weights
     static constexpr int STAGES = NT == 1 ? 2 : 3, BLOCKS = NT == 1 ? 3 : 2;  // 12 warps of 168 registers on an SM, or 8 of 255
+    static constexpr float UP = std::is_same<T, __half>::value ? 15.f : 0.f;  // weights up to 2^15 (weight_reference)
     static constexpr int PITCH = KS * 32 + 16;               // bytes of a row in shared memory
     static constexpr int HALF_STAGE = PT_KEYS * PITCH;       // keys of a stage, or values
     static constexpr int RING = PT_WARPS * STAGES * 2 * HALF_STAGE;
@@ -328,7 +335,10 @@ __global__ void __launch_bounds__(PT_WARPS * 32, (ThinTraits<T, TIO, KS, NT>::BL
 #pragma unroll
                 for (int i = 0; i < 2 * NT; ++i) mx[i] = fmaxf(mx[i], __shfl_xor_sync(0xffffffffu, mx[i], o));
 #pragma unroll
-            for (int i = 0; i < 2 * NT; ++i) up |= mx[i] > m[i];
+            for (int i = 0; i < 2 * NT; ++i) {
+                if (TR::UP != 0.f) mx[i] = weight_reference(mx[i], TR::UP);
+                up |= mx[i] > m[i];
+            }
             if (__any_sync(0xffffffffu, up)) {
 #pragma unroll
                 for (int i = 0; i < 2 * NT; ++i) {

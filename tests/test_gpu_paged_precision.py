@@ -61,3 +61,41 @@ def test_rows_of_16_bits_are_rounded_once(L, io, lengths, prefix, heads, kv, hs)
         err = (out[row].double().view(heads, hs) - want).abs()
         least = 2.0 ** -25 if io == "f16" else 0.0
         assert (err <= tol + half(t) * (want.abs() + tol) + least).all(), (row, float((err / (half(t) * want.abs() + tol)).max()))
+
+
+@pytest.mark.parametrize("io", ["f32", "f16"])
+@pytest.mark.parametrize("own,prefix,heads", [(8001, 0, 4), (1, 8000, 4), (1, 8000, 48)])
+@pytest.mark.parametrize("log2_rest", [-7, -10, -12])
+def test_one_key_has_nearly_all_of_the_mass(L, io, own, prefix, heads, log2_rest):
+    """A key that every query asks for, whose value is zero, in front of 8 000 others that share 2^log2_rest of its mass: the result is what those others say,
+    and weights of 2^-20 to 2^-25 of the largest must keep their bits.
+
+    Weights in two f16 terms: off by 2^-22 relative, or by half a step of 2^-24 where the largest is 2^15 (own positions) or 2^9 at least (a prefix): 2^-40 or 2^-34 of
+    it.  Such errors of 8 000 keys are independent and evenly spread: their sum has a deviation of 2^-34 / sqrt(3) * sqrt(sum v^2), and six of those are allowed."""
+    import torch
+    hs, n = 64, own + prefix
+    b = Batch(L, [own], kv=1, hs=hs, page=64, prefix=prefix, cache="f16", seed=3)
+    g = torch.Generator(device="cuda").manual_seed(4)
+    flat = (lambda pages, pool, count: [(int(pages[i // 64]), i % 64) for i in range(count)])
+    places = flat(b.prefix_pages, b.k, prefix) + flat(b.table[0], b.k, own)
+    page, slot = (torch.tensor(x, device="cuda") for x in zip(*places))
+    # scores: q = (1, 0, ..), so a key's first value is its score at scale 1
+    k = torch.randn((n, hs), generator=g, device="cuda").half()
+    k[:, 0] = (torch.rand(n, generator=g, device="cuda") * 0.5).half()
+    k[0, 0] = 0.0
+    v = (1 + torch.rand((n, hs), generator=g, device="cuda")).half()
+    v[0] = 0
+    k[0, 0] = float(torch.logsumexp(k[1:, 0].double(), 0)) - log2_rest * 0.6931471805599453
+    b.k[page, 0, slot], b.v[page, 0, slot] = k, v
+    q = torch.zeros((1, heads * hs), device="cuda", dtype=dtype(io))
+    q[0, ::hs] = 1
+    out = attended(b, q, heads, 1.0)
+    z = k[:, 0].double()
+    w = torch.softmax(z, 0)
+    want = w @ v.double()
+    # scores are exact; the exponent's argument (up to 31 in base 2) is off by half a step of 2^-19, the exponential by 2^-22; sums: a step per 16 keys
+    tol = want * (2.0 ** -20 + 2.0 ** -22 + 2.0 ** -22 + (n / 16 + 16) * 2.0 ** -23)
+    tol = tol + (2.0 ** -34 if prefix else 2.0 ** -40) * 6 / 3 ** 0.5 * (v.double() ** 2).sum(0).sqrt()
+    tol = tol + half(q.dtype) * want + (2.0 ** -25 if io == "f16" else 0.0)
+    err = (out.double().view(heads, hs) - want).abs()
+    assert (err <= tol).all(), float((err / want).max())
