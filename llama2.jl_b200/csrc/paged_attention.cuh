@@ -231,7 +231,7 @@ __global__ void __launch_bounds__(PT_WARPS * 32, (ThinTraits<T, TIO, KS, NT>::BL
                     qv[ks][2 * h + 1] = x[1];
                 }
             unscale[nt] = 1.f;
-            if (TR::WIDE && std::is_same<T, __half>::value) {  // f16 terms: the row's largest value between 1/2 and 1
+            if (TR::WIDE && std::is_same<T, __half>::value) {  // f16 terms: the row's largest value between 2^14 and 2^15, so that the steps of 2^-24 at which they stop are 2^-38 of it
                 float mx = 0.f;
 #pragma unroll
                 for (int ks = 0; ks < KS; ++ks)
@@ -240,7 +240,7 @@ __global__ void __launch_bounds__(PT_WARPS * 32, (ThinTraits<T, TIO, KS, NT>::BL
                 mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 1));
                 mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 2));
                 int e = 0;
-                if (mx > 0.f && mx < INFINITY) e = max(-100, min(100, ilogbf(mx) + 1));
+                if (mx > 0.f && mx < INFINITY) e = max(-100, ilogbf(mx) + 1) - 15;
                 unscale[nt] = ldexpf(1.f, e);
                 const float f = ldexpf(1.f, -e);
 #pragma unroll

@@ -100,13 +100,13 @@ __device__ __forceinline__ void load_queries(const PrefixParams& p, uint8_t* sq,
         } else {
             float x[8] = {};
             if (real) get(src, x);
-            if (TR::F16) {  // f16 terms: the row's largest value between 1/2 and 1
+            if (TR::F16) {  // f16 terms: the row's largest value between 2^14 and 2^15, so that the steps of 2^-24 at which they stop are 2^-38 of it
                 float mx = 0.f;
 #pragma unroll
                 for (int e = 0; e < 8; ++e) mx = fmaxf(mx, fabsf(x[e]));
                 for (int o = 1 << shift >> 1; o > 0; o >>= 1) mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, o));
                 int ex = 0;
-                if (mx > 0.f && mx < INFINITY) ex = max(-100, min(100, ilogbf(mx) + 1));
+                if (mx > 0.f && mx < INFINITY) ex = max(-100, ilogbf(mx) + 1) - 15;
                 if (ch == 0) s_exp[r] = ex;
                 const float f = ldexpf(1.f, -ex);
 #pragma unroll

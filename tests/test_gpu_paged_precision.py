@@ -99,3 +99,28 @@ def test_one_key_has_nearly_all_of_the_mass(L, io, own, prefix, heads, log2_rest
     tol = tol + half(q.dtype) * want + (2.0 ** -25 if io == "f16" else 0.0)
     err = (out.double().view(heads, hs) - want).abs()
     assert (err <= tol).all(), float((err / want).max())
+
+
+@pytest.mark.parametrize("heads,own,prefix", [(4, 90, 0), (48, 1, 90)])
+def test_f32_queries_of_many_sizes_over_f16_keys(L, heads, own, prefix):
+    """One value of the query 2^17 times as large as the others, where the keys are zero: the others' bits count.
+
+    A query's value in two f16 terms is off by 2^-22 relative, or by 2^-39 of the row's largest."""
+    import torch
+    hs = 64
+    b = Batch(L, [own], kv=1, hs=hs, page=16, prefix=prefix, cache="f16", seed=5)
+    b.k *= 30
+    b.k[..., 0] = 0
+    g = torch.Generator(device="cuda").manual_seed(6)
+    q = torch.randn((1, heads, hs), generator=g, device="cuda") * 0.05
+    q[..., 0] = 8000.0
+    q = q.view(1, -1)
+    out = attended(b, q, heads)
+    k, v = (x[:, 0] for x in keys_of(b, 0, own - 1))
+    x = q.double().view(heads, hs)
+    w = torch.softmax(x @ k.T * hs ** -0.5, -1)
+    want, size = w @ v, w @ v.abs()
+    ds = ((x.abs() * 2.0 ** -18 + 2.0 ** -39 * 8000) @ k.abs().T * hs ** -0.5).amax(-1)[:, None]  # (2^-18: terms and sums, as for every score)
+    tol = (ds + 2.0 ** -22 + (len(k) / 16 + 16) * 2.0 ** -23) * size + 2.0 ** -24 * want.abs()
+    err = (out.double().view(heads, hs) - want).abs()
+    assert (err <= tol).all(), float((err - tol).max())
