@@ -124,3 +124,50 @@ def test_f32_queries_of_many_sizes_over_f16_keys(L, heads, own, prefix):
     tol = (ds + 2.0 ** -22 + (len(k) / 16 + 16) * 2.0 ** -23) * size + 2.0 ** -24 * want.abs()
     err = (out.double().view(heads, hs) - want).abs()
     assert (err <= tol).all(), float((err - tol).max())
+
+
+def terms(x, t, n):
+    """x in f64 as the sum of n terms of the type t."""
+    import torch
+    left, total = x.clone(), torch.zeros_like(x)
+    for _ in range(n):
+        y = left.to(t).double()
+        total, left = total + y, left - y
+    return total
+
+
+@pytest.mark.parametrize("cache", ["bf16", "f16"])
+@pytest.mark.parametrize("own,prefix,heads", [(2, 0, 8), (2, 0, 64), (1, 1, 64), (0, 2, 64)])
+def test_every_term_of_f32_rows_counts(L, cache, own, prefix, heads):
+    """Two keys, a power of two and zero, queries with one value: the score q * 2^j is exact, the result is w / (1 + w) times a value of one, w = exp(-score).
+
+    Score about 8: the result hangs on the query's last bits.  Score about 1: on the weight's."""
+    import torch
+    hs, t = 64, dtype(cache)
+    full = 3 if cache == "bf16" else 2
+    for j, bound_of_terms in ((3, "query"), (0, "weight")):
+        b = Batch(L, [own], kv=1, hs=hs, page=8, prefix=prefix, cache=cache, width=1)
+        for pool in (b.k, b.v):
+            pool.zero_()
+        where = [(b.prefix_pages, i) for i in range(prefix)] + [(b.table[0], i) for i in range(own)]
+        (p0, s0), (p1, s1) = [(int(pages[0]), i) for pages, i in where]
+        b.k[p0, 0, s0, 5] = 2.0 ** j  # the dominant key, with a value of zero
+        b.v[p1, 0, s1] = 1
+        g = torch.Generator(device="cuda").manual_seed(7)
+        q = torch.zeros((1, heads, hs), device="cuda")
+        q[0, :, 5] = 1 + torch.rand(heads, generator=g, device="cuda")
+        out = attended(b, q.view(1, -1), heads, 1.0).double().view(heads, hs)
+        score = q[0, :, 5].double() * 2.0 ** j
+        w = torch.exp(-score)
+        want = (w / (1 + w))[:, None]
+        # relative: the score off by a step of f32 for its scale and one for each of its sums (4), the exponent's argument (below 32, 4 in base 2) by half a step,
+        # the exponential by 2^-22, three terms by 2^-24 (two of f16: 2^-22), sum, quotient and their rounding by 2^-22
+        tol = score * 5 * 2.0 ** -23 + (2.0 ** -20 if j else 2.0 ** -23) + 3 * 2.0 ** -22
+        assert ((out - want).abs() <= tol[:, None] * want).all(), (bound_of_terms, float(((out - want).abs() / want).max()))
+        # a term fewer would not pass
+        if bound_of_terms == "query":
+            lost = torch.exp(-terms(q[0, :, 5].double(), t, full - 1) * 2.0 ** j)
+            lost = lost / (1 + lost)
+        else:
+            lost = terms(w, t, full - 1) / (1 + w)
+        assert ((lost - want[:, 0]).abs() > 1.5 * tol * want[:, 0]).any()
