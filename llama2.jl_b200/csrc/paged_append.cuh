@@ -30,7 +30,7 @@ struct AppendParams {
     int64_t q_stride, k_stride, v_stride, q_out_stride;
     const float *q_gain, *k_gain;  // null: no norm
     float eps, inv_size;
-    int n_heads, rotate, tokens;  // tokens of a block
+    int n_heads, tokens;  // tokens of a block
     double turns[PA_MAX_SIZE / 2];      // turns per position
 };
 
@@ -76,11 +76,14 @@ __device__ __forceinline__ void put(T* p, const float (&x)[N]) {
     *reinterpret_cast<Pack<T, N>*>(p) = a;
 }
 
-// TI: type of the rows, TC: of the cache, P: values of a piece (8, or 4 for heads that are no multiple of 16),
-// NEOX: pairs half a head apart
-template <typename TI, typename TC, int P, bool NEOX>
+// What rotation pairs.  Without it no pairs are formed at all: with sines of 0 an infinite value would be no number in its partner's place.
+enum RowPairs { PAIRS_NONE, PAIRS_NEIGHBOURS, PAIRS_HALF_APART };
+
+// TI: type of the rows, TC: of the cache, P: values of a piece (8, or 4 for heads that are no multiple of 16)
+template <typename TI, typename TC, int P, RowPairs PAIRS>
 __global__ void __launch_bounds__(PA_THREADS, 3) paged_append_kernel(const __grid_constant__ AppendParams p) {
     constexpr int AHEAD = 32 / (P * (int)sizeof(TI));  // groups of heads under way
+    constexpr bool ROTATE = PAIRS != PAIRS_NONE, NEOX = PAIRS == PAIRS_HALF_APART;
     __shared__ __align__(16) float2 s_cs[PA_MAX_TOKENS][PA_MAX_SIZE / 2];
     __shared__ int s_page[PA_MAX_TOKENS], s_slot[PA_MAX_TOKENS], s_new[PA_MAX_TOKENS];
     const int hs = p.pool.hs, half = hs / 2, units = hs / (2 * P), tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
@@ -107,7 +110,7 @@ __global__ void __launch_bounds__(PA_THREADS, 3) paged_append_kernel(const __gri
         s_slot[tid] = pos & ((1 << p.pool.page_shift) - 1);
         s_new[tid] = j < count;
     }
-    if (p.rotate) {
+    if constexpr (ROTATE) {
         for (int i = tid; i < here * half; i += PA_THREADS) {
             const int t = i / half, f = i - t * half;
             const int64_t row = row0 + t;
@@ -139,7 +142,7 @@ __global__ void __launch_bounds__(PA_THREADS, 3) paged_append_kernel(const __gri
                 const int da = NEOX ? d0 + i : (i < P / 2 ? d0 + 2 * i : d1 + 2 * i - P), db = NEOX ? d1 + i : da + 1;
                 float2 cs = make_float2(1.f, 0.f);
                 float ga = 1.f, gb = 1.f;
-                if (active && p.rotate) cs = s_cs[t][NEOX ? da : da / 2];
+                if (ROTATE && active) cs = s_cs[t][NEOX ? da : da / 2];
                 if (active && gains) {
                     ga = gains[da];
                     gb = gains[db];
@@ -184,8 +187,8 @@ __global__ void __launch_bounds__(PA_THREADS, 3) paged_append_kernel(const __gri
                         float& xa = NEOX ? x[0][i] : x[2 * i / P][2 * i % P];
                         float& xb = NEOX ? x[1][i] : x[2 * i / P][2 * i % P + 1];
                         const float a = xa * r, b = xb * r;
-                        xa = a * ca[i] - b * cb[i];
-                        xb = a * cc[i] + b * cd[i];
+                        xa = ROTATE ? a * ca[i] - b * cb[i] : a * ca[i];
+                        xb = ROTATE ? a * cc[i] + b * cd[i] : b * cd[i];
                     }
                 }
                 if (go) {

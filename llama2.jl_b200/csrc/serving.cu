@@ -218,8 +218,9 @@ extern "C" int32_t l2b_paged_append_device(const l2b_paged_cache* cache, const l
     p.q = rows->dev_q; p.k = rows->dev_k; p.v = rows->dev_v; p.q_out = rows->dev_q_out;
     p.q_stride = rows->q_stride; p.k_stride = rows->k_stride; p.v_stride = rows->v_stride; p.q_out_stride = rows->q_out_stride;
     p.q_gain = rows->dev_q_gain; p.k_gain = rows->dev_k_gain; p.eps = rows->eps; p.inv_size = 1.f / (float)hs;
-    p.n_heads = rows->n_heads; p.rotate = rows->rope_freq_base > 0.f;
-    if (p.rotate) {
+    p.n_heads = rows->n_heads;
+    const bool rotate = rows->rope_freq_base > 0.f;
+    if (rotate) {
         const long double step = powl((long double)rows->rope_freq_base, -2.0L / hs);
         long double f = 0.15915494309189533576888376337251436L;  // turns per radian
         for (int i = 0; i < hs / 2; ++i, f *= step) p.turns[i] = (double)f;
@@ -250,9 +251,12 @@ extern "C" int32_t l2b_paged_append_device(const l2b_paged_cache* cache, const l
             CU(launch_kernel(kernel, grid, dim3(PA_THREADS), 0, st, true, p));
             return L2B_OK;
         };
-        const bool neox = rows->rope_is_neox != 0;
-        if (piece == 8) L2B_TRY(neox ? go(paged_append_kernel<TIO, T, 8, true>) : go(paged_append_kernel<TIO, T, 8, false>));
-        else L2B_TRY(neox ? go(paged_append_kernel<TIO, T, 4, true>) : go(paged_append_kernel<TIO, T, 4, false>));
+        auto pairs = [&](auto size) -> int32_t {
+            constexpr int P = decltype(size)::value;
+            if (!rotate) return go(paged_append_kernel<TIO, T, P, PAIRS_NONE>);
+            return rows->rope_is_neox ? go(paged_append_kernel<TIO, T, P, PAIRS_HALF_APART>) : go(paged_append_kernel<TIO, T, P, PAIRS_NEIGHBOURS>);
+        };
+        L2B_TRY(piece == 8 ? pairs(std::integral_constant<int, 8>()) : pairs(std::integral_constant<int, 4>()));
         return L2B_OK;
     });
 }

@@ -171,3 +171,32 @@ def test_every_term_of_f32_rows_counts(L, cache, own, prefix, heads):
         else:
             lost = terms(w, t, full - 1) / (1 + w)
         assert ((lost - want[:, 0]).abs() > 1.5 * tol * want[:, 0]).any()
+
+
+@pytest.mark.parametrize("heads,kv,hs,neox", [(4, 2, 64, False), (4, 2, 64, True), (3, 1, 40, False), (3, 1, 40, True)])
+@pytest.mark.parametrize("norm", [False, True])
+def test_append_without_rotation_leaves_neighbours_alone(L, heads, kv, hs, neox, norm):
+    """rope_freq_base 0: every value comes from its own place; infinities and values that are no numbers reach no pair's other half."""
+    import torch
+    b = Batch(L, [3, 20], kv=kv, hs=hs, page=8, cache="bf16", filled=False)
+    g = torch.Generator(device="cuda").manual_seed(8)
+    q, k = (torch.randn((2, n, hs), generator=g, device="cuda") for n in (heads, kv))
+    v = torch.randn((2, kv * hs), generator=g, device="cuda")
+    for x in (q, k):
+        x[0, 0, 6], x[1, 0, 7] = float("inf"), -float("inf")
+        if not norm:
+            x[0, 0, hs // 2 + 3] = float("nan")
+    q_out = torch.zeros_like(q)
+    gain = (1 + 0.2 * torch.randn(hs, generator=g, device="cuda")) if norm else None
+    b.append(L.PagedRows(type=0, n_heads=heads, dev_q=at(q), dev_k=at(k), dev_v=at(v), q_stride=heads * hs, k_stride=kv * hs, v_stride=kv * hs, dev_q_out=at(q_out), q_out_stride=heads * hs,
+                         dev_q_gain=at(gain), dev_k_gain=at(gain), eps=1e-6, rope_is_neox=int(neox)))
+    for i, n in enumerate((3, 20)):
+        page, slot = b.place(i, n - 1)
+        for x, got, bits in ((q, q_out[i], 0), (k, b.k[page, :, slot], 2.0 ** -8)):
+            want = x[i].double()
+            if norm:
+                want = want / torch.sqrt((want * want).mean(-1, keepdim=True) + 1e-6) * gain.double()
+            got = got.double()
+            fine = want.isfinite()
+            assert torch.equal(got[~fine].isnan(), want[~fine].isnan()) and torch.equal(got[~fine].nan_to_num(9), want[~fine].nan_to_num(9))
+            assert ((got[fine] - want[fine]).abs() <= (bits + 32 * 2.0 ** -24) * want[fine].abs() * (1 + 2.0 ** -16)).all()
