@@ -512,11 +512,11 @@ __global__ void __launch_bounds__(PJ_WARPS * 32) paged_join_kernel(const __grid_
         }
         float2 v = make_float2(-INFINITY, 0.f);
         if (ml) v = __ldcg(reinterpret_cast<const float2*>(ml));
-        const uint32_t off = acc ? (uint32_t)((acc - p.slot_acc) >> 2) : 0;  // (everything lies behind the slots, in steps of 16 bytes)
+        const int64_t off = acc ? (acc - p.slot_acc) >> 2 : 0;  // (in steps of 16 bytes; 64 bits: a million tokens' partial results are more than 64 GiB)
         const int last = min(32, (parts - first + per_row - 1) >> per_row_shift);
         // the sums of four parts under way while the maxima come
         auto take = [&](int i, float4& x) {
-            const uint32_t at = __shfl_sync(0xffffffffu, off, i);
+            const int64_t at = __shfl_sync(0xffffffffu, off, i);
             x = make_float4(0.f, 0.f, 0.f, 0.f);
             if (i < last && d < hs) x = __ldcg(reinterpret_cast<const float4*>(p.slot_acc) + at + lane);
         };

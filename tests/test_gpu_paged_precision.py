@@ -200,3 +200,33 @@ def test_append_without_rotation_leaves_neighbours_alone(L, heads, kv, hs, neox,
             fine = want.isfinite()
             assert torch.equal(got[~fine].isnan(), want[~fine].isnan()) and torch.equal(got[~fine].nan_to_num(9), want[~fine].nan_to_num(9))
             assert ((got[fine] - want[fine]).abs() <= (bits + 32 * 2.0 ** -24) * want[fine].abs() * (1 + 2.0 ** -16)).all()
+
+
+def test_a_workspace_of_more_than_64_gib(L):
+    """More than a million tokens of 64 heads behind a prefix: partial results lie further from each other than 2^32 steps of 16 bytes."""
+    import torch
+    if torch.cuda.mem_get_info()[0] < 125 << 30:
+        pytest.skip("needs 125 GB of device memory")
+    n_seq, heads, hs, page, prefix = 1_040_000, 64, 128, 8, 8
+    g = torch.Generator(device="cuda").manual_seed(9)
+    k, v = (torch.randn((2, 1, page, hs), generator=g, device="cuda").bfloat16() for _ in "kv")
+    q = torch.empty((n_seq, heads * hs), device="cuda", dtype=torch.bfloat16).normal_(generator=g)
+    out = torch.full_like(q, 7.0)
+    lengths, table, first = (torch.full(s, x, dtype=torch.int32, device="cuda") for s, x in (((n_seq,), 3), ((n_seq, 1), 1), ((1,), 0)))
+    cache = L.PagedCache(dev_k=at(k), dev_v=at(v), type=GGML["bf16"], n_pages=2, page_size=page, n_kv_heads=1, head_size=hs)
+    batch = L.PagedBatch(n_seq=n_seq, n_query=1, dev_lengths=at(lengths), dev_pages=at(table), pages_per_seq=1, prefix_len=prefix, dev_prefix_pages=at(first))
+    qs = L.PagedQueries(type=GGML["bf16"], n_heads=heads, dev_q=at(q), q_stride=heads * hs, dev_out=at(out), out_stride=heads * hs)
+    need = C.c_int64()
+    L.check(L.lib().l2b_paged_attention_workspace(C.byref(cache), C.byref(batch), C.byref(qs), C.byref(need)))
+    assert need.value > 65 << 30
+    w = torch.empty((need.value // 4,), device="cuda")
+    L.check(L.lib().l2b_paged_attention_device(C.byref(cache), C.byref(batch), C.byref(qs), at(w), need.value, stream()))
+    keys, values = (torch.cat([x[0, 0], x[1, 0, :3]]).double() for x in (k, v))
+    rows = torch.cat([torch.arange(0, n_seq, 4999, device="cuda"), torch.arange(n_seq - 40, n_seq, device="cuda")])
+    z = torch.softmax(q[rows].double().view(-1, heads, hs) @ keys.T * hs ** -0.5, -1)
+    want, size = z @ values, z @ values.abs()
+    err = (out[rows].double().view(-1, heads, hs) - want).abs()
+    # scores of about 11 in absolute size, off by 2^-18 of it; everything else is smaller
+    tol = 2.0 ** -14 * size + 2.0 ** -8 * want.abs()
+    bad = ((err > tol).any(-1).any(-1)).nonzero()
+    assert len(bad) == 0, (len(bad), rows[bad[0]])
