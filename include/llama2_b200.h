@@ -197,9 +197,11 @@ int32_t l2b_generate(l2b_session* session, const int32_t* host_prompt, int32_t n
 
 /* Copy the logits of the most recent position to the host (state.logits). */
 int32_t l2b_session_logits(l2b_session* session, float* host_logits);
-/* A token from those logits (of the most recent l2b_forward, l2b_decode_next or l2b_prefill call) by temperature and the cuts of l2b_sample_device
- * (top_k 0, top_p 1 and min_p 0: none); temperature 0: argmax.  l2b_forward(session, token, pos, NULL) and this call are one iteration of the loop in
- * `sample` (src/inference.jl:349-385) with cuts. */
+/* A token from those logits by temperature and the cuts of l2b_sample_device (top_k 0, top_p 1 and min_p 0: none); temperature 0: argmax.
+ * l2b_forward(session, token, pos, NULL) and this call are one iteration of the loop in `sample` (src/inference.jl:349-385) with cuts.  The logits are those of the
+ * most recent l2b_forward, l2b_decode_next or l2b_prefill call, or of l2b_generate's last position.  L2B_ERR_STATE where there are none: before the first such
+ * call, after a reset, after one that failed or ended inside l2b_generate's prompt, and after l2b_session_extend has taken several tokens of a layer-stack model
+ * (whose logits go to the caller alone). */
 int32_t l2b_session_sample(l2b_session* session, float temperature, int32_t top_k, float top_p, float min_p, double uniform, int32_t* next_token);
 /* Copy an activation buffer of the most recent forward for stage-wise checks:
  * which: 0 = x (residual stream after the last layer, before the final norm is applied in place),

@@ -611,6 +611,7 @@ struct l2b_session {
     l2b_model* model = nullptr;
     StackSession* stack = nullptr;  // layer-stack models: caches and activations
     int state_pos = 0;              // models with a recurrent state: the position it is ready for (-1: none but 0, which starts afresh)
+    bool has_logits = false;        // `logits` are those of the position the session stands at (l2b_session_sample chooses from them)
     cudaStream_t stream = nullptr;
     bool own_stream = false;
     DeviceInfo di;
@@ -1773,6 +1774,7 @@ extern "C" int32_t l2b_session_create(l2b_model* m, void* stream, l2b_session** 
 extern "C" int32_t l2b_session_reset(l2b_session* s) {
     if (!s) return fail(L2B_ERR_BAD_ARG, "null session");
     CU(cudaSetDevice(s->model->device));
+    s->has_logits = false;
     if (s->stack) {
         L2B_TRY(stack_session_reset(s->stack, s->stream));
         CU(cudaStreamSynchronize(s->stream));
@@ -1860,6 +1862,11 @@ static int32_t state_at(int32_t status, int& state_pos, int pos) {
     if (status == L2B_OK) state_pos = pos;
     return status;
 }
+// The same of a session's last call, and whether it has left the last position's logits.
+static int32_t session_at(int32_t status, l2b_session* s, int pos, bool logits) {
+    s->has_logits = status == L2B_OK && logits;
+    return state_at(status, s->state_pos, pos);
+}
 
 // One graph launch with the control block set from the host.
 static int32_t run_one(l2b_session* s, int token, int pos, float temperature, double uniform) {
@@ -1870,6 +1877,7 @@ static int32_t run_one(l2b_session* s, int token, int pos, float temperature, do
     if (!s->graph) return fail(L2B_ERR_STATE, "tensor-parallel session: call l2b_session_tp_connect first");
     L2B_TRY(check_state(s->model, s->state_pos, pos));
     s->state_pos = -1;
+    s->has_logits = false;
     CU(cudaSetDevice(s->model->device));
     Control& h = *s->h_ctl;
     memset(&h, 0, sizeof(h));
@@ -1886,7 +1894,7 @@ static int32_t run_one(l2b_session* s, int token, int pos, float temperature, do
     CU(cudaEventRecord(s->ev1, s->stream));
     CU(cudaStreamSynchronize(s->stream));
     CU(cudaEventElapsedTime(&s->last_ms, s->ev0, s->ev1));
-    return state_at(check_status_word(s), s->state_pos, pos + 1);
+    return session_at(check_status_word(s), s, pos + 1, true);
 }
 
 // ---- many-token prompt pass ---------------------------------------------------------------------------------
@@ -2256,6 +2264,7 @@ extern "C" int32_t l2b_prefill(l2b_session* s, const int32_t* tokens, int32_t n,
     if (!s->graph) return fail(L2B_ERR_STATE, "tensor-parallel session: call l2b_session_tp_connect first");
     L2B_TRY(check_state(s->model, s->state_pos, pos0));
     s->state_pos = -1;
+    s->has_logits = false;
     CU(cudaSetDevice(s->model->device));
     Control& h = *s->h_ctl;
     memset(&h, 0, sizeof(h));
@@ -2280,7 +2289,7 @@ extern "C" int32_t l2b_prefill(l2b_session* s, const int32_t* tokens, int32_t n,
     CU(cudaStreamSynchronize(s->stream));
     CU(cudaEventElapsedTime(&s->last_ms, s->ev0, s->ev1));
     if (next) *next = s->h_small[0];
-    return state_at(check_status_word(s), s->state_pos, end);
+    return session_at(check_status_word(s), s, end, true);
 }
 
 // Feed a portion of n tokens at positions pos0 .. and return the logits at n_want places among them (ascending).  Layer-stack
@@ -2308,6 +2317,7 @@ extern "C" int32_t l2b_session_extend(l2b_session* s, const int32_t* tokens, int
     }
     L2B_TRY(check_state(s->model, s->state_pos, pos0));
     s->state_pos = -1;
+    s->has_logits = false;
     CU(cudaSetDevice(s->model->device));
     constexpr int WANT_ROWS = 128;  // rows per classifier pass
     const int max_rows = stack_session_max_rows(s->stack);
@@ -2339,7 +2349,7 @@ extern "C" int32_t l2b_session_extend(l2b_session* s, const int32_t* tokens, int
     CU(cudaEventRecord(s->ev1, s->stream));
     CU(cudaStreamSynchronize(s->stream));
     CU(cudaEventElapsedTime(&s->last_ms, s->ev0, s->ev1));
-    return state_at(check_status_word(s), s->state_pos, pos0 + n);
+    return session_at(check_status_word(s), s, pos0 + n, false);
 }
 
 extern "C" int32_t l2b_session_prefill_gemm(l2b_session* s, int32_t* min_tokens) {
@@ -2367,6 +2377,7 @@ extern "C" int32_t l2b_generate(l2b_session* s, const int32_t* prompt, int32_t n
     if (!s->graph) return fail(L2B_ERR_STATE, "tensor-parallel session: call l2b_session_tp_connect first");
     L2B_TRY(check_state(s->model, s->state_pos, 0));
     s->state_pos = -1;
+    s->has_logits = false;
     CU(cudaSetDevice(s->model->device));
     Control& h = *s->h_ctl;
     memset(&h, 0, sizeof(h));
@@ -2405,7 +2416,7 @@ extern "C" int32_t l2b_generate(l2b_session* s, const int32_t* prompt, int32_t n
     CU(cudaEventElapsedTime(&s->last_prompt_ms, s->ev0, s->ev_mid));
     CU(cudaEventElapsedTime(&s->last_decode_ms, s->ev_mid, s->ev1));
     if (device_ms) *device_ms = s->last_ms;
-    return state_at(check_status_word(s), s->state_pos, n_positions);
+    return session_at(check_status_word(s), s, n_positions, first < n_positions || whole);
 }
 
 extern "C" int32_t l2b_session_logits(l2b_session* s, float* host_logits) {
@@ -2422,6 +2433,7 @@ extern "C" int32_t l2b_session_sample(l2b_session* s, float temperature, int32_t
     if (!(uniform >= 0.0 && uniform < 1.0)) return fail(L2B_ERR_BAD_ARG, "uniform must lie in [0,1)");
     const int vocab = s->model->cfg.vocab_size;
     if (vocab > SAMPLE_MAX_VOCAB) return fail(L2B_ERR_BAD_ARG, "a vocabulary of more than 393216");
+    if (!s->has_logits) return fail(L2B_ERR_STATE, "the session holds no logits: none computed since it was created or reset, or the last call failed or kept none");
     CU(cudaSetDevice(s->model->device));
     L2B_TRY(enqueue_filtered_sample(s->logits, vocab, temperature, top_k, top_p, min_p, uniform, s->next_token, s->model->device, s->stream));
     CU(cudaMemcpyAsync(&s->h_small[0], s->next_token, 4, cudaMemcpyDeviceToHost, s->stream));

@@ -67,3 +67,69 @@ def test_refusals(pkg, model):
     assert lib.l2b_session_sample(s.session, float("nan"), 0, 1.0, 0.0, 0.5, C.byref(n)) == 1
     for u in (-0.1, 1.0, float("nan")):
         assert lib.l2b_session_sample(s.session, 1.0, 0, 1.0, 0.0, u, C.byref(n)) == 1
+
+
+def test_no_token_without_logits(pkg, synth):
+    """A session that holds no logits of its last position refuses to sample: new, reset, after a call that failed, after a prompt that was cut inside."""
+    lib, n = pkg.lib(), C.c_int32()
+    cfg = pkg.ModelConfig(64, 96, 2, 4, 4, 700, 48, 10000.0, False)
+    m = pkg.LanguageModel(cfg, Tokenizer(700), synth.model_weights(cfg, dict.fromkeys(("wq", "wk", "wv", "wo", "w1", "w2", "w3", "token_embd", "output"), 0), seed=3))
+    s = pkg.RunState(m)
+
+    def status():
+        return lib.l2b_session_sample(s.session, 0.0, 0, 1.0, 0.0, 0.5, C.byref(n))
+    assert status() == 7 and b"logits" in lib.l2b_last_error_string()
+    pkg.transformer_(5, 0, cfg, s)
+    assert status() == 0 and n.value == int(s.logits.argmax())
+    s.reset()
+    assert status() == 7
+    first = pkg.prefill(s, [5, 9, 33])
+    assert status() == 0 and n.value == first
+    assert lib.l2b_forward(s.session, 700, 3, None) == 1  # (refused before anything has changed)
+    assert status() == 0 and n.value == first
+    got, _ = pkg.generate(m, np.array([5, 9, 33], np.int32), 6)
+    assert status() == 0 and n.value == got[5]
+    pkg.generate(m, np.array([5, 9, 33, 7, 8], np.int32), 3)
+    assert status() == 7
+    nxt = C.c_int32()
+    assert lib.l2b_decode_next(s.session, 8, 3, 0.7, 0.3, C.byref(nxt)) == 0 and status() == 0
+    m.close()
+    # one rank of two that has not been connected to the other: nothing can have been computed
+    from tp_worker import tiny_config
+    cfg = tiny_config(pkg)
+    m = pkg.LanguageModel(cfg, None, synth.model_weights(cfg, synth.ALL(synth.Q4), seed=3), tp_size=2, tp_rank=0)
+    s = pkg.RunState(m)
+    assert status() == 7 and lib.l2b_forward(s.session, 1, 0, None) == 7 and status() == 7
+    m.close()
+
+
+@pytest.mark.parametrize("compute", ["float32", "bfloat16"])
+def test_layer_stack_sessions(pkg, compute):
+    """The same on a layer-stack model, token by token and after prompts; a portion of several tokens keeps no logits in the session."""
+    import savozen_cases as sc
+    from stack_common import build
+    cfg = sc.CASES["all"]
+    model = build(pkg, cfg, sc.weights(cfg, 5), 40, compute)
+    s, t = pkg.RunState(model), sc.tokens(cfg, 12, 6)
+    lib, n, rng = pkg.lib(), C.c_int32(), np.random.default_rng(2)
+
+    def status():
+        return lib.l2b_session_sample(s.session, 1.0, 5, 1.0, 0.0, 0.5, C.byref(n))
+
+    def tokens_agree():
+        L_logits = np.zeros_like(s.logits)
+        assert lib.l2b_session_logits(s.session, L_logits.ctypes.data) == 0
+        for cuts, short in ((dict(top_k=5), dict(k=5)), (dict(top_p=0.5), dict(p=0.5)), (dict(), dict())):
+            u = float(rng.random())
+            assert pkg.sample_next(s, 0.75, uniform=u, **cuts) == reference(L_logits.astype(np.float64), t=0.75, u=u, **short)[0]
+    assert status() == 7
+    for pos in range(3):
+        pkg.transformer_(int(t[pos]), pos, model.config, s)
+        tokens_agree()
+    assert pkg.prefill(s, t[3:8], 3) >= 0
+    tokens_agree()
+    pkg.extend(s, t[8:11], 8, [2])
+    assert status() == 7
+    pkg.extend(s, t[11:12], 11, [0])
+    tokens_agree()
+    model.close()
