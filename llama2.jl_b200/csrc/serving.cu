@@ -91,6 +91,7 @@ int32_t check_batch(const l2b_paged_batch* b, const PagedPool& pool, PagedSeqs& 
     if (b->n_seq < 0 || b->n_query < 1 || b->pages_per_seq < 0 || b->prefix_len < 0) return fail(L2B_ERR_BAD_ARG, "bad batch shape");
     if ((b->n_seq > 0 && !b->dev_lengths) || (b->n_seq > 0 && b->pages_per_seq > 0 && !b->dev_pages) || (b->prefix_len > 0 && !b->dev_prefix_pages))
         return fail(L2B_ERR_BAD_ARG, "null argument");
+    if (!aligned(b->dev_lengths, 4) || !aligned(b->dev_counts, 4) || !aligned(b->dev_pages, 4) || !aligned(b->dev_prefix_pages, 4)) return fail(L2B_ERR_BAD_ARG, "misaligned pointer");
     if (((int64_t)b->pages_per_seq << pool.page_shift) + b->prefix_len > 0x7fffffff) return fail(L2B_ERR_BAD_ARG, "more than 2^31 - 1 positions");
     if ((int64_t)b->n_seq * b->n_query > 0x7fffffff) return fail(L2B_ERR_BAD_ARG, "more than 2^31 - 1 rows");
     s.lengths = b->dev_lengths;
@@ -396,7 +397,9 @@ extern "C" int32_t l2b_sample_device(const l2b_sampling* a, void* stream) {
     if (a->n_rows < 0 || a->vocab < 1 || a->vocab > SAMPLE_MAX_VOCAB) return fail(L2B_ERR_BAD_ARG, "bad number of rows, or a vocabulary of more than 393216");
     if (a->n_rows > 0x7fffffff / FS_CLUSTER) return fail(L2B_ERR_BAD_ARG, "too many rows");
     if (a->stride < a->vocab) return fail(L2B_ERR_BAD_ARG, "rows overlap");
-    if (!aligned(a->dev_logits, type_bytes(a->type)) || !aligned(a->dev_tokens, 4) || !aligned(a->dev_uniform, 8)) return fail(L2B_ERR_BAD_ARG, "misaligned pointer");
+    if (!aligned(a->dev_logits, type_bytes(a->type)) || !aligned(a->dev_tokens, 4) || !aligned(a->dev_uniform, 8) || !aligned(a->dev_temperature, 4) || !aligned(a->dev_top_k, 4) ||
+        !aligned(a->dev_top_p, 4) || !aligned(a->dev_min_p, 4) || !aligned(a->dev_probs, 4))
+        return fail(L2B_ERR_BAD_ARG, "misaligned pointer");
     OnDeviceOf on;
     L2B_TRY(on.enter(a->dev_logits, "dev_logits"));
     if (a->n_rows == 0) return L2B_OK;
