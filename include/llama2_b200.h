@@ -360,7 +360,7 @@ typedef struct l2b_paged_queries {
     int64_t q_stride;
     void* dev_out;
     int64_t out_stride;
-    float scale;       /* 0: 1 / sqrt(head_size) */
+    float scale;       /* 0: 1 / sqrt(head_size); at most 2.3e38 in size (scale * log2(e) is a number) */
     int32_t reserved;
 } l2b_paged_queries;
 /* attention_weights! + scale + softmax! + combine_values! (src/inference.jl:263-278) of every new token over the prefix and over its sequence's own

@@ -13,6 +13,7 @@ using namespace l2b;
 namespace {
 
 constexpr int MAX_DEVICES = 64;
+constexpr float LOG2E = 1.4426950408889634f;  // the kernels' exponents count in powers of two
 static_assert(SAMPLE_MAX_VOCAB == FS_CLUSTER * FS_SLICE, "what a cluster's shared memory holds");
 
 // The device that a pointer's memory is on is the current one while this lives.
@@ -190,7 +191,7 @@ int32_t check_queries(const l2b_paged_cache* c, const l2b_paged_queries* q, cons
     L2B_TRY(check_row_type(q->type, c->type));
     if (q->n_heads <= 0 || q->n_heads > 65535 || q->n_heads % c->n_kv_heads) return fail(L2B_ERR_BAD_ARG, "n_heads must be a multiple of n_kv_heads");
     if ((int64_t)s.n_seq * s.n_query * q->n_heads > 0x7fffffff) return fail(L2B_ERR_BAD_ARG, "more than 2^31 - 1 query heads");
-    if (!std::isfinite(q->scale)) return fail(L2B_ERR_BAD_ARG, "scale must be finite, or 0 for 1 / sqrt(head_size)");
+    if (!std::isfinite(q->scale * LOG2E)) return fail(L2B_ERR_BAD_ARG, "scale must be at most 2.3e38 in size, or 0 for 1 / sqrt(head_size)");
     return L2B_OK;
 }
 
@@ -298,7 +299,7 @@ extern "C" int32_t l2b_paged_attention_device(const l2b_paged_cache* cache, cons
     p.q = queries->dev_q; p.out = queries->dev_out; p.q_stride = queries->q_stride; p.out_stride = queries->out_stride;
     p.n_heads = queries->n_heads;
     p.group = queries->n_heads / p.pool.n_kv;
-    p.scale2 = (queries->scale != 0.f ? queries->scale : 1.f / sqrtf((float)hs)) * 1.4426950408889634f;
+    p.scale2 = (queries->scale != 0.f ? queries->scale : 1.f / sqrtf((float)hs)) * LOG2E;
     p.thin_prefix = plan.thin_prefix;
     p.cut = plan.cut;
     p.workers = plan.blocks * PT_WARPS;

@@ -19,3 +19,14 @@ def test_misaligned_arrays_are_refused(L, what, field, which, off):  # noqa: F81
     got = dict(zip("awts", calls(L, d)))
     want = BAD if torch.cuda.is_available() else L.ERR_NO_DEVICE
     assert all(got[c] == want for c in which), got
+
+
+@pytest.mark.parametrize("scale,fine", [(3e38, False), (-3e38, False), (2.4e38, False), (2.3e38, True), (-2.3e38, True), (1e-45, True)])
+def test_scales_whose_exponents_overflow_are_refused(L, scale, fine):  # noqa: F811
+    """exp(scale * x) is taken as a power of two: scale * log2(e) has to be a number."""
+    import torch
+    d = good(L)
+    d["queries"].scale = scale
+    got = calls(L, d)
+    want = BAD if not fine or torch.cuda.is_available() else L.ERR_NO_DEVICE
+    assert got[1] == got[2] == want
