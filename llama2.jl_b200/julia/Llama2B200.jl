@@ -168,6 +168,12 @@ function sample_next(s::B200RunState, temperature::Float32, top_k::Int, top_p::F
     return Int(next[]) + 1
 end
 
+# One iteration with cuts: the logits stay on the device.
+function decode_next(s::B200RunState, token::Int, pos::Int, temperature::Float32, top_k::Int, top_p::Float32, min_p::Float32)
+    check(ccall((:l2b_forward, LIB), Int32, (Ptr{Cvoid}, Int32, Int32, Ptr{Float32}), s.session, token - 1, pos - 1, C_NULL))
+    return sample_next(s, temperature, top_k, top_p, min_p)
+end
+
 # The iterations of that loop whose next token is a prompt token (src/inference.jl:349-356), as one call: tokens at
 # positions 1..length(tokens) (the library streams the weights once for two positions where it can).
 function prefill!(s::B200RunState, tokens::Vector{Int})
@@ -223,8 +229,7 @@ function sample(
     end
     for pos in first_pos:limit
         if temperature != 0f0 && (top_k > 0 || top_p < 1f0 || min_p > 0f0)
-            transformer!(token, pos, config, state, model.weights)
-            next = sample_next(state, temperature, top_k, top_p, min_p)
+            next = decode_next(state, token, pos, temperature, top_k, top_p, min_p)
         else
             next = decode_next(state, token, pos, temperature)
         end

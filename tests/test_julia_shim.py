@@ -84,3 +84,14 @@ def test_config_struct_matches_the_c_struct(pkg):
     fields = re.findall(r"([a-z_]+)::(Int32|Float32|NTuple\{7,Int32\})", body)
     want = [(n, {C.c_int32: "Int32", C.c_float: "Float32"}.get(t, "NTuple{7,Int32}")) for n, t in L.Config._fields_]
     assert fields == want
+
+
+def test_sampling_with_cuts_copies_no_logits():
+    """A position of `sample` brings one token to the host: l2b_forward without a place for the logits, then l2b_session_sample."""
+    src = open(SHIM).read()
+    body = src[src.index("function sample("):]
+    assert "transformer!(" not in body and "s.logits" not in body
+    step = src[src.index("function decode_next(s::B200RunState, token::Int, pos::Int, temperature::Float32, top_k::Int"):]
+    step = step[:step.index("\nend")]
+    assert re.search(r"l2b_forward.*C_NULL\)", step) and "sample_next(s, temperature, top_k, top_p, min_p)" in step
+    assert "decode_next(state, token, pos, temperature, top_k, top_p, min_p)" in body
