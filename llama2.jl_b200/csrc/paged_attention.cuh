@@ -89,8 +89,8 @@ __device__ __forceinline__ uint32_t split_pair(float& a, float& b) {
 
 // What the exponents of weights are counted from: the maximum, less `up`.  bf16 has f32's range, but f16's terms stop at steps of 2^-24: behind a maximum of 1, weights of
 // 2^-20 would keep four bits, and many such keys may be all there is in a result whose largest weight has a value near zero.  With weights up to 2^15 the steps end at
-// 2^-39 of the largest here; behind a prefix, whose reference may lag by 2^6, at 2^-33 (a lag of 2^4 would make it 2^-35 and 128 rows behind 16 000 positions 135 us
-// instead of 128, one of 2 149).  Totals and sums carry the factor; a row's partial results say what they are counted from.  (Beyond 2^23 the difference would not be exact.)
+// 2^-39 of the largest.  Behind a prefix the reference may lag: by 2 for f32 rows, which leaves 2^-38; by 2^6 for 16-bit ones, 2^-33 (128 rows behind 16 000 positions: 128 us;
+// with a lag of 2^4 135, of 2 149).  Totals and sums carry the factor; a row's partial results say what they are counted from.  (Beyond 2^23 the difference would not be exact.)
 __device__ __forceinline__ float weight_reference(float mx, float up) { return fabsf(mx) < 8388608.f ? mx - up : mx; }
 
 // KS: steps of 16 values of a head, NT: tiles of 8 rows

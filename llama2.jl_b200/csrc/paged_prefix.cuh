@@ -12,7 +12,7 @@
 //   warps 8, 10     issue a stream's products each: P V of a step, then Q K^T of the step that gets its buffer
 //   warp 9          TMA copies of keys and values straight from the pages: 8 rows or more at a time, V's rows behind the prefix's end through a map
 //                   that ends there, so that they are zeros; pages that are none lie outside the map and are zeros, too
-// Rows are rescaled only when a maximum has grown by more than 2^8 (f16: 2^6), and then all 32 of a warp.  The work, items (key/value head, row tile) of the prefix' key tiles, is cut
+// Rows are rescaled only when a maximum has grown by more than 2^8 (f16 caches: 2^6, f32 rows over them: 2), and then all 32 of a warp.  The work, items (key/value head, row tile) of the prefix' key tiles, is cut
 // into equal shares of a block per SM (paged.h).  Every wait is bounded; a block whose wait ran out leaves NaN.
 // Measured: 128 rows of 64 heads over 8 x 16 000 keys of 128 values (65.5 GFLOP) in 77 us of the 116, 0.86 PFLOP/s; bound by the chain scores - maximum - exponentials of
 // a stream and the exponentials' rate.
@@ -38,7 +38,7 @@ template <typename T, typename TIO, int TILES>
 struct PrefixTraits {
     static constexpr bool WIDE = sizeof(TIO) == 4, F16 = std::is_same<T, __half>::value;
     static constexpr int QT = !WIDE ? 1 : F16 ? 2 : 3, PT = WIDE ? QT : 2;  // terms of Q and of P
-    static constexpr float UP = F16 ? 9.f : 0.f, GROWTH = F16 ? 6.f : 8.f;  // weights up to 2^(UP + GROWTH) (weight_reference)
+    static constexpr float UP = !F16 ? 0.f : WIDE ? 14.f : 9.f, GROWTH = !F16 ? 8.f : WIDE ? 1.f : 6.f;  // weights up to 2^(UP + GROWTH) (weight_reference)
     static constexpr int KEYS = WIDE ? 64 : 128, STEPS = KEYS / 64, BUFFERS = STEPS;  // steps of 64 keys of a tile, buffers of a stream's scores
     static constexpr int SUB_Q = PX_ROWS * 128, SUB_K = KEYS * 128;  // bytes of 64 values of a tile's rows
     // bytes of Q's place: its terms, or 4 KB for each of the eight warps that take the sums out
