@@ -232,3 +232,12 @@ def test_a_workspace_of_more_than_64_gib(L):
     tol = 2.0 ** -14 * size + 2.0 ** -8 * want.abs()
     bad = ((err > tol).any(-1).any(-1)).nonzero()
     assert len(bad) == 0, (len(bad), rows[bad[0]])
+
+
+@pytest.mark.parametrize("io,cache", TYPES)
+@pytest.mark.parametrize("n_query,counts,lengths,prefix", [(300, [300, 257, 1], [300, 1000, 40], 0), (701, [701, 0], [1402, 9], 333)])
+def test_attention_of_prompts(L, io, cache, n_query, counts, lengths, prefix):
+    """Hundreds of new tokens a sequence, with and without positions before them."""
+    from test_gpu_paged import check_attention
+    b = Batch(L, lengths, n_query=n_query, counts=counts, kv=2, hs=64, page=16, prefix=prefix, cache=cache, seed=n_query)
+    check_attention(b, queries(b, 4, io), 4)
