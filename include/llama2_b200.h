@@ -364,7 +364,9 @@ typedef struct l2b_paged_queries {
     int32_t reserved;
 } l2b_paged_queries;
 /* attention_weights! + scale + softmax! + combine_values! (src/inference.jl:263-278) of every new token over the prefix and over its sequence's own
- * positions up to its own (the last of dev_counts[i] tokens sees dev_lengths[i] of them).  A token that sees nothing gets zeros.
+ * positions up to its own (the last of dev_counts[i] tokens sees dev_lengths[i] of them).  A token that sees nothing gets zeros.  Scores, weights and sums
+ * keep more bits than the rows' type; results are rounded once.  Keys or values that are infinite may make the results of tokens that see them NaN, and of no others.  So
+ * does a copy inside the kernels that does not arrive within its bounded wait: its rows get NaN, there is no other report.
  * The workspace (at least l2b_paged_attention_workspace bytes, on a 16-byte boundary; any contents) is written while the call runs: calls that may run
  * at the same time take different ones, captured calls too. */
 int32_t l2b_paged_attention_workspace(const l2b_paged_cache* cache, const l2b_paged_batch* batch, const l2b_paged_queries* queries, int64_t* bytes);
@@ -378,8 +380,9 @@ int32_t l2b_paged_attention_device(const l2b_paged_cache* cache, const l2b_paged
  *   top_p < 1 keeps those of them before which less than top_p of their whole mass lies; 1 and more: no cut;
  *   min_p > 0 keeps those with w_i >= min_p (more than 1 counts as 1);
  *   the first one is always kept.
- * The token is the first, by index, at which the kept tokens' cumulated mass exceeds uniform times their whole (computed so that the result hangs on the
- * row alone).  T <= 0: argmax, first of equals.  Logits that are -inf or no numbers are never chosen; a row without any other gets token -1 and
+ * The token is the first, by index, at which the kept tokens' cumulated mass exceeds uniform times their whole.  Masses are whole multiples of 2^-44 of the largest
+ * weight, so that the result hangs on the row alone: a weight below half of that counts as 0, and the border of a nucleus or of a token may lie off by
+ * vocab * 2^-45 of the largest weight.  T <= 0: argmax, first of equals.  Logits that are -inf or no numbers are never chosen; a row without any other gets token -1 and
  * probability 0.  Several +inf share the mass equally. */
 typedef struct l2b_sampling {
     int32_t type;                 /* of the logits: L2B_TYPE_F32, L2B_TYPE_F16 or L2B_TYPE_BF16 */

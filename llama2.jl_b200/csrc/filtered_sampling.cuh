@@ -5,6 +5,7 @@
 //
 // A cluster of up to eight blocks holds a row in its shared memory, read once; every pass after that is over shared memory.  Masses are whole numbers of
 // 2^-44 of the largest weight (weights computed in 64 bits), so that sums do not depend on their order and no cut or choice hangs on the blocks or on atomics.
+// (The whole of a row is below 2^63 then.  Weights below half a unit are none; a border may lie off by half a unit a logit, 1.1e-8 of the largest weight for 393 216.)
 //   top-k up to FS_FAST: every block takes its share of the k-th place among its threads' maxima, so that the lowest of the blocks' values has at least k
 //     values that are no smaller; those few go to the first block, which does the rest alone while the others leave.
 //   other cuts: equal bins of the distance from the maximum are counted, or weighed; only the bin with the k-th value, or the nucleus' border, is listed and
@@ -12,8 +13,10 @@
 //   the choice: masses of stretches of the row, then inside the stretch that holds it.
 // Blocks write what the others need into the others' shared memory in front of a barrier, so that it is at hand behind it; nothing is fetched from a block
 // after the last barrier, so blocks leave at once.
-// Passes that compare take four logits at a time.  A pass that weighs all logits is bound by 64-bit arithmetic (about 40 issue slots per logit and
-// scheduler); with a cut below it the kept logits are collected 32 at a time first.  With a top-k the barriers are what is left over the logits' read.
+// Passes that compare take four logits at a time.  With a cut below it the kept logits are collected 32 at a time before they are weighed.  A pass that weighs all
+// logits is bound by issue slots: 200 rows of 32 000 logits with top-p alone are 181 warp instructions per 32 logits, the ALU 44 % and the 64-bit pipe 12 % busy; the 400
+// blocks find 296 places, so that the schedulers issue 65 % of the time and the busiest 98 %.  With a top-k it is the three barriers (the first arrived at early) and
+// the dependent passes between them that are left over the logits' read.
 // Measured: a row of 128 256 f32 logits with top-k 40 and top-p 0.95 in 10.5 us, 64 such rows in 32 us; 200 rows of 32 000 bf16 logits with top-p alone in 67 us.
 #pragma once
 #include <cfloat>

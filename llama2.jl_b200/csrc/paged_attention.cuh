@@ -10,8 +10,8 @@
 // run ahead over the ends of items; the page of a tile's keys is looked up one tile before it is needed, and the lengths of 32 sequences at a time.  Rows
 // of keys and values lie 16 bytes further apart in shared memory than they are long, so that ldmatrix reads eight rows without bank conflicts.
 //
-// Measured: 24 sequences of up to 4001 positions, 24 heads of 96 f16 values, nothing shared (661 MB): 99 us with the join, 0.77 of the copy rate; one sequence of 501
-// positions: 7.6 us and 3.8 for the join, chains of look-ups.
+// Measured: 24 sequences of up to 4001 positions, 24 heads of 96 f16 values, nothing shared (496 MB): 98 to 104 us with the join from one run to another, 0.73 to 0.78 of the
+// copy rate; one sequence of 501 positions: 7.6 us and 3.8 for the join, chains of look-ups.
 //
 // f32 rows over a 16-bit cache: a query and a weight are split into terms of the cache's type (three of bf16, two of f16, the query's behind a power of two
 // per row), which keeps the products' error at 2^-22 or less.  For 16-bit rows a weight is two terms (bf16: off by 2^-15 at most, f16: by 2^-22): rounded once

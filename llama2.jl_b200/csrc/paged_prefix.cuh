@@ -7,15 +7,15 @@
 //   TILES = 1: one row tile, the streams take the tiles of keys in turn and leave a partial result each: for few rows, and for f32 rows, whose three (f16: two)
 //              terms of Q take the place of a second tile (64 keys a tile).
 // The scores come in steps of 64 keys.  16-bit rows have two buffers of them, so that the next step's Q K^T is done before this step's exponentials are: with one
-// buffer of 128 keys a stream waited 2000 of 3900 cycles per tile for its products, and attention behind 16 000 positions took 128 us instead of 116.
+// buffer of 128 keys a stream waited 2000 of 3900 cycles per tile for its products (P was one term then: attention behind 16 000 positions took 128 us instead of 116).
 //   warps 0-3, 4-7  the streams' softmax; before it they bring the block's rows of Q into shared memory, after it the sums to the workspace
 //   warps 8, 10     issue a stream's products each: P V of a step, then Q K^T of the step that gets its buffer
 //   warp 9          TMA copies of keys and values straight from the pages: 8 rows or more at a time, V's rows behind the prefix's end through a map
 //                   that ends there, so that they are zeros; pages that are none lie outside the map and are zeros, too
 // Rows are rescaled only when a maximum has grown by more than 2^8 (f16 caches: 2^6, f32 rows over them: 2), and then all 32 of a warp.  The work, items (key/value head, row tile) of the prefix' key tiles, is cut
 // into equal shares of a block per SM (paged.h).  Every wait is bounded; a block whose wait ran out leaves NaN.
-// Measured: 128 rows of 64 heads over 8 x 16 000 keys of 128 values (65.5 GFLOP) in 77 us of the 116, 0.86 PFLOP/s; bound by the chain scores - maximum - exponentials of
-// a stream and the exponentials' rate.
+// Measured: 128 rows of 64 heads over 8 x 16 000 keys of 128 values (67.1 GFLOP) in about 94 us of the 134, 0.71 PFLOP/s; the tensor pipe, for which P's second term is half as
+// much again, is 63 % active, the exponential unit 43 %: bound by a stream's chain scores - maximum - exponentials - terms, whose phases overlap in part.
 #pragma once
 #include "paged_attention.cuh"
 #include "tcgen05.cuh"

@@ -368,8 +368,9 @@ extern "C" int32_t l2b_paged_attention_device(const l2b_paged_cache* cache, cons
         L2B_TRY(plan.tile_rows == 8 ? size(std::integral_constant<int, 1>()) : size(std::integral_constant<int, 2>()));
         JoinParams j;
         j.a = p;
-        // A warp per row once there are rows for a few warps on every SM, else the block's eight share one.  (2 048 rows: 58 us of a call with a warp each, 59 with four;
-        // 8 192 rows: 116 with one, 134 with four; one row's 16 parts want them.)
+        // A warp per row once there are rows for a few warps on every SM, else the block's eight share one.  Whole calls, eight warps / one, 32 heads of 128 values: own
+        // positions alone (1 500 each) 256 rows 16.8 / 22.8 us, 768 31.5 / 31.3, 1 024 37.5 / 36.0, 2 048 59.4 / 51.4; behind a prefix of 6 001, whose parts are
+        // more, 256 rows 33 / 40, 768 42 / 48, 1 024 47 / 51, 1 536 55 / 54, 2 048 64 / 60.  The border lies between the two kinds'.
         j.heads = n_rows >= 1024 ? PJ_WARPS : 1;
         const dim3 grid((unsigned)(p.seqs.n_seq * p.seqs.n_query), (unsigned)((p.n_heads + j.heads - 1) / j.heads));
         CU(launch_kernel(paged_join_kernel<TIO>, grid, dim3(PJ_WARPS * 32), 0, st, true, j));
