@@ -365,8 +365,10 @@ typedef struct l2b_paged_queries {
 } l2b_paged_queries;
 /* attention_weights! + scale + softmax! + combine_values! (src/inference.jl:263-278) of every new token over the prefix and over its sequence's own
  * positions up to its own (the last of dev_counts[i] tokens sees dev_lengths[i] of them).  A token that sees nothing gets zeros.  Scores, weights and sums
- * keep more bits than the rows' type; results are rounded once.  Keys or values that are infinite may make the results of tokens that see them NaN, and of no others.  So
- * does a copy inside the kernels that does not arrive within its bounded wait: its rows get NaN, there is no other report.
+ * keep more bits than the rows' type; results are rounded once.  Keys or values that are infinite may make the results of tokens that see them NaN, and of
+ * no others.  So does a copy inside the kernels that does not arrive within its bounded wait: its rows get NaN, there is no other report.
+ * Made for few new tokens of a sequence at a time: hundreds are right, but their own positions go through tiles of 16 rows (12 000 tokens of 64 heads of
+ * 128 values: 38 ms).
  * The workspace (at least l2b_paged_attention_workspace bytes, on a 16-byte boundary; any contents) is written while the call runs: calls that may run
  * at the same time take different ones, captured calls too. */
 int32_t l2b_paged_attention_workspace(const l2b_paged_cache* cache, const l2b_paged_batch* batch, const l2b_paged_queries* queries, int64_t* bytes);

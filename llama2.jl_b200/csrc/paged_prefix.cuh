@@ -12,8 +12,8 @@
 //   warps 8, 10     issue a stream's products each: P V of a step, then Q K^T of the step that gets its buffer
 //   warp 9          TMA copies of keys and values straight from the pages: 8 rows or more at a time, V's rows behind the prefix's end through a map
 //                   that ends there, so that they are zeros; pages that are none lie outside the map and are zeros, too
-// Rows are rescaled only when a maximum has grown by more than 2^8 (f16 caches: 2^6, f32 rows over them: 2), and then all 32 of a warp.  The work, items (key/value head, row tile) of the prefix' key tiles, is cut
-// into equal shares of a block per SM (paged.h).  Every wait is bounded; a block whose wait ran out leaves NaN.
+// Rows are rescaled only when a maximum has grown by more than 2^8 (f16 caches: 2^6, f32 rows over them: 2), and then all 32 of a warp.  The work, items (key/value
+// head, row tile) of the prefix' key tiles, is cut into equal shares of a block per SM (paged.h).  Every wait is bounded; a block whose wait ran out leaves NaN.
 // Measured: 128 rows of 64 heads over 8 x 16 000 keys of 128 values (67.1 GFLOP): a call takes 124 us with keys and values in the cache, 132 to 134 with new ones, of which own
 // parts 24 and the join 14; what is left, 86 to 94, is 0.71 to 0.78 PFLOP/s.  The tensor pipe, for which P's second term is half as much again, is 63 % active, the
 // exponential unit 43 %: bound by a stream's chain scores - maximum - exponentials - terms, whose phases overlap in part.
